@@ -1,4 +1,5 @@
-"""ctypes binding of libdeltacore.so (the C ABI declared in include/deltacore.h).
+"""ctypes binding of libdeltacore.so (the C ABI declared in include/deltacore.h and
+include/deltacore_layers.h).
 
 The library is loaded from this package directory and nowhere else.  There is
 no fallback: if the library is missing the import of the binding raises.
@@ -46,6 +47,18 @@ EXPORTS = (
     "dc_chunk_fwd_out_norm_fused",
     "dc_qkv_prologue",
     "dc_gates",
+    "dc_rms_norm",
+    "dc_rms_norm_bwd_workspace_size",
+    "dc_rms_norm_bwd",
+    "dc_causal_conv",
+    "dc_causal_conv_bwd_workspace_size",
+    "dc_causal_conv_bwd",
+    "dc_selective_scan_checkpoint_size",
+    "dc_selective_scan_workspace_size",
+    "dc_selective_scan",
+    "dc_selective_scan_step",
+    "dc_selective_scan_bwd_workspace_size",
+    "dc_selective_scan_bwd",
 )
 
 
@@ -139,6 +152,99 @@ class GateArgs(ctypes.Structure):
     ]
 
 
+# include/deltacore_layers.h
+DC_E4M3 = 2
+DC_RMS_MAX_WIDTH = 16384
+DC_CONV_MAX_TAPS = 8
+DC_SCAN_MAX_STATE = 64
+DC_CONV_SILU = 0x1
+DC_SCAN_SOFTPLUS = 0x1
+
+
+class RmsNormArgs(ctypes.Structure):
+    """struct dc_rms_norm_args."""
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("width", ctypes.c_int64), ("x_stride", ctypes.c_int64),
+        ("residual_in_stride", ctypes.c_int64), ("residual_out_stride", ctypes.c_int64),
+        ("y_stride", ctypes.c_int64), ("x_dtype", ctypes.c_int32), ("residual_dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32), ("group", ctypes.c_int32), ("eps", ctypes.c_float),
+        ("x", ctypes.c_void_p), ("residual_in", ctypes.c_void_p), ("weight", ctypes.c_void_p),
+        ("residual_out", ctypes.c_void_p), ("y", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+    ]
+
+
+class RmsNormBwdArgs(ctypes.Structure):
+    """struct dc_rms_norm_bwd_args."""
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("width", ctypes.c_int64), ("d_y_stride", ctypes.c_int64),
+        ("d_r_stride", ctypes.c_int64), ("r_stride", ctypes.c_int64), ("d_x_stride", ctypes.c_int64),
+        ("d_residual_stride", ctypes.c_int64), ("y_dtype", ctypes.c_int32), ("r_dtype", ctypes.c_int32),
+        ("x_dtype", ctypes.c_int32), ("eps", ctypes.c_float), ("d_y", ctypes.c_void_p),
+        ("d_r", ctypes.c_void_p), ("r", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("d_x", ctypes.c_void_p),
+        ("d_residual", ctypes.c_void_p), ("d_weight", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class CausalConvArgs(ctypes.Structure):
+    """struct dc_causal_conv_args."""
+    _fields_ = [
+        ("batch", ctypes.c_int64), ("seq", ctypes.c_int64), ("channels", ctypes.c_int64),
+        ("x_batch_stride", ctypes.c_int64), ("x_token_stride", ctypes.c_int64),
+        ("y_batch_stride", ctypes.c_int64), ("y_token_stride", ctypes.c_int64), ("taps", ctypes.c_int32),
+        ("in_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32), ("flags", ctypes.c_uint32),
+        ("x", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+        ("window_in", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("y", ctypes.c_void_p),
+        ("window_out", ctypes.c_void_p),
+    ]
+
+
+class CausalConvBwdArgs(ctypes.Structure):
+    """struct dc_causal_conv_bwd_args."""
+    _fields_ = [
+        ("batch", ctypes.c_int64), ("seq", ctypes.c_int64), ("channels", ctypes.c_int64),
+        ("x_batch_stride", ctypes.c_int64), ("x_token_stride", ctypes.c_int64),
+        ("d_y_batch_stride", ctypes.c_int64), ("d_y_token_stride", ctypes.c_int64),
+        ("d_x_batch_stride", ctypes.c_int64), ("d_x_token_stride", ctypes.c_int64), ("taps", ctypes.c_int32),
+        ("in_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32), ("flags", ctypes.c_uint32),
+        ("d_y", ctypes.c_void_p), ("d_window_out", ctypes.c_void_p), ("x", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("window_in", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p), ("d_x", ctypes.c_void_p), ("d_weight", ctypes.c_void_p),
+        ("d_bias", ctypes.c_void_p), ("d_window_in", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class SelectiveScanArgs(ctypes.Structure):
+    """struct dc_selective_scan_args."""
+    _fields_ = [
+        ("batch", ctypes.c_int64), ("seq", ctypes.c_int64), ("channels", ctypes.c_int64),
+        ("state", ctypes.c_int64), ("groups", ctypes.c_int64), ("u_batch_stride", ctypes.c_int64),
+        ("u_token_stride", ctypes.c_int64), ("dt_batch_stride", ctypes.c_int64),
+        ("dt_token_stride", ctypes.c_int64), ("z_batch_stride", ctypes.c_int64),
+        ("z_token_stride", ctypes.c_int64), ("b_batch_stride", ctypes.c_int64),
+        ("b_token_stride", ctypes.c_int64), ("c_batch_stride", ctypes.c_int64),
+        ("c_token_stride", ctypes.c_int64), ("y_batch_stride", ctypes.c_int64),
+        ("y_token_stride", ctypes.c_int64), ("in_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32),
+        ("flags", ctypes.c_uint32), ("u", ctypes.c_void_p), ("dt", ctypes.c_void_p), ("a", ctypes.c_void_p),
+        ("b", ctypes.c_void_p), ("c", ctypes.c_void_p), ("d", ctypes.c_void_p), ("z", ctypes.c_void_p),
+        ("dt_bias", ctypes.c_void_p), ("state_in", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+        ("y", ctypes.c_void_p), ("state_out", ctypes.c_void_p), ("checkpoints", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class SelectiveScanBwdArgs(ctypes.Structure):
+    """struct dc_selective_scan_bwd_args."""
+    _fields_ = [
+        ("fwd", SelectiveScanArgs), ("d_y_batch_stride", ctypes.c_int64), ("d_y_token_stride", ctypes.c_int64),
+        ("d_y", ctypes.c_void_p), ("d_state_out", ctypes.c_void_p), ("d_u", ctypes.c_void_p),
+        ("d_dt", ctypes.c_void_p), ("d_a", ctypes.c_void_p), ("d_b", ctypes.c_void_p), ("d_c", ctypes.c_void_p),
+        ("d_d", ctypes.c_void_p), ("d_z", ctypes.c_void_p), ("d_dt_bias", ctypes.c_void_p),
+        ("d_state_in", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
 _lib = None
 
 
@@ -188,6 +294,16 @@ def lib() -> ctypes.CDLL:
         L.dc_qkv_prologue.restype = ctypes.c_int
         L.dc_gates.argtypes = [ctypes.POINTER(GateArgs), ctypes.c_void_p]
         L.dc_gates.restype = ctypes.c_int
+        for name, args in (("dc_rms_norm", RmsNormArgs), ("dc_rms_norm_bwd", RmsNormBwdArgs), ("dc_causal_conv", CausalConvArgs),
+                           ("dc_causal_conv_bwd", CausalConvBwdArgs), ("dc_selective_scan", SelectiveScanArgs),
+                           ("dc_selective_scan_step", SelectiveScanArgs), ("dc_selective_scan_bwd", SelectiveScanBwdArgs)):
+            fn = getattr(L, name)
+            fn.argtypes, fn.restype = [ctypes.POINTER(args), ctypes.c_void_p], ctypes.c_int
+        for name, args in (("dc_rms_norm_bwd_workspace_size", RmsNormBwdArgs), ("dc_causal_conv_bwd_workspace_size", CausalConvBwdArgs),
+                           ("dc_selective_scan_checkpoint_size", SelectiveScanArgs), ("dc_selective_scan_workspace_size", SelectiveScanArgs),
+                           ("dc_selective_scan_bwd_workspace_size", SelectiveScanBwdArgs)):
+            fn = getattr(L, name)
+            fn.argtypes, fn.restype = [ctypes.POINTER(args)], ctypes.c_uint64
         _lib = L
     return _lib
 

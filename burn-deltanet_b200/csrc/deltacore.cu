@@ -24,6 +24,7 @@
 #include "out_norm.cuh"
 #include "prologue.cuh"
 #include "common.cuh"
+#include "host.hpp"
 #include "step.cuh"
 #include "step_stream.cuh"
 
@@ -263,6 +264,16 @@ int validate_step(const dc_step_args *a) {
 }
 
 }  // namespace
+
+namespace dc {
+namespace host {
+
+int cuda_fail(cudaError_t e) { return ::cuda_fail(e); }
+int check_device() { return ::check_device(nullptr); }
+int sm_count() { return ::sm_count(); }
+
+}  // namespace host
+}  // namespace dc
 
 extern "C" {
 

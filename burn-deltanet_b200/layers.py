@@ -1,0 +1,513 @@
+"""The operators around the token mixers of a block stack, over the C ABI of include/deltacore_layers.h.
+
+* :func:`add_rms_norm`, :func:`add_rms_norm_f8`, :func:`add_rms_norm_backward` — the residual stream's addition and the RMS
+  norm of the sum, in float32 / bfloat16 or in 8 bits (e4m3) with scales;
+* :func:`causal_conv`, :func:`causal_conv_step`, :func:`causal_conv_backward` — the short causal depthwise convolution;
+* :func:`selective_scan`, :func:`selective_scan_step`, :func:`selective_scan_backward` — the selective state space scan;
+* :class:`AddRmsNormFunction`, :class:`CausalConvFunction`, :class:`SelectiveScanFunction` — their autograd nodes.
+
+They have no counterpart in burn-deltanet (the norm in front of a block is a Burn module there, and the selective scan is the
+diagonal relative of the delta rule that hybrid stacks interleave with it).  The manner is :mod:`.core`'s: CUDA tensors only,
+errors as :class:`~.core.DeltaCoreError` / :class:`~.core.DeltaShapeError`, work on the tensors' device and its current
+stream, outputs as new tensors unless given.  Inputs may be column slices of a projection where the text says so: the last
+axis contiguous, one stride per token.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _abi
+from .core import DeltaCoreError, DeltaShapeError, _raise
+
+_CODES = {torch.float32: _abi.DC_F32, torch.bfloat16: _abi.DC_BF16}
+
+
+def _code(dtype: torch.dtype, what: str) -> int:
+    code = _CODES.get(dtype)
+    if code is None:
+        raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"{what} has dtype {dtype}")
+    return code
+
+
+def _cuda(t: torch.Tensor, what: str, device: Optional[torch.device] = None) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise DeltaCoreError(_abi.DC_EDEVICE, f"{what} is on {t.device}: the delta-rule core runs on CUDA only")
+    if device is not None and t.device != device:
+        raise DeltaCoreError(_abi.DC_EDEVICE, f"{what} is on {t.device}, the other tensors on {device}")
+
+
+def _whole(t: Optional[torch.Tensor], what: str, shape, dtype: torch.dtype, device: torch.device):
+    """The address of a contiguous tensor of this shape and dtype (None: no address)."""
+    if t is None:
+        return None
+    _cuda(t, what, device)
+    if t.dtype != dtype:
+        raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"{what} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"{what} has shape {tuple(t.shape)}, want {tuple(shape)}")
+    if not t.is_contiguous():
+        raise DeltaCoreError(_abi.DC_EINVAL_ARG, f"{what} must be contiguous")
+    return t.data_ptr()
+
+
+def _row_stride(t: torch.Tensor, what: str) -> int:
+    """The one stride between the rows (all axes but the last) of `t`."""
+    width = t.shape[-1]
+    if t.is_contiguous():
+        return width
+    if t.stride(-1) != 1 and width > 1:
+        raise DeltaCoreError(_abi.DC_EINVAL_ARG, f"{what} must have a contiguous last axis")
+    stride, span = width, None
+    for size, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if span is None:
+            stride = st
+        elif st != span:
+            raise DeltaCoreError(_abi.DC_EINVAL_ARG, f"{what} must have one stride between its rows")
+        span = st * size
+    return stride
+
+
+def _strides(t: torch.Tensor, what: str, shape, dtype: torch.dtype, device: torch.device):
+    """(sequence stride, token stride) of a [batch, seq, channels] tensor with contiguous channels."""
+    _cuda(t, what, device)
+    if t.dtype != dtype:
+        raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"{what} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"{what} has shape {tuple(t.shape)}, want {shape}")
+    if t.stride(2) != 1 and shape[2] > 1:
+        raise DeltaCoreError(_abi.DC_EINVAL_ARG, f"{what} must have contiguous channels")
+    return t.stride(0), t.stride(1)
+
+
+def _call(fn, args, device: torch.device, what: str) -> None:
+    """Run a C entry point on `device`'s current stream."""
+    if torch.cuda.current_device() == device.index:
+        status = fn(args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            status = fn(args, torch.cuda.current_stream(device).cuda_stream)
+    if status:
+        _raise(status, what)
+
+
+def _workspace(size_fn, args, workspace: Optional[torch.Tensor], device: torch.device):
+    """Point `args` at a workspace of the size that `size_fn` asks for; returns the tensor, to be kept until the launch."""
+    if workspace is None:
+        if torch.cuda.current_device() == device.index:
+            need = int(size_fn(args))
+        else:
+            with torch.cuda.device(device):
+                need = int(size_fn(args))
+        if need == 0:
+            return None
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    else:
+        _cuda(workspace, "workspace", device)
+        if not workspace.is_contiguous():
+            raise DeltaCoreError(_abi.DC_EINVAL_ARG, "workspace must be contiguous")
+    args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return workspace
+
+
+# ------------------------------------------------------------------------------------------------ residual add + norm
+def _norm_args(x, weight, residual, eps, residual_dtype, residual_out):
+    """The fields that the two outputs' forms share; returns (args, residual_out or x)."""
+    _cuda(x, "x")
+    if x.dim() < 1:
+        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, "x must have at least one axis")
+    width, dev = x.shape[-1], x.device
+    a = _abi.RmsNormArgs()
+    a.rows, a.width = x.numel() // width if width else 0, width
+    a.eps = float(eps)
+    a.weight = _whole(weight, "weight", (width,), torch.float32, dev)
+    a.x, a.x_dtype, a.x_stride = x.data_ptr(), _code(x.dtype, "x"), _row_stride(x, "x")
+    r_dtype = residual_dtype or (residual.dtype if residual is not None else residual_out.dtype if residual_out is not None else x.dtype)
+    if residual is not None:
+        _cuda(residual, "residual", dev)
+        if residual.shape != x.shape:
+            raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"residual has shape {tuple(residual.shape)}, want {tuple(x.shape)}")
+        if residual.dtype != r_dtype:
+            raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"residual must be {r_dtype}, got {residual.dtype}")
+        a.residual_in, a.residual_in_stride = residual.data_ptr(), _row_stride(residual, "residual")
+    a.residual_dtype = _code(r_dtype, "residual")
+    if residual is None and residual_out is None and r_dtype == x.dtype:
+        return a, x  # the sum is x itself
+    if residual_out is None:
+        residual_out = torch.empty(x.shape, device=dev, dtype=r_dtype)
+    _cuda(residual_out, "residual_out", dev)
+    if residual_out.shape != x.shape or residual_out.dtype != r_dtype:
+        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"residual_out must be {r_dtype}, shaped like x")
+    a.residual_out, a.residual_out_stride = residual_out.data_ptr(), _row_stride(residual_out, "residual_out")
+    return a, residual_out
+
+
+def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-5, *,
+                 out_dtype: Optional[torch.dtype] = None, residual_dtype: Optional[torch.dtype] = None,
+                 y_out: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None):
+    """The residual stream's addition and the RMS norm of the sum (``dc_rms_norm``) over the last axis of ``x``:
+    ``s = x + residual``, ``y = s / sqrt(mean(s^2) + eps) * weight``.
+
+    ``x`` and ``residual`` (the same shape; ``None``: zero) are float32 or bfloat16 each; their rows may be column slices with
+    one stride.  ``weight`` is float32 ``[width]``.  Returns ``(y, r)``: ``y`` in ``out_dtype`` (default: ``x``'s), ``r`` the
+    sum in ``residual_dtype`` (default: ``residual``'s), the next layer's ``residual``; without a residual ``r`` is ``x``.
+    ``y`` is made from the sum before ``r``'s rounding.  ``residual_out`` may be ``residual`` and ``y_out`` may be ``x``.
+    """
+    a, r = _norm_args(x, weight, residual, eps, residual_dtype, residual_out)
+    y = y_out if y_out is not None else torch.empty(x.shape, device=x.device, dtype=out_dtype or x.dtype)
+    if y_out is not None:
+        _cuda(y, "y_out", x.device)
+        if y.shape != x.shape or (out_dtype is not None and y.dtype != out_dtype):
+            raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, "y_out must be shaped like x, in out_dtype")
+    a.y, a.out_dtype, a.y_stride = y.data_ptr(), _code(y.dtype, "y"), _row_stride(y, "y_out")
+    _call(_abi.lib().dc_rms_norm, a, x.device, "dc_rms_norm")
+    return y, r
+
+
+def add_rms_norm_f8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-5, *,
+                    group: int = 0, residual_dtype: Optional[torch.dtype] = None, residual_out: Optional[torch.Tensor] = None):
+    """:func:`add_rms_norm` with ``y`` in 8 bits: returns ``(q, scale, r)``, ``y = q * scale`` with ``q`` float8_e4m3fn shaped
+    like ``x`` and one float32 scale, ``max|y| / 448``, per ``group`` consecutive columns (32, 64, 128 or 256 dividing the
+    width; 0: per row).  ``scale`` is ``x``'s shape with the last axis ``width / group`` (1 per row)."""
+    a, r = _norm_args(x, weight, residual, eps, residual_dtype, residual_out)
+    width = x.shape[-1]
+    group = int(group)
+    if group not in (0, 32, 64, 128, 256):
+        raise DeltaShapeError(_abi.DC_EINVAL_WIDTH, f"group must be 0, 32, 64, 128 or 256, got {group}")
+    if group and width % group:
+        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"group {group} does not divide the width {width}")
+    q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
+    scale = torch.empty((*x.shape[:-1], width // group if group else 1), device=x.device, dtype=torch.float32)
+    a.y, a.out_dtype, a.y_stride, a.group, a.scale = q.data_ptr(), _abi.DC_E4M3, width, group, scale.data_ptr()
+    _call(_abi.lib().dc_rms_norm, a, x.device, "dc_rms_norm")
+    return q, scale, r
+
+
+def add_rms_norm_backward(d_y: torch.Tensor, d_r: Optional[torch.Tensor], r: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *,
+                          x_dtype: Optional[torch.dtype] = None, workspace: Optional[torch.Tensor] = None):
+    """The backward of :func:`add_rms_norm` (``dc_rms_norm_bwd``) from its ``r``: returns ``(d_x, d_residual, d_weight)``,
+    ``d_x`` in ``x_dtype`` (default: ``r``'s), ``d_residual`` in ``r``'s dtype (the same tensor where the dtypes are equal: the
+    two gradients are), ``d_weight`` float32.  ``d_r`` is the gradient of the returned sum, in ``r``'s dtype (``None``: zero)."""
+    _cuda(r, "r")
+    dev, width = r.device, r.shape[-1]
+    _cuda(d_y, "d_y", dev)
+    if d_y.shape != r.shape or (d_r is not None and d_r.shape != r.shape):
+        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, "d_y and d_r must be shaped like r")
+    a = _abi.RmsNormBwdArgs()
+    a.rows, a.width, a.eps = r.numel() // width if width else 0, width, float(eps)
+    a.weight = _whole(weight, "weight", (width,), torch.float32, dev)
+    a.r, a.r_dtype, a.r_stride = r.data_ptr(), _code(r.dtype, "r"), _row_stride(r, "r")
+    a.d_y, a.y_dtype, a.d_y_stride = d_y.data_ptr(), _code(d_y.dtype, "d_y"), _row_stride(d_y, "d_y")
+    if d_r is not None:
+        _cuda(d_r, "d_r", dev)
+        if d_r.dtype != r.dtype:
+            raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"d_r must be {r.dtype}, got {d_r.dtype}")
+        a.d_r, a.d_r_stride = d_r.data_ptr(), _row_stride(d_r, "d_r")
+    d_residual = torch.empty(r.shape, device=dev, dtype=r.dtype)
+    a.d_residual, a.d_residual_stride = d_residual.data_ptr(), width
+    d_x = d_residual
+    if x_dtype is not None and x_dtype != r.dtype:
+        d_x = torch.empty(r.shape, device=dev, dtype=x_dtype)
+        a.d_x, a.d_x_stride, a.x_dtype = d_x.data_ptr(), width, _code(x_dtype, "x_dtype")
+    d_weight = torch.empty(width, device=dev, dtype=torch.float32)
+    a.d_weight = d_weight.data_ptr()
+    L = _abi.lib()
+    keep = _workspace(L.dc_rms_norm_bwd_workspace_size, a, workspace, dev)
+    _call(L.dc_rms_norm_bwd, a, dev, "dc_rms_norm_bwd")
+    del keep
+    return d_x, d_residual, d_weight
+
+
+class AddRmsNormFunction(torch.autograd.Function):
+    """``y, r = AddRmsNormFunction.apply(x, weight, residual, eps)`` (only ``y`` without a residual): :func:`add_rms_norm` as an
+    autograd node.  It keeps the sum and the weight."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual=None, eps=1e-5):
+        y, r = add_rms_norm(x, weight, residual, eps)
+        ctx.save_for_backward(r, weight)
+        ctx.cfg = (eps, x.dtype, residual is not None)
+        return y if residual is None else (y, r)
+
+    @staticmethod
+    def backward(ctx, d_y, d_r=None):
+        r, weight = ctx.saved_tensors
+        eps, x_dtype, has_residual = ctx.cfg
+        d_x, d_residual, d_weight = add_rms_norm_backward(d_y.contiguous(), None if d_r is None else d_r.contiguous(), r, weight, eps,
+                                                          x_dtype=x_dtype)
+        return d_x, d_weight, d_residual if has_residual else None, None
+
+
+# ------------------------------------------------------------------------------------------------ causal convolution
+def _conv_args(a, x, weight, bias, window, silu, lengths):
+    """The forward's and the backward's common fields, for x [batch, seq, channels]."""
+    _cuda(x, "x")
+    if x.dim() != 3:
+        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"x must be [batch, seq, channels], got {tuple(x.shape)}")
+    b, s, c = x.shape
+    dev = x.device
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"weight must be [{c}, taps]")
+    k = weight.shape[1]
+    a.batch, a.seq, a.channels, a.taps = b, s, c, k
+    a.in_dtype = _code(x.dtype, "x")
+    a.flags = _abi.DC_CONV_SILU if silu else 0
+    a.x_batch_stride, a.x_token_stride = _strides(x, "x", (b, s, c), x.dtype, dev)
+    a.x = x.data_ptr()
+    a.weight = _whole(weight, "weight", (c, k), torch.float32, dev)
+    a.bias = _whole(bias, "bias", (c,), torch.float32, dev)
+    a.window_in = _whole(window, "window", (b, c, k), torch.float32, dev)
+    a.lengths = _whole(lengths, "lengths", (b,), torch.int32, dev)
+
+
+def causal_conv(x_bsc: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, window: Optional[torch.Tensor] = None, *,
+                silu: bool = True, lengths: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                y_out: Optional[torch.Tensor] = None, window_out: Optional[torch.Tensor] = None):
+    """The causal depthwise convolution of ``x [batch, seq, channels]`` (``dc_causal_conv``) with ``weight [channels, taps]``
+    (up to 8 taps) and ``bias``, then SiLU (``silu``): ``y_t = silu(bias + sum_j weight[:, j] x_{t - taps + 1 + j})``.
+
+    ``window [batch, channels, taps]`` (float32, ``None``: zeros) holds the tokens before the first in its last ``taps - 1``
+    columns, as :func:`~.core.qkv_prologue`'s does.  ``lengths`` (int32 ``[batch]``) ends each sequence early: the padding is
+    not read and its ``y`` is zero.  ``x`` may be a column slice.  Returns ``(y, next window)``.
+    """
+    a = _abi.CausalConvArgs()
+    _conv_args(a, x_bsc, weight, bias, window, silu, lengths)
+    b, s, c = x_bsc.shape
+    dev = x_bsc.device
+    y = y_out if y_out is not None else torch.empty(b, s, c, device=dev, dtype=out_dtype or x_bsc.dtype)
+    if out_dtype is not None and y.dtype != out_dtype:
+        raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"y_out must be {out_dtype}")
+    nxt = window_out if window_out is not None else torch.empty(b, c, weight.shape[1], device=dev, dtype=torch.float32)
+    a.y_batch_stride, a.y_token_stride = _strides(y, "y_out", (b, s, c), y.dtype, dev)
+    a.y, a.out_dtype = y.data_ptr(), _code(y.dtype, "y")
+    a.window_out = _whole(nxt, "window_out", (b, c, weight.shape[1]), torch.float32, dev)
+    _call(_abi.lib().dc_causal_conv, a, dev, "dc_causal_conv")
+    return y, nxt
+
+
+def causal_conv_step(x_bc: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, window: Optional[torch.Tensor] = None, *,
+                     silu: bool = True, out_dtype: Optional[torch.dtype] = None, y_out: Optional[torch.Tensor] = None,
+                     window_out: Optional[torch.Tensor] = None):
+    """:func:`causal_conv` for one token per sequence: ``x [batch, channels]`` to ``(y [batch, channels], next window)``; pass
+    ``window_out=window`` to roll the window in place."""
+    if not isinstance(x_bc, torch.Tensor) or x_bc.dim() != 2:
+        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, "x must be [batch, channels]")
+    y, nxt = causal_conv(x_bc.unsqueeze(1), weight, bias, window, silu=silu, out_dtype=out_dtype,
+                         y_out=None if y_out is None else y_out.unsqueeze(1), window_out=window_out)
+    return (y.squeeze(1) if y_out is None else y_out), nxt
+
+
+def causal_conv_backward(d_y: torch.Tensor, d_window_out: Optional[torch.Tensor], x_bsc: torch.Tensor, weight: torch.Tensor,
+                         bias: Optional[torch.Tensor] = None, window: Optional[torch.Tensor] = None, *, silu: bool = True,
+                         lengths: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None):
+    """The backward of :func:`causal_conv` (``dc_causal_conv_bwd``), given ``d_y`` and the gradient of the returned window
+    (``None``: zero): returns ``(d_x, d_weight, d_bias, d_window)``, ``d_x`` in ``x``'s dtype, the others float32; ``d_bias`` and
+    ``d_window`` are ``None`` where ``bias`` and ``window`` are."""
+    a = _abi.CausalConvBwdArgs()
+    _conv_args(a, x_bsc, weight, bias, window, silu, lengths)
+    b, s, c = x_bsc.shape
+    dev, k = x_bsc.device, weight.shape[1]
+    _cuda(d_y, "d_y", dev)
+    a.out_dtype = _code(d_y.dtype, "d_y")
+    a.d_y_batch_stride, a.d_y_token_stride = _strides(d_y, "d_y", (b, s, c), d_y.dtype, dev)
+    a.d_y = d_y.data_ptr()
+    a.d_window_out = _whole(d_window_out, "d_window_out", (b, c, k), torch.float32, dev)
+    d_x = torch.empty(b, s, c, device=dev, dtype=x_bsc.dtype)
+    d_weight = torch.empty(c, k, device=dev, dtype=torch.float32)
+    d_bias = None if bias is None else torch.empty(c, device=dev, dtype=torch.float32)
+    d_window = None if window is None else torch.empty(b, c, k, device=dev, dtype=torch.float32)
+    a.d_x, a.d_x_batch_stride, a.d_x_token_stride = d_x.data_ptr(), s * c, c
+    a.d_weight = d_weight.data_ptr()
+    a.d_bias = None if d_bias is None else d_bias.data_ptr()
+    a.d_window_in = None if d_window is None else d_window.data_ptr()
+    L = _abi.lib()
+    keep = _workspace(L.dc_causal_conv_bwd_workspace_size, a, workspace, dev)
+    _call(L.dc_causal_conv_bwd, a, dev, "dc_causal_conv_bwd")
+    del keep
+    return d_x, d_weight, d_bias, d_window
+
+
+class CausalConvFunction(torch.autograd.Function):
+    """``y, next_window = CausalConvFunction.apply(x, weight, bias, window, silu, lengths)``: :func:`causal_conv` as an autograd
+    node that keeps its inputs and recomputes the convolution in the backward."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias=None, window=None, silu=True, lengths=None):
+        y, nxt = causal_conv(x, weight, bias, window, silu=silu, lengths=lengths)
+        ctx.save_for_backward(x, weight, bias, window, lengths)
+        ctx.silu = silu
+        return y, nxt
+
+    @staticmethod
+    def backward(ctx, d_y, d_next):
+        x, weight, bias, window, lengths = ctx.saved_tensors
+        d_x, d_weight, d_bias, d_window = causal_conv_backward(d_y.contiguous(), d_next.contiguous(), x, weight, bias, window,
+                                                               silu=ctx.silu, lengths=lengths)
+        return d_x, d_weight, d_bias, d_window, None, None
+
+
+# ------------------------------------------------------------------------------------------------ selective scan
+def _bc(t, what, b, s, dtype, dev):
+    """(groups, state, sequence stride, token stride) of b or c: [batch, seq, groups, state] or [batch, seq, state]."""
+    _cuda(t, what, dev)
+    if t.dtype != dtype:
+        raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"{what} must be {dtype}, got {t.dtype}")
+    if t.dim() not in (3, 4) or t.shape[0] != b or t.shape[1] != s:
+        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"{what} has shape {tuple(t.shape)}, want [{b}, {s}, groups, state]")
+    g, n = (1, t.shape[2]) if t.dim() == 3 else t.shape[2:]
+    if (n > 1 and t.stride(-1) != 1) or (t.dim() == 4 and g > 1 and t.stride(2) != n):
+        raise DeltaCoreError(_abi.DC_EINVAL_ARG, f"{what} must have contiguous [groups, state]")
+    return g, n, t.stride(0), t.stride(1)
+
+
+def _scan_args(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths):
+    """dc_selective_scan_args but for the outputs, for u [batch, seq, channels]."""
+    _cuda(u, "u")
+    if u.dim() != 3:
+        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"u must be [batch, seq, channels], got {tuple(u.shape)}")
+    bs, s, ch = u.shape
+    dev, dtype = u.device, u.dtype
+    g = _abi.SelectiveScanArgs()
+    g.in_dtype = _code(dtype, "u")
+    groups, n, g.b_batch_stride, g.b_token_stride = _bc(b, "b", bs, s, dtype, dev)
+    groups_c, n_c, g.c_batch_stride, g.c_token_stride = _bc(c, "c", bs, s, dtype, dev)
+    if (groups_c, n_c) != (groups, n):
+        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"c has [groups, state] {(groups_c, n_c)}, b {(groups, n)}")
+    g.batch, g.seq, g.channels, g.state, g.groups = bs, s, ch, n, groups
+    g.u_batch_stride, g.u_token_stride = _strides(u, "u", (bs, s, ch), dtype, dev)
+    g.dt_batch_stride, g.dt_token_stride = _strides(dt, "dt", (bs, s, ch), dtype, dev)
+    if z is not None:
+        g.z_batch_stride, g.z_token_stride = _strides(z, "z", (bs, s, ch), dtype, dev)
+        g.z = z.data_ptr()
+    g.flags = _abi.DC_SCAN_SOFTPLUS if softplus else 0
+    g.u, g.dt, g.b, g.c = u.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr()
+    g.a = _whole(a, "a", (ch, n), torch.float32, dev)
+    g.d = _whole(d, "d", (ch,), torch.float32, dev)
+    g.dt_bias = _whole(dt_bias, "dt_bias", (ch,), torch.float32, dev)
+    g.state_in = _whole(state, "state", (bs, ch, n), torch.float32, dev)
+    g.lengths = _whole(lengths, "lengths", (bs,), torch.int32, dev)
+    return g
+
+
+def _scan_outputs(g, u, out_dtype, y_out, state_out):
+    dev = u.device
+    shape = (g.batch, g.seq, g.channels)
+    y = y_out if y_out is not None else torch.empty(shape, device=dev, dtype=out_dtype or u.dtype)
+    if out_dtype is not None and y.dtype != out_dtype:
+        raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"y_out must be {out_dtype}")
+    h = state_out if state_out is not None else torch.empty(g.batch, g.channels, g.state, device=dev, dtype=torch.float32)
+    g.y_batch_stride, g.y_token_stride = _strides(y, "y_out", shape, y.dtype, dev)
+    g.y, g.out_dtype = y.data_ptr(), _code(y.dtype, "y")
+    g.state_out = _whole(h, "state_out", (g.batch, g.channels, g.state), torch.float32, dev)
+    return y, h
+
+
+def selective_scan(u: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, d: Optional[torch.Tensor] = None,
+                   z: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None, *,
+                   softplus: bool = True, lengths: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                   checkpoints: bool = False, y_out: Optional[torch.Tensor] = None, state_out: Optional[torch.Tensor] = None,
+                   workspace: Optional[torch.Tensor] = None):
+    """The selective state space scan over a prompt (``dc_selective_scan``).  Per sequence and channel, with a state ``h`` of
+    ``state`` values::
+
+        step = softplus(dt + dt_bias)
+        h    = exp(step * a) * h + step * u * b
+        y    = (c . h + d * u) * silu(z)
+
+    ``u``, ``dt`` and ``z`` are ``[batch, seq, channels]``, ``b`` and ``c`` ``[batch, seq, groups, state]`` (or ``[batch, seq,
+    state]``; channel ``i`` reads group ``i // (channels / groups)``), all of one dtype, float32 or bfloat16, and any of them may
+    be a column slice.  ``a [channels, state]``, ``d``, ``dt_bias [channels]`` and ``state [batch, channels, state]`` are float32;
+    ``d``, ``z``, ``dt_bias`` and ``state`` may be ``None``.  ``lengths`` (int32 ``[batch]``) ends each sequence early.  Returns
+    ``(y, final state)``, with ``checkpoints=True`` also what :func:`selective_scan_backward` starts from.  ``state_out`` may be
+    ``state``; ``softplus=False`` takes ``dt + dt_bias`` as it is.
+    """
+    g = _scan_args(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths)
+    y, h = _scan_outputs(g, u, out_dtype, y_out, state_out)
+    L = _abi.lib()
+    saved = None
+    if checkpoints:
+        saved = torch.empty(int(L.dc_selective_scan_checkpoint_size(g)) // 4, device=u.device, dtype=torch.float32)
+        g.checkpoints = saved.data_ptr()
+    keep = _workspace(L.dc_selective_scan_workspace_size, g, workspace, u.device)
+    _call(L.dc_selective_scan, g, u.device, "dc_selective_scan")
+    del keep
+    return (y, h, saved) if checkpoints else (y, h)
+
+
+def selective_scan_step(u: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, d: Optional[torch.Tensor] = None,
+                        z: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None, *,
+                        softplus: bool = True, out_dtype: Optional[torch.dtype] = None, y_out: Optional[torch.Tensor] = None,
+                        state_out: Optional[torch.Tensor] = None):
+    """:func:`selective_scan` for one token per sequence (``dc_selective_scan_step``): ``u``, ``dt``, ``z [batch, channels]``, ``b``,
+    ``c [batch, groups, state]`` or ``[batch, state]``; returns ``(y [batch, channels], next state)``.  Pass ``state_out=state`` to
+    update the state in place."""
+    if not isinstance(u, torch.Tensor) or u.dim() != 2:
+        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, "u must be [batch, channels]")
+    one = lambda t: t.unsqueeze(1) if isinstance(t, torch.Tensor) else t
+    g = _scan_args(one(u), one(dt), a, one(b), one(c), d, one(z), dt_bias, state, softplus, None)
+    y, h = _scan_outputs(g, u, out_dtype, one(y_out), state_out)
+    _call(_abi.lib().dc_selective_scan_step, g, u.device, "dc_selective_scan_step")
+    return (y.squeeze(1) if y_out is None else y_out), h
+
+
+def selective_scan_backward(d_y: torch.Tensor, d_state: Optional[torch.Tensor], u: torch.Tensor, dt: torch.Tensor, a: torch.Tensor,
+                            b: torch.Tensor, c: torch.Tensor, d: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
+                            dt_bias: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None, *, softplus: bool = True,
+                            lengths: Optional[torch.Tensor] = None, checkpoints: Optional[torch.Tensor] = None,
+                            workspace: Optional[torch.Tensor] = None):
+    """The backward of :func:`selective_scan` (``dc_selective_scan_bwd``), given ``d_y`` and the gradient of the final state
+    (``None``: zero), on the forward's inputs and its ``checkpoints`` (``None``: the forward is run again for them).  Returns
+    ``(d_u, d_dt, d_a, d_b, d_c, d_d, d_z, d_dt_bias, d_state)``: those of ``u``, ``dt``, ``b``, ``c``, ``z`` in their dtype, the others
+    float32, ``None`` where the input is."""
+    if checkpoints is None:
+        checkpoints = selective_scan(u, dt, a, b, c, d, z, dt_bias, state, softplus=softplus, lengths=lengths, checkpoints=True)[2]
+    w = _abi.SelectiveScanBwdArgs()
+    g = _scan_args(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths)
+    dev, dtype = u.device, u.dtype
+    shape = (g.batch, g.seq, g.channels)
+    L = _abi.lib()
+    g.checkpoints = _whole(checkpoints, "checkpoints", (int(L.dc_selective_scan_checkpoint_size(g)) // 4,), torch.float32, dev)
+    _cuda(d_y, "d_y", dev)
+    g.out_dtype = _code(d_y.dtype, "d_y")
+    w.d_y_batch_stride, w.d_y_token_stride = _strides(d_y, "d_y", shape, d_y.dtype, dev)
+    w.d_y = d_y.data_ptr()
+    w.d_state_out = _whole(d_state, "d_state", (g.batch, g.channels, g.state), torch.float32, dev)
+    new = lambda shape, dt=torch.float32: torch.empty(shape, device=dev, dtype=dt)
+    d_u, d_dt, d_z = new(shape, dtype), new(shape, dtype), None if z is None else new(shape, dtype)
+    d_b, d_c = new(b.shape, dtype), new(c.shape, dtype)
+    d_a = new((g.channels, g.state))
+    d_d, d_dt_bias = None if d is None else new(g.channels), None if dt_bias is None else new(g.channels)
+    d_state_in = None if state is None else new((g.batch, g.channels, g.state))
+    for name, t in (("d_u", d_u), ("d_dt", d_dt), ("d_a", d_a), ("d_b", d_b), ("d_c", d_c), ("d_d", d_d), ("d_z", d_z),
+                    ("d_dt_bias", d_dt_bias), ("d_state_in", d_state_in)):
+        if t is not None:
+            setattr(w, name, t.data_ptr())
+    w.fwd = g
+    keep = _workspace(L.dc_selective_scan_bwd_workspace_size, w, workspace, dev)
+    _call(L.dc_selective_scan_bwd, w, dev, "dc_selective_scan_bwd")
+    del keep
+    return d_u, d_dt, d_a, d_b, d_c, d_d, d_z, d_dt_bias, d_state_in
+
+
+class SelectiveScanFunction(torch.autograd.Function):
+    """``y, final_state = SelectiveScanFunction.apply(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths)``:
+    :func:`selective_scan` as an autograd node.  It keeps its inputs and the checkpoints (the state at the first token of every
+    tile), and the backward recomputes the states between them."""
+
+    @staticmethod
+    def forward(ctx, u, dt, a, b, c, d=None, z=None, dt_bias=None, state=None, softplus=True, lengths=None):
+        y, h, saved = selective_scan(u, dt, a, b, c, d, z, dt_bias, state, softplus=softplus, lengths=lengths, checkpoints=True)
+        ctx.save_for_backward(u, dt, a, b, c, d, z, dt_bias, state, lengths, saved)
+        ctx.softplus = softplus
+        return y, h
+
+    @staticmethod
+    def backward(ctx, d_y, d_h):
+        *args, lengths, saved = ctx.saved_tensors
+        grads = selective_scan_backward(d_y.contiguous(), d_h.contiguous(), *args, softplus=ctx.softplus, lengths=lengths, checkpoints=saved)
+        return (*grads, None, None)

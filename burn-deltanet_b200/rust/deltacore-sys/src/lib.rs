@@ -12,6 +12,9 @@
 
 use std::ffi::{c_char, c_int, c_void, CStr};
 
+/// The operators around the token mixers (`include/deltacore_layers.h`).
+pub mod layers;
+
 /// `cudaStream_t` / `CUstream` (null = the legacy default stream).
 pub type dc_stream_t = *mut c_void;
 
