@@ -21,19 +21,70 @@ int validate_output(const dc_selective_scan_args *a, int64_t seq) {
     return DC_OK;
 }
 
+// How a prompt is cut (selective_scan.cuh): segments side by side, or a walk of `pieces` pieces of `piece` tokens.
+struct Cut {
+    bool segments;
+    int64_t pieces, piece;
+};
+
+// By the CTAs that the walk would give and those that the card holds (`room`).  Measured, state 16, bfloat16, microseconds:
+//   8 x 4096 x 2048 (1024 CTAs): walk 467, segments 1067      4 x 2048 x 2048 (512): walk 153, segments 311
+//   2 x 4096 x 2048 (256): walk 254, segments 310, 4 pieces 217
+//   1 x 4096 x 2048 (128): walk 223, segments 159, 8 pieces 119
+//   1 x 16384 x 1024 (64): walk 872, segments 478, 16 pieces 226
+// So: the walk from a third of the room on; below that as many pieces as fill the room, each 128 tokens at least, if
+// that makes three or more of them; else segments.
+Cut cut_of(const dc_selective_scan_args *a, bool workspace) {
+    constexpr int64_t kLeast = 128;  // a multiple of every checkpoint's distance
+    const int lanes = sc::lanes_of(a->state);
+    const int64_t ctas = a->batch * a->groups * ceil_div(a->channels / a->groups, sc::walk_channels(lanes));
+    const int64_t room = (int64_t)sm_count() * sc::walk_ctas(lanes);
+    Cut c{false, 1, a->seq};
+    if (3 * ctas > room) return c;
+    const int64_t want = room / ctas, most = a->seq / kLeast, pieces = want < most ? want : most;
+    if (workspace && pieces >= 3) {
+        c.piece = ceil_div(ceil_div(a->seq, pieces), kLeast) * kLeast;
+        c.pieces = ceil_div(a->seq, c.piece);
+    } else {
+        c.segments = true;
+    }
+    return c;
+}
+
+// Floats of the pieces' end states, then of their sums of steps.
+int64_t piece_floats(const dc_selective_scan_args *a, const Cut &c) {
+    return c.pieces > 1 ? a->batch * a->channels * (c.pieces * a->state + c.pieces - 1) : 0;
+}
+
+template <typename Smem, typename K>
+int launch(K *kernel, const sc::Params &p, int64_t ctas, int threads, cudaStream_t s) {
+    if (ctas > 0x7fffffff) return DC_EUNSUPPORTED;
+    if (sizeof(Smem) > 48 * 1024) {
+        const int st = sc::allow_smem(kernel, sizeof(Smem));
+        if (st != DC_OK) return st;
+    }
+    kernel<<<(unsigned)ctas, threads, sizeof(Smem), s>>>(p);
+    return launched();
+}
+
 template <typename TI>
 struct Launch {
     const sc::Params &p;
+    const Cut &c;
     cudaStream_t s;
     template <int P>
     int operator()() const {
-        const int64_t ctas = p.batch * p.groups * p.blocks;
-        if (ctas > 0x7fffffff) return DC_EUNSUPPORTED;
-        constexpr size_t smem = sizeof(sc::FwdSmem<TI, P>);
-        const int st = sc::allow_smem(&sc::scan_kernel<TI, P>, smem);
-        if (st != DC_OK) return st;
-        sc::scan_kernel<TI, P><<<(unsigned)ctas, sc::kThreads, smem, s>>>(p);
-        return launched();
+        using Walk = sc::WalkShape<P>;
+        using Seg = sc::SegShape<P>;
+        const int64_t seqs = p.batch * p.groups;
+        if (c.segments)
+            return launch<sc::SegSmem<TI, P>>(&sc::scan_segments_kernel<TI, P>, p, seqs * ceil_div(p.per, Seg::kCh), Seg::kNT, s);
+        const int64_t blocks = seqs * ceil_div(p.per, Walk::kCh);
+        if (c.pieces > 1) {
+            const int st = launch<sc::WalkSmem<TI, P>>(&sc::scan_walk_kernel<TI, P, false>, p, blocks * (c.pieces - 1), Walk::kNT, s);
+            if (st != DC_OK) return st;
+        }
+        return launch<sc::WalkSmem<TI, P>>(&sc::scan_walk_kernel<TI, P, true>, p, blocks * c.pieces, Walk::kNT, s);
     }
 };
 
@@ -59,7 +110,10 @@ uint64_t dc_selective_scan_checkpoint_size(const dc_selective_scan_args *a) {
     return (uint64_t)a->batch * (uint64_t)ceil_div(a->seq, sc::tile_tokens(a->state)) * (uint64_t)a->channels * (uint64_t)a->state * 4;
 }
 
-uint64_t dc_selective_scan_workspace_size(const dc_selective_scan_args *) { return 0; }
+uint64_t dc_selective_scan_workspace_size(const dc_selective_scan_args *a) {
+    if (sc::validate_dims(a) != DC_OK || a->batch == 0 || a->channels == 0) return 0;
+    return (uint64_t)piece_floats(a, cut_of(a, true)) * 4;
+}
 
 int dc_selective_scan(const dc_selective_scan_args *a, dc_stream_t stream) {
     int st = sc::validate_dims(a);
@@ -69,11 +123,19 @@ int dc_selective_scan(const dc_selective_scan_args *a, dc_stream_t stream) {
     if (st == DC_OK) st = validate_output(a, a->seq);
     if (st == DC_OK) st = check_device();
     if (st != DC_OK) return st;
+    const Cut c = cut_of(a, a->workspace != nullptr);
+    if (c.pieces > 1) {
+        if (a->workspace_bytes < (uint64_t)piece_floats(a, c) * 4) return DC_EWORKSPACE;
+        if (!aligned(a->workspace, 16)) return DC_EINVAL_ARG;
+    }
     sc::Params p = sc::params_of(a);
-    p.blocks = (int32_t)ceil_div(p.per, sc::kCh);
+    p.pieces = (int32_t)c.pieces;
+    p.piece = c.piece;
+    p.piece_end = static_cast<float *>(a->workspace);
+    p.piece_step = p.piece_end + a->batch * a->channels * c.pieces * a->state;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (a->in_dtype == DC_BF16) return sc::for_lanes(a->state, Launch<__nv_bfloat16>{p, s});
-    return sc::for_lanes(a->state, Launch<float>{p, s});
+    if (a->in_dtype == DC_BF16) return sc::for_lanes(a->state, Launch<__nv_bfloat16>{p, c, s});
+    return sc::for_lanes(a->state, Launch<float>{p, c, s});
 }
 
 int dc_selective_scan_step(const dc_selective_scan_args *a, dc_stream_t stream) {

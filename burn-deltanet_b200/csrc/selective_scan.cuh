@@ -6,14 +6,20 @@
 // per (sequence, channel), `state` values of h.  The exponentials bound it: state + 4 of them and their like
 // (softplus, silu) per (token, channel) at 16 a clock and SM, against 4 elements read or written.
 //
-// Layout.  A CTA of 256 threads owns 16 channels of one sequence and walks its tokens in tiles.  Four states of a
-// channel live in a thread's registers, so a channel spans P = state / 4 threads (padded to a power of two, the padding
-// with a = b = c = 0), and the CTA's 16 / P segments of 16 P threads take consecutive runs of K = 8 tokens of the tile.
-// The recurrence is linear, so each segment first runs its K tokens from zero while it keeps the decays and the products
-// in registers (every exponential is taken once), the segments exchange (product of decays, end state) through shared
-// memory, and each runs its K tokens again from the state that reaches it, now reading out: two multiply-adds per token
-// and state more than a serial walk, hidden behind the exponentials, for 16 / P times the parallel work.  b and c of a
-// tile are read once for the CTA's channels and kept in float32 in shared memory.
+// Layout.  A CTA owns a block of channels of one sequence and walks its tokens in tiles that it stages in shared memory
+// (asynchronous copies, the next tile's under this one's arithmetic).  Four states of a channel live in a thread's
+// registers, so a channel spans P = state / 4 threads (padded to a power of two, the padding with a = b = c = 0).  b and c
+// of a tile are read once for the CTA's channels and kept in float32.
+//
+// Three ways along the time axis, chosen by how many channels there are to fill the card with (selective_scan.cu):
+//   * walk: a thread walks its channel's tokens one by one.  Least work.
+//   * segments: the CTA's W segments of threads take consecutive runs of K = 8 tokens.  The recurrence is linear, so each
+//     segment first runs its tokens from zero while it keeps the decays and products in registers (every exponential is
+//     still taken once), the segments exchange (product of decays, end state) through shared memory, and each runs its
+//     tokens again from the state that reaches it, now reading out: about a third more instructions for W times the threads.
+//   * pieces: the time axis cut over CTAs that walk: a first launch finds each piece's end state from zero and its sum of steps (whose
+//     exponential is the product of its decays), the second starts each piece from what the pieces before it give and does
+//     the work: nearly twice the exponentials, for sequences long enough and channels few enough.
 #pragma once
 
 #include "common.cuh"
@@ -23,12 +29,13 @@
 namespace dc {
 namespace scan {
 
-constexpr int kThreads = 256;
-constexpr int kCh = 16;   // channels of a CTA
-constexpr int kK = 8;     // tokens of a segment
-constexpr int kS = 4;     // states of a thread
+constexpr int kThreads = 256;  // of the step and the backward
+constexpr int kCh = 16;        // channels of a block in the backward
+constexpr int kK = 8;          // tokens of a segment
+constexpr int kS = 4;          // states of a thread
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// The backward's tile; the forward's checkpoints are at its first tokens.
 template <int P>
 struct Tile {
     static constexpr int kSegs = kThreads / (kCh * P);  // 16 / P
@@ -42,13 +49,16 @@ struct Params {
     int64_t u_b, u_t, dt_b, dt_t, z_b, z_t, b_b, b_t, c_b, c_t, y_b, y_t;
     int32_t softplus, y_dt;
     int32_t vec_x, vec_bc;  // strides allow 16-byte copies of the channel rows / of the b and c rows
-    int32_t blocks;         // CTAs of a group: ceil(per / 16)
     int32_t tiles;          // checkpoints of a sequence
+    int32_t pieces;         // pieces of the time axis, `piece` tokens each (a multiple of every tile's)
+    int64_t piece;
     const void *u, *dt, *z, *b, *c;
     const float *a, *d, *dt_bias, *state_in;
     const int32_t *lengths;
     void *y;
     float *state_out, *ckpt;
+    float *piece_end;   // [batch, pieces, channels, N]: the state before the first token, then the pieces' end states from zero
+    float *piece_step;  // [batch, pieces - 1, channels]: their sums of steps
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -62,23 +72,6 @@ __device__ __forceinline__ float rcp(float x) {
     return y;
 }
 __device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-kLog2e * x)); }
-
-// max(x, 0) + log(1 + e), e = exp(-|x|), with log(1 + e) = 2 atanh(s) at s = e / (2 + e) <= 1/3 by its series
-// s + s^3/3 + ...: full relative precision for small steps, where 1 + e would have rounded e away; the terms left out
-// are below 2^-26 of the sum.  NaN stays NaN.
-__device__ __forceinline__ float softplus(float x) {
-    const float e = ex2(-kLog2e * fabsf(x));
-    const float s = e * rcp(2.f + e), q = s * s;
-    float p = 1.f / 15.f;
-    p = fmaf(p, q, 1.f / 13.f);
-    p = fmaf(p, q, 1.f / 11.f);
-    p = fmaf(p, q, 1.f / 9.f);
-    p = fmaf(p, q, 1.f / 7.f);
-    p = fmaf(p, q, 1.f / 5.f);
-    p = fmaf(p, q, 1.f / 3.f);
-    p = fmaf(p, q, 1.f);
-    return (x > 0.f ? x : x < 0.f ? 0.f : x) + 2.f * s * p;
-}
 
 // Pairs of float32 in one instruction (both lanes rounded as the single forms round them).
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -95,6 +88,21 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     return r;
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// max(x, 0) + log(1 + e), e = exp(-|x|), with log(1 + e) = 2 atanh(s) at s = e / (2 + e) <= 1/3 by its series
+// s + s^3/3 + ... + s^11/11: full relative precision for small steps, where 1 + e would have rounded e away; the terms
+// left out are below 1.6e-7 of the sum (at x = 0, and far less elsewhere).  Two at a time.  NaN stays NaN (through e).
+__device__ __forceinline__ float2 softplus2(float2 x) {
+    const float2 e = make_float2(ex2(-kLog2e * fabsf(x.x)), ex2(-kLog2e * fabsf(x.y)));
+    const float2 s = mul2(e, make_float2(rcp(2.f + e.x), rcp(2.f + e.y))), q = mul2(s, s);
+    float2 p = fma2(both(1.f / 11.f), q, both(1.f / 9.f));
+    p = fma2(p, q, both(1.f / 7.f));
+    p = fma2(p, q, both(1.f / 5.f));
+    p = fma2(p, q, both(1.f / 3.f));
+    p = fma2(p, q, both(1.f));
+    return fma2(mul2(both(2.f), s), p, make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)));
+}
+__device__ __forceinline__ float softplus(float x) { return softplus2(make_float2(x, x)).x; }
 
 struct F4 {  // four states
     float2 lo, hi;
@@ -192,20 +200,22 @@ __device__ __forceinline__ Place place_of(int64_t block, const Params &p, int wi
     return q;
 }
 
-// `rows` rows of 16 channels (nch of them real) from src (row stride st) into dst [rows][16]; rows from `live` on and
-// missing channels are zeros.  The copies are asynchronous where vec says 16-byte copies are possible.
-template <typename TI>
-__device__ __forceinline__ void stage_x(TI *dst, const TI *src, int64_t st, int rows, int live, int nch, bool vec) {
-    constexpr int kPer = kCh * sizeof(TI) / 16, kEl = 16 / sizeof(TI);
-    if (vec && nch == kCh && aligned16(src)) {
-        for (int i = threadIdx.x; i < rows * kPer; i += kThreads) {
+// `rows` rows of CH channels (nch of them real) from src (row stride st) into dst [rows][CH], by NT threads; rows from
+// `live` on and missing channels are zeros.  The copies are asynchronous where vec says 16-byte copies are possible.
+template <int NT, int CH, typename TI>
+__device__ __forceinline__ void stage_x(TI *dst, const TI *src, int64_t st, int rows, int live, int nch, bool vec,
+                                        int tid = threadIdx.x) {
+    constexpr int kEl = 16 / sizeof(TI), kPer = CH / kEl;
+    if (vec && nch == CH && aligned16(src)) {
+#pragma unroll 1
+        for (int i = tid; i < rows * kPer; i += NT) {
             const int r = i / kPer, q = i % kPer;
-            if (r < live) ptx::cp_async16(ptx::smem_u32(dst + r * kCh + q * kEl), src + r * st + q * kEl, 16u);
-            else *reinterpret_cast<uint4 *>(dst + r * kCh + q * kEl) = make_uint4(0, 0, 0, 0);
+            ptx::cp_async16(ptx::smem_u32(dst + i * kEl), src + (r < live ? r * st : 0) + q * kEl, r < live ? 16u : 0u);
         }
     } else {
-        for (int i = threadIdx.x; i < rows * kCh; i += kThreads) {
-            const int r = i / kCh, q = i % kCh;
+#pragma unroll 1
+        for (int i = tid; i < rows * CH; i += NT) {
+            const int r = i / CH, q = i % CH;
             TI v;
             dc::st(&v, 0.f);
             if (r < live && q < nch) v = src[r * st + q];
@@ -214,18 +224,27 @@ __device__ __forceinline__ void stage_x(TI *dst, const TI *src, int64_t st, int 
     }
 }
 // the same for `rows` rows of N states into dst [rows][NP] (columns from N on were zeroed once)
-template <typename TI, int NP>
-__device__ __forceinline__ void stage_bc(TI *dst, const TI *src, int64_t st, int rows, int live, int N, bool vec) {
+template <int NT, int NP, typename TI>
+__device__ __forceinline__ void stage_bc(TI *dst, const TI *src, int64_t st, int rows, int live, int N, bool vec,
+                                         int tid = threadIdx.x) {
     constexpr int kEl = 16 / sizeof(TI);
-    if (vec && N % kEl == 0 && aligned16(src)) {
+    if (vec && N == NP && NP % kEl == 0 && aligned16(src)) {
+        constexpr int kPer = NP >= kEl ? NP / kEl : 1;
+#pragma unroll 1
+        for (int i = tid; i < rows * kPer; i += NT) {
+            const int r = i / kPer, q = i % kPer;
+            ptx::cp_async16(ptx::smem_u32(dst + i * kEl), src + (r < live ? r * st : 0) + q * kEl, r < live ? 16u : 0u);
+        }
+    } else if (vec && N % kEl == 0 && aligned16(src)) {
         const int per = N / kEl;
-        for (int i = threadIdx.x; i < rows * per; i += kThreads) {
+#pragma unroll 1
+        for (int i = tid; i < rows * per; i += NT) {
             const int r = i / per, q = i % per;
-            if (r < live) ptx::cp_async16(ptx::smem_u32(dst + r * NP + q * kEl), src + r * st + q * kEl, 16u);
-            else *reinterpret_cast<uint4 *>(dst + r * NP + q * kEl) = make_uint4(0, 0, 0, 0);
+            ptx::cp_async16(ptx::smem_u32(dst + r * NP + q * kEl), src + (r < live ? r * st : 0) + q * kEl, r < live ? 16u : 0u);
         }
     } else {
-        for (int i = threadIdx.x; i < rows * NP; i += kThreads) {
+#pragma unroll 1
+        for (int i = tid; i < rows * NP; i += NT) {
             const int r = i / NP, q = i % NP;
             TI v;
             dc::st(&v, 0.f);
@@ -234,159 +253,445 @@ __device__ __forceinline__ void stage_bc(TI *dst, const TI *src, int64_t st, int
         }
     }
 }
+// `n` values (a multiple of 4) in shared memory to float32, by NT threads
+template <int NT, typename TI>
+__device__ __forceinline__ void widen(float4 *dst, const TI *src, int n, int tid) {
+#pragma unroll 2
+    for (int i = tid; i < n / 4; i += NT) {
+        float v[4];
+        vec::load<true>(src + 4 * i, v);
+        dst[i] = make_float4(v[0], v[1], v[2], v[3]);
+    }
+}
 
 // ------------------------------------------------------------------------------------------------ forward
+// What both forward kernels know about their CTA: where it works, and how it stages a tile and writes y.
+template <typename TI, int CH, int N4>
+struct Work {
+    const Params &p;
+    Place at;
+    int64_t first, last, len;  // this CTA's tokens, and where those inside the sequence end
+    const TI *U, *D, *Z, *B, *C;
+
+    __device__ __forceinline__ Work(const Params &p, int64_t block, int64_t pieces) : p(p) {
+        const int64_t piece = pieces > 1 ? block % pieces : 0;
+        at = place_of(pieces > 1 ? block / pieces : block, p, CH);
+        const int64_t all = length_of(p.lengths, at.b, p.seq);
+        first = piece * p.piece;
+        last = p.pieces > 1 && first + p.piece < p.seq ? first + p.piece : p.seq;
+        len = all < last ? all : last;
+        U = static_cast<const TI *>(p.u) + at.b * p.u_b + at.d0, D = static_cast<const TI *>(p.dt) + at.b * p.dt_b + at.d0;
+        Z = p.z ? static_cast<const TI *>(p.z) + at.b * p.z_b + at.d0 : nullptr;
+        B = static_cast<const TI *>(p.b) + at.b * p.b_b + at.e * p.N, C = static_cast<const TI *>(p.c) + at.b * p.c_b + at.e * p.N;
+    }
+    template <int NT, int TOK, bool FULL, typename Raw>
+    __device__ __forceinline__ void load(Raw &w, int64_t t0, int tid) const {
+        const int live = len - t0 < TOK ? (int)(len - t0) : TOK;
+        stage_x<NT, CH>(w.dt, D + t0 * p.dt_t, p.dt_t, TOK, live, at.nch, p.vec_x, tid);
+        stage_x<NT, CH>(w.u, U + t0 * p.u_t, p.u_t, TOK, live, at.nch, p.vec_x, tid);
+        stage_bc<NT, N4>(w.b, B + t0 * p.b_t, p.b_t, TOK, live, p.N, p.vec_bc, tid);
+        if (FULL) {
+            stage_bc<NT, N4>(w.c, C + t0 * p.c_t, p.c_t, TOK, live, p.N, p.vec_bc, tid);
+            if (Z) stage_x<NT, CH>(w.z, Z + t0 * p.z_t, p.z_t, TOK, live, at.nch, p.vec_x, tid);
+        }
+    }
+};
+
+// The part of a tile's work that goes by token and channel, four channels of a token at a time: the steps before the
+// recurrence, the skip and the gate after it.  A thread of NT always has the same four channels.
+template <typename TI, int P, int CH, int TOK, int NT>
+struct Quads {
+    static constexpr int kQuads = CH / 4, kRows = NT / kQuads;
+    static_assert(NT % kQuads == 0, "one quad of channels per thread");
+    const Params &p;
+    int oc, orow, ny, nch;
+    float bias[4], skip[4];
+    int64_t y0;
+    bool yquad;
+
+    __device__ __forceinline__ Quads(const Params &p, const Place &at, int tid) : p(p) {
+        oc = 4 * (tid % kQuads), orow = tid / kQuads, nch = at.nch;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            bias[j] = p.dt_bias && oc + j < at.nch ? p.dt_bias[at.d0 + oc + j] : 0.f;
+            skip[j] = p.d && oc + j < at.nch ? p.d[at.d0 + oc + j] : 0.f;
+        }
+        y0 = at.b * p.y_b + at.d0 + oc;
+        const int ysize = p.y_dt ? 2 : 4;
+        ny = at.nch - oc;  // channels of the quad that exist (<= 0: none)
+        yquad = ny >= 4 && (reinterpret_cast<uintptr_t>(p.y) + y0 * ysize) % (4 * ysize) == 0 && p.y_t % 4 == 0;
+    }
+    __device__ __forceinline__ void put(int64_t t, const float (&v)[4]) const {
+        if (yquad) vec::store_as<true>(p.y_dt, p.y, y0 + t * p.y_t, v);
+        else vec::store_as<false>(p.y_dt, p.y, y0 + t * p.y_t, v, ny);
+    }
+    // raw dt and u of `live` tokens to (step, step * u)
+    __device__ __forceinline__ void steps(float2 *step, const TI *dt, const TI *u, int live) const {
+#pragma unroll 2
+        for (int t = orow; t < TOK; t += kRows) {
+            float v[4], x[4];
+            vec::load<true>(dt + t * CH + oc, v);
+            vec::load<true>(u + t * CH + oc, x);
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+                float2 f = make_float2(v[j] + bias[j], v[j + 1] + bias[j + 1]);
+                if (p.softplus) f = softplus2(f);
+                v[j] = t < live ? f.x : 0.f, v[j + 1] = t < live ? f.y : 0.f;  // past the end: decay 1, nothing added
+            }
+            float4 *o = reinterpret_cast<float4 *>(step + t * CH + oc);
+            o[0] = make_float4(v[0], v[0] * x[0], v[1], v[1] * x[1]);
+            o[1] = make_float4(v[2], v[2] * x[2], v[3], v[3] * x[3]);
+        }
+    }
+    // y of `live` tokens from t0 on, from the P shares of each: y[token][state group][channel]
+    __device__ __forceinline__ void outputs(const float *y, const TI *u, const TI *z, int64_t t0, int live) const {
+#pragma unroll 2
+        for (int t = orow; t < live; t += kRows) {
+            float v[4] = {0.f, 0.f, 0.f, 0.f}, x[4];
+            // from another share on in each token, so that a warp's reads meet in no bank
+            const float *row = y + t * CH * P + oc;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const float4 f = *reinterpret_cast<const float4 *>(row + ((i + t) & (P - 1)) * CH);
+                v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
+            }
+            vec::load<true>(u + t * CH + oc, x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = fmaf(skip[j], x[j], v[j]);
+            if (z) {
+                vec::load<true>(z + t * CH + oc, x);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] *= x[j] * sigmoid(x[j]);
+            }
+            put(t0 + t, v);
+        }
+    }
+    __device__ __forceinline__ void zeros(int64_t from, int64_t to) const {
+        const float none[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int64_t t = from + orow; t < to; t += kRows) put(t, none);
+    }
+};
+
+template <typename TI, int CH, int TOK, int N4>
+struct RawTile {
+    TI u[TOK * CH], dt[TOK * CH], z[TOK * CH];
+    TI b[TOK * N4], c[TOK * N4];
+};
+
+// b's and c's padding columns of every stage, zeroed once
+template <int NT, int TOK, int N4, int STAGES, typename Raw>
+__device__ __forceinline__ void clear_padding(Raw *raw, int N, int tid) {
+    if (N < N4)
+        for (int i = tid; i < TOK * N4; i += NT)
+            if (i % N4 >= N)
+#pragma unroll
+                for (int s = 0; s < STAGES; ++s) st(&raw[s].b[i], 0.f), st(&raw[s].c[i], 0.f);
+}
+
+__device__ __forceinline__ void checkpoint(const Params &p, const Place &at, int64_t t, int tokens, int64_t d, int q, F4 h) {
+    store4(p.ckpt + ((at.b * p.tiles + t / tokens) * p.channels + d) * p.N, kS * q, p.N, h);
+}
+
+// A thread's share of the 16-byte copies of a tile, where the rows start on 16-byte boundaries: the sources move on by one
+// tile a call.  What a row lacks of its last copies (missing channels, padding states) is filled with zeros.
+template <typename TI, int CH, int N4, int TOK, int NT, bool FULL>
+struct Stager {
+    static constexpr int kEs = sizeof(TI), kEl = 16 / kEs, kXRow = CH / kEl, kBRow = N4 >= kEl ? N4 / kEl : 1;  // copies per row
+    static constexpr int kX = TOK * kXRow, kB = TOK * kBRow;                                                    // and per tensor
+    static constexpr int kAll = FULL ? 3 * kX + 2 * kB : 2 * kX + kB, kEach = (kAll + NT - 1) / NT;
+    const char *src[kEach];
+    int64_t step[kEach];  // bytes a tile
+    int dst[kEach], row[kEach], bytes[kEach];
+    bool on;
+
+    __device__ __forceinline__ Stager(const Work<TI, CH, N4> &wk, int tid) {
+        const Params &p = wk.p;
+        on = p.vec_x && p.vec_bc && N4 % kEl == 0 && (!FULL || wk.Z) && aligned16(wk.U) && aligned16(wk.D) && aligned16(wk.B) &&
+             (!FULL || (aligned16(wk.Z) && aligned16(wk.C)));
+        if (!on) return;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            int c = tid + j * NT, base = 0, per = kXRow, width = wk.at.nch;  // tensors in RawTile's order: u, dt, (z,) b, (c)
+            const bool used = c < kAll;
+            const TI *t = wk.U;
+            int64_t st = p.u_t;
+            auto next = [&](int count, int at, int row_copies, int w, const TI *tensor, int64_t stride) {
+                if (c < count) return false;
+                c -= count, base = at, per = row_copies, width = w, t = tensor, st = stride;
+                return true;
+            };
+            if (next(kX, kX, kXRow, wk.at.nch, wk.D, p.dt_t)) {
+                if (FULL) {
+                    if (next(kX, 2 * kX, kXRow, wk.at.nch, wk.Z, p.z_t) && next(kX, 3 * kX, kBRow, p.N, wk.B, p.b_t))
+                        next(kB, 3 * kX + kB, kBRow, p.N, wk.C, p.c_t);
+                } else {
+                    next(kX, 3 * kX, kBRow, p.N, wk.B, p.b_t);
+                }
+            }
+            const int r = used ? c / per : 0, q = used ? c % per : 0, left = (width - q * kEl) * kEs;
+            row[j] = used ? r : TOK;  // a row that no tile has
+            bytes[j] = left < 0 ? 0 : left > 16 ? 16 : left;
+            dst[j] = (base + (used ? c : 0)) * 16;
+            src[j] = reinterpret_cast<const char *>(t + (wk.first + r) * st + (bytes[j] ? q * kEl : 0));
+            step[j] = st * (int64_t)(TOK * kEs);
+        }
+    }
+    template <typename Raw>
+    __device__ __forceinline__ void copy(Raw &raw, int live) {
+        const uint32_t to = ptx::smem_u32(&raw);
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            // past the end: no bytes, from the tile's first row, which is always inside the sequence
+            if (row[j] < TOK)
+                ptx::cp_async16(to + dst[j], row[j] < live ? src[j] : src[j] - step[j] / TOK * row[j], row[j] < live ? bytes[j] : 0);
+            src[j] += step[j];
+        }
+    }
+};
+
+// ---- token by token.  A thread of the recurrence has four states of two neighbouring channels: b and c come from shared
+// memory once for both, and shared memory's bandwidth would be the bound otherwise (at one channel a thread, 80 % of it
+// was in use and the largest case took 568 us).  kHelp further threads stage the tiles, take the steps of the next tile
+// and write y of the last one, so that the two kinds of work, each a chain of dependent instructions, fill each other's
+// gaps.  One barrier per tile of 16 tokens.
+// FULL: the whole scan; else only the piece's end state from zero and its sum of steps.
+constexpr int walk_channels(int lanes) { return lanes >= 4 ? 16 : 64 / lanes; }       // of a CTA: a warp's at least
+constexpr int walk_ctas(int lanes) { return lanes == 4 ? 7 : lanes == 2 || lanes == 8 ? 4 : lanes == 16 ? 3 : 2; }  // of an SM, by their registers and shared memory
+template <int P>
+struct WalkShape {
+    static constexpr int kCh = walk_channels(P), kMain = kCh * P / 2, kHelp = 4 * kCh, kNT = kMain + kHelp;
+    static constexpr int kTok = 16, kStages = 4, kN = kS * P;
+};
 template <typename TI, int P>
-struct FwdSmem {
-    using T = Tile<P>;
-    struct Raw {
-        TI u[T::kTokens * kCh], dt[T::kTokens * kCh], z[T::kTokens * kCh];
-        TI b[T::kTokens * T::kN], c[T::kTokens * T::kN];
-    };
-    Raw raw[2];
-    float2 step[T::kTokens * kCh];  // (step, step * u)
-    float4 b[T::kTokens * P], c[T::kTokens * P];
-    float4 decay[kThreads], end[kThreads];  // each segment's product of decays and end state
-    float y[T::kTokens * kCh];
+struct WalkSmem {
+    using S = WalkShape<P>;
+    RawTile<TI, S::kCh, S::kTok, S::kN> raw[S::kStages];
+    float2 step[2][S::kTok * S::kCh];
+    float4 b[2][S::kTok * P], c[2][S::kTok * P];
+    float y[2][S::kTok * S::kCh * P];
+};
+
+template <typename TI, int P, bool FULL>
+__global__ void __launch_bounds__(WalkShape<P>::kNT, walk_ctas(P)) scan_walk_kernel(const Params p) {
+    using S = WalkShape<P>;
+    constexpr int kTok = S::kTok, CH = S::kCh, kBatch = 4;
+    extern __shared__ __align__(16) unsigned char smem_bytes[];
+    WalkSmem<TI, P> &sm = *reinterpret_cast<WalkSmem<TI, P> *>(smem_bytes);
+    const int64_t pieces = FULL ? p.pieces : p.pieces - 1;  // nothing follows the last piece's end
+    const Work<TI, CH, S::kN> wk(p, blockIdx.x, pieces);
+    const Place &at = wk.at;
+    const int64_t first = wk.first, len = wk.len;
+    const int n = len > first ? (int)((len - first + kTok - 1) / kTok) : 0;  // tiles
+
+    if (threadIdx.x >= S::kMain) {
+        const int tid = threadIdx.x - S::kMain;
+        const Quads<TI, P, CH, kTok, S::kHelp> quads(p, at, tid);
+        Stager<TI, CH, S::kN, kTok, S::kHelp, FULL> stager(wk, tid);
+        if (!stager.on) clear_padding<S::kHelp, kTok, S::kN, S::kStages>(sm.raw, p.N, tid);
+        auto live = [&](int i) { return len - first - (int64_t)i * kTok < kTok ? (int)(len - first - (int64_t)i * kTok) : kTok; };
+        auto prepare = [&](int i) {  // tile i's steps, b and c, once every helper's copies of it have landed
+            const auto &w = sm.raw[i % S::kStages];
+            ptx::named_sync(1, S::kHelp);
+            quads.steps(sm.step[i & 1], w.dt, w.u, live(i));
+            widen<S::kHelp>(sm.b[i & 1], w.b, kTok * S::kN, tid);
+            if (FULL) widen<S::kHelp>(sm.c[i & 1], w.c, kTok * S::kN, tid);
+        };
+        auto load = [&](int i) {
+            if (i < n) {
+                if (stager.on) stager.copy(sm.raw[i % S::kStages], live(i));
+                else wk.template load<S::kHelp, kTok, FULL>(sm.raw[i % S::kStages], first + (int64_t)i * kTok, tid);
+            }
+            ptx::cp_async_commit();
+        };
+        load(0);
+        load(1);
+        ptx::cp_async_wait<1>();
+        if (n > 0) prepare(0);
+        __syncthreads();
+        for (int i = 0; i < n; ++i) {
+            load(i + 2);
+            if (FULL && i > 0) {
+                const auto &w = sm.raw[(i - 1) % S::kStages];
+                quads.outputs(sm.y[(i - 1) & 1], w.u, wk.Z ? w.z : nullptr, first + (int64_t)(i - 1) * kTok, kTok);
+            }
+            ptx::cp_async_wait<1>();
+            if (i + 1 < n) prepare(i + 1);
+            __syncthreads();
+        }
+        if (FULL && n > 0) {
+            const auto &w = sm.raw[(n - 1) % S::kStages];
+            quads.outputs(sm.y[(n - 1) & 1], w.u, wk.Z ? w.z : nullptr, first + (int64_t)(n - 1) * kTok, live(n - 1));
+        }
+        if (FULL) quads.zeros(len > first ? len : first, wk.last);
+        return;
+    }
+
+    const int ch = 2 * (threadIdx.x % (CH / 2)), q = threadIdx.x / (CH / 2), N = p.N;
+    const int64_t d = at.d0 + ch, piece = pieces > 1 ? blockIdx.x % pieces : 0;
+    bool real[2];
+    F4 a2[2], h[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        real[j] = ch + j < at.nch;
+        a2[j] = real[j] ? mul(kLog2e, load4(p.a + (d + j) * N, kS * q, N)) : zero4();
+        h[j] = zero4();
+        if (FULL && p.pieces > 1 && real[j]) {  // what the pieces before this one make of the first state
+            const int64_t at_end = at.b * p.pieces * p.channels + d + j, at_step = at.b * (p.pieces - 1) * p.channels + d + j;
+            h[j] = load4(p.piece_end + at_end * N, kS * q, N);
+#pragma unroll 4
+            for (int64_t i = 0; i < piece; ++i)
+                h[j] = fma(ex2(mul(p.piece_step[at_step + i * p.channels], a2[j])), h[j],
+                           load4(p.piece_end + (at_end + (i + 1) * p.channels) * N, kS * q, N));
+        } else if (FULL && p.state_in && real[j]) {
+            h[j] = load4(p.state_in + (at.b * p.channels + d + j) * N, kS * q, N);
+        }
+    }
+    float2 steps = make_float2(0.f, 0.f);
+    __syncthreads();
+    for (int i = 0; i < n; ++i) {
+        const float2 *step = sm.step[i & 1] + ch;
+        const float4 *b = sm.b[i & 1] + q, *c = sm.c[i & 1] + q;
+        float *y = sm.y[i & 1] + q * CH + ch;
+#pragma unroll 1
+        for (int k0 = 0; k0 < kTok; k0 += kK) {
+            if (FULL && p.ckpt) {
+                const int64_t t = first + (int64_t)i * kTok + k0;
+                if (t < len && t % Tile<P>::kTokens == 0)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        if (real[j]) checkpoint(p, at, t, Tile<P>::kTokens, d + j, q, h[j]);
+            }
+#pragma unroll
+            for (int k1 = 0; k1 < kK; k1 += kBatch) {
+                F4 av[kBatch][2], bv[kBatch][2];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    const int t = k0 + k1 + k;
+                    const float4 sd = *reinterpret_cast<const float4 *>(step + t * CH);  // both channels' (step, step * u)
+                    const F4 bt = f4(b[t * P]);
+                    av[k][0] = ex2(mul(sd.x, a2[0])), av[k][1] = ex2(mul(sd.z, a2[1]));
+                    bv[k][0] = mul(sd.y, bt), bv[k][1] = mul(sd.w, bt);
+                    if (!FULL) steps.x += sd.x, steps.y += sd.z;
+                }
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    const int t = k0 + k1 + k;
+                    h[0] = fma(av[k][0], h[0], bv[k][0]), h[1] = fma(av[k][1], h[1], bv[k][1]);
+                    if (FULL) {
+                        const F4 ct = f4(c[t * P]);
+                        *reinterpret_cast<float2 *>(y + t * CH * P) = make_float2(dot(h[0], ct), dot(h[1], ct));
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        if (!real[j]) continue;
+        const int64_t own = (at.b * p.channels + d + j) * N;
+        if (FULL) {
+            if (p.state_out && piece == p.pieces - 1) store4(p.state_out + own, kS * q, N, h[j]);
+            continue;
+        }
+        const int64_t row = at.b * p.pieces * p.channels + d + j;
+        store4(p.piece_end + (row + (piece + 1) * p.channels) * N, kS * q, N, h[j]);
+        if (q == 0) p.piece_step[(at.b * (p.pieces - 1) + piece) * p.channels + d + j] = j ? steps.y : steps.x;
+        // the first state is kept with them: the second launch may overwrite state_in (state_out == state_in)
+        if (piece == 0) store4(p.piece_end + row * N, kS * q, N, p.state_in ? load4(p.state_in + own, kS * q, N) : zero4());
+    }
+}
+
+// ---- segments side by side: CH channels of P threads each, W segments of them; kSub tokens go by between two exchanges,
+// kTok between two stagings.
+template <int P>
+struct SegShape {
+    static constexpr int kCh = 8, kW = P == 1 ? 16 : 32 / P, kLanes = kCh * P, kNT = kLanes * kW;
+    static constexpr int kSub = kW * kK, kTok = kSub < 32 ? 32 : kSub, kN = kS * P;
+};
+template <typename TI, int P>
+struct SegSmem {
+    using S = SegShape<P>;
+    RawTile<TI, S::kCh, S::kTok, S::kN> raw[2];
+    float2 step[S::kTok * S::kCh];  // (step, step * u)
+    float4 b[S::kTok * P], c[S::kTok * P];
+    float y[S::kTok * S::kLanes];
+    float4 decay[S::kNT], end[S::kNT];  // each segment's product of decays and end state
 };
 
 template <typename TI, int P>
-__global__ void __launch_bounds__(kThreads) scan_kernel(const Params p) {
-    using T = Tile<P>;
-    using Smem = FwdSmem<TI, P>;
-    constexpr int kTok = T::kTokens, kLanes = kCh * P;
+__global__ void __launch_bounds__(SegShape<P>::kNT, 512 / SegShape<P>::kNT) scan_segments_kernel(const Params p) {
+    using S = SegShape<P>;
+    constexpr int kTok = S::kTok, CH = S::kCh, kLanes = S::kLanes, kNT = S::kNT, W = S::kW;
     extern __shared__ __align__(16) unsigned char smem_bytes[];
-    Smem &sm = *reinterpret_cast<Smem *>(smem_bytes);
-    const int tid = threadIdx.x, seg = tid / kLanes, r = tid % kLanes, ch = r / P, q = r % P;
-    const Place at = place_of(blockIdx.x, p, kCh);
-    const int64_t len = length_of(p.lengths, at.b, p.seq);
-    const int N = p.N;
-    const TI *U = static_cast<const TI *>(p.u) + at.b * p.u_b + at.d0, *D = static_cast<const TI *>(p.dt) + at.b * p.dt_b + at.d0;
-    const TI *Z = p.z ? static_cast<const TI *>(p.z) + at.b * p.z_b + at.d0 : nullptr;
-    const TI *B = static_cast<const TI *>(p.b) + at.b * p.b_b + at.e * N, *C = static_cast<const TI *>(p.c) + at.b * p.c_b + at.e * N;
-
-    auto load_tile = [&](int64_t t0, int s) {
-        const int live = len - t0 < kTok ? (int)(len - t0) : kTok;
-        typename Smem::Raw &w = sm.raw[s];
-        stage_x(w.u, U + t0 * p.u_t, p.u_t, kTok, live, at.nch, p.vec_x);
-        stage_x(w.dt, D + t0 * p.dt_t, p.dt_t, kTok, live, at.nch, p.vec_x);
-        if (Z) stage_x(w.z, Z + t0 * p.z_t, p.z_t, kTok, live, at.nch, p.vec_x);
-        stage_bc<TI, T::kN>(w.b, B + t0 * p.b_t, p.b_t, kTok, live, N, p.vec_bc);
-        stage_bc<TI, T::kN>(w.c, C + t0 * p.c_t, p.c_t, kTok, live, N, p.vec_bc);
-        ptx::cp_async_commit();
+    SegSmem<TI, P> &sm = *reinterpret_cast<SegSmem<TI, P> *>(smem_bytes);
+    const int tid = threadIdx.x, seg = tid / kLanes, r = tid % kLanes, ch = r % CH, q = r / CH, N = p.N;
+    const Work<TI, CH, S::kN> wk(p, blockIdx.x, 1);
+    const Place &at = wk.at;
+    const int64_t len = wk.len;
+    const Quads<TI, P, CH, kTok, kNT> quads(p, at, tid);
+    clear_padding<kNT, kTok, S::kN, 2>(sm.raw, N, tid);
+    auto prepare = [&](int64_t t0, int s) {
+        const auto &w = sm.raw[s];
+        quads.steps(sm.step, w.dt, w.u, len - t0 < kTok ? (int)(len - t0) : kTok);
+        widen<kNT>(sm.b, w.b, kTok * S::kN, tid);
+        widen<kNT>(sm.c, w.c, kTok * S::kN, tid);
     };
-
-    // the padding of b and c, zeroed once
-    for (int i = tid; i < kTok * T::kN; i += kThreads)
-        if (i % T::kN >= N)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) st(&sm.raw[s].b[i], 0.f), st(&sm.raw[s].c[i], 0.f);
-
     const bool real = ch < at.nch;
     const int64_t d = at.d0 + (real ? ch : 0);
     const F4 a2 = real ? mul(kLog2e, load4(p.a + d * N, kS * q, N)) : zero4();
-    F4 carry = zero4();
-    if (p.state_in && real) carry = load4(p.state_in + (at.b * p.channels + d) * N, kS * q, N);
-    // the output phase: this thread's pair of channels
-    const int oc = 2 * (tid % (kCh / 2));
-    const float bias_pre = p.dt_bias && tid % kCh < at.nch ? p.dt_bias[at.d0 + tid % kCh] : 0.f;
-    const float d0v = p.d && oc < at.nch ? p.d[at.d0 + oc] : 0.f, d1v = p.d && oc + 1 < at.nch ? p.d[at.d0 + oc + 1] : 0.f;
-    const int64_t y0 = at.b * p.y_b + at.d0 + oc;
-    const int64_t ysize = p.y_dt ? 2 : 4;
-    const bool ypair = oc + 1 < at.nch && (reinterpret_cast<uintptr_t>(p.y) + y0 * ysize) % (2 * ysize) == 0 && p.y_t % 2 == 0;
-    auto put = [&](int64_t t, float v0, float v1) {
-        const int64_t o = y0 + t * p.y_t;
-        if (p.y_dt) {
-            __nv_bfloat16 *Y = static_cast<__nv_bfloat16 *>(p.y) + o;
-            if (ypair) *reinterpret_cast<uint32_t *>(Y) = vec::pack(v0, v1);
-            else {
-                if (oc < at.nch) st(Y, v0);
-                if (oc + 1 < at.nch) st(Y + 1, v1);
-            }
-        } else {
-            float *Y = static_cast<float *>(p.y) + o;
-            if (ypair) *reinterpret_cast<float2 *>(Y) = make_float2(v0, v1);
-            else {
-                if (oc < at.nch) Y[0] = v0;
-                if (oc + 1 < at.nch) Y[1] = v1;
-            }
-        }
-    };
-
-    if (len > 0) load_tile(0, 0);
-    int s = 0;
-    for (int64_t t0 = 0, tile = 0; t0 < len; t0 += kTok, ++tile, s ^= 1) {
+    F4 carry = p.state_in && real ? load4(p.state_in + (at.b * p.channels + d) * N, kS * q, N) : zero4();
+    if (len > 0) {
+        wk.template load<kNT, kTok, true>(sm.raw[0], 0, tid);
+        ptx::cp_async_commit();
         ptx::cp_async_wait<0>();
-        __syncthreads();  // the tile has landed, and the last tile's shared values are done with
-        if (t0 + kTok < len) load_tile(t0 + kTok, s ^ 1);
-        const int live = len - t0 < kTok ? (int)(len - t0) : kTok;
-        typename Smem::Raw &w = sm.raw[s];
-        for (int i = tid; i < kTok * kCh; i += kThreads) {  // kThreads is a multiple of kCh: always the same channel
-            float v = ld(&w.dt[i]) + bias_pre;
-            if (p.softplus) v = softplus(v);
-            if (i / kCh >= live) v = 0.f;  // past the end: decay 1, nothing added
-            sm.step[i] = make_float2(v, v * ld(&w.u[i]));
-        }
-        {
-            float *fb = reinterpret_cast<float *>(sm.b), *fc = reinterpret_cast<float *>(sm.c);
-            for (int i = tid; i < kTok * T::kN; i += kThreads) fb[i] = ld(&w.b[i]), fc[i] = ld(&w.c[i]);
-        }
-        if (p.ckpt && seg == 0 && real) store4(p.ckpt + ((at.b * p.tiles + tile) * p.channels + d) * N, kS * q, N, carry);
         __syncthreads();
-
-        F4 av[kK], bv[kK];
-        F4 prod = one4(), h = zero4();
+        prepare(0, 0);
+    }
+    int s = 0;
+    for (int64_t t0 = 0; t0 < len; t0 += kTok, s ^= 1) {
+        __syncthreads();  // this tile's values are ready, the other stage is free
+        if (t0 + kTok < len) wk.template load<kNT, kTok, true>(sm.raw[s ^ 1], t0 + kTok, tid);
+        ptx::cp_async_commit();
+        const int live = len - t0 < kTok ? (int)(len - t0) : kTok;
+#pragma unroll 1
+        for (int sub = 0; sub < kTok; sub += S::kSub) {
+            const int k0 = sub + seg * kK;  // this segment's first token
+            F4 av[kK], bv[kK], prod, h;
 #pragma unroll
-        for (int k = 0; k < kK; ++k) {
-            const int t = seg * kK + k;
-            const float2 sd = sm.step[t * kCh + ch];
-            av[k] = ex2(mul(sd.x, a2));
-            bv[k] = mul(sd.y, f4(sm.b[t * P + q]));
-            if constexpr (T::kSegs > 1) {
-                prod = mul(prod, av[k]);
-                h = fma(av[k], h, bv[k]);
+            for (int k = 0; k < kK; ++k) {
+                const int t = k0 + k;
+                const float2 sd = sm.step[t * CH + ch];
+                av[k] = ex2(mul(sd.x, a2));
+                bv[k] = mul(sd.y, f4(sm.b[t * P + q]));
+                prod = k ? mul(prod, av[k]) : av[k];
+                h = k ? fma(av[k], h, bv[k]) : bv[k];
             }
-        }
-        if constexpr (T::kSegs > 1) {
             sm.decay[tid] = f4(prod);
             sm.end[tid] = f4(h);
             __syncthreads();
             h = carry;
 #pragma unroll
-            for (int i = 0; i < T::kSegs; ++i) {
+            for (int i = 0; i < W; ++i) {
                 if (i == seg) h = carry;
                 carry = fma(f4(sm.decay[i * kLanes + r]), carry, f4(sm.end[i * kLanes + r]));
             }
-        } else {
-            h = carry;
-        }
-        float y[kK];
+            if (p.ckpt && real && k0 < live && (t0 + k0) % Tile<P>::kTokens == 0) checkpoint(p, at, t0 + k0, Tile<P>::kTokens, d, q, h);
+            float *y = sm.y + k0 * kLanes + r;
 #pragma unroll
-        for (int k = 0; k < kK; ++k) {
-            h = fma(av[k], h, bv[k]);
-            y[k] = dot(h, f4(sm.c[(seg * kK + k) * P + q]));
-        }
-        if constexpr (T::kSegs == 1) carry = h;
-        LaneSum<P, 1>::run(y, q);
-        const int first = seg * kK + LaneSum<P, 1>::first(q);
-#pragma unroll
-        for (int k = 0; k < LaneSum<P, 1>::kOut; ++k) sm.y[(first + k) * kCh + ch] = y[k];
-        __syncthreads();
-        for (int i = tid; i < kTok * kCh / 2; i += kThreads) {
-            const int t = i / (kCh / 2);
-            if (t < live) {
-                const float2 yv = *reinterpret_cast<const float2 *>(&sm.y[t * kCh + oc]);
-                float v0 = fmaf(d0v, ld(&w.u[t * kCh + oc]), yv.x), v1 = fmaf(d1v, ld(&w.u[t * kCh + oc + 1]), yv.y);
-                if (Z) {
-                    const float z0 = ld(&w.z[t * kCh + oc]), z1 = ld(&w.z[t * kCh + oc + 1]);
-                    v0 *= z0 * sigmoid(z0), v1 *= z1 * sigmoid(z1);
-                }
-                put(t0 + t, v0, v1);
+            for (int k = 0; k < kK; ++k) {
+                h = fma(av[k], h, bv[k]);
+                y[k * kLanes] = dot(h, f4(sm.c[(k0 + k) * P + q]));
             }
+            if (sub + S::kSub < kTok) __syncthreads();  // decay and end have been read
         }
+        ptx::cp_async_wait<0>();
+        __syncthreads();  // this tile's y is complete, the next tile has landed
+        quads.outputs(sm.y, sm.raw[s].u, wk.Z ? sm.raw[s].z : nullptr, t0, live);
+        if (t0 + kTok < len) prepare(t0 + kTok, s ^ 1);
     }
     if (p.state_out && seg == 0 && real) store4(p.state_out + (at.b * p.channels + d) * N, kS * q, N, carry);
-    for (int64_t t = len + tid / (kCh / 2); t < p.seq; t += kThreads / (kCh / 2)) put(t, 0.f, 0.f);
+    quads.zeros(len, wk.last);
 }
 
 // ------------------------------------------------------------------------------------------------ one token

@@ -87,18 +87,18 @@ __global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(const BwdParams b
         const int nch = at.nch - c0 < kCh ? at.nch - c0 : kCh;
         const int live = len - t0 < kTok ? (int)(len - t0) : kTok;
         typename Smem::RawX &w = sm.x[it & 1];
-        stage_x(w.u, U + t0 * p.u_t + c0, p.u_t, kTok, live, nch, p.vec_x);
-        stage_x(w.dt, D + t0 * p.dt_t + c0, p.dt_t, kTok, live, nch, p.vec_x);
-        if (Z) stage_x(w.z, Z + t0 * p.z_t + c0, p.z_t, kTok, live, nch, p.vec_x);
+        stage_x<kThreads, kCh>(w.u, U + t0 * p.u_t + c0, p.u_t, kTok, live, nch, p.vec_x);
+        stage_x<kThreads, kCh>(w.dt, D + t0 * p.dt_t + c0, p.dt_t, kTok, live, nch, p.vec_x);
+        if (Z) stage_x<kThreads, kCh>(w.z, Z + t0 * p.z_t + c0, p.z_t, kTok, live, nch, p.vec_x);
         if (p.y_dt)
-            stage_x(reinterpret_cast<__nv_bfloat16 *>(w.dy), reinterpret_cast<const __nv_bfloat16 *>(DY) + t0 * bp.dy_t + c0, bp.dy_t, kTok,
+            stage_x<kThreads, kCh>(reinterpret_cast<__nv_bfloat16 *>(w.dy), reinterpret_cast<const __nv_bfloat16 *>(DY) + t0 * bp.dy_t + c0, bp.dy_t, kTok,
                     live, nch, p.vec_x);
         else
-            stage_x(w.dy, reinterpret_cast<const float *>(DY) + t0 * bp.dy_t + c0, bp.dy_t, kTok, live, nch, p.vec_x);
+            stage_x<kThreads, kCh>(w.dy, reinterpret_cast<const float *>(DY) + t0 * bp.dy_t + c0, bp.dy_t, kTok, live, nch, p.vec_x);
         if (sub == 0) {
             typename Smem::RawBC &v = sm.bc[back & 1];
-            stage_bc<TI, T::kN>(v.b, B + t0 * p.b_t, p.b_t, kTok, live, N, p.vec_bc);
-            stage_bc<TI, T::kN>(v.c, C + t0 * p.c_t, p.c_t, kTok, live, N, p.vec_bc);
+            stage_bc<kThreads, T::kN>(v.b, B + t0 * p.b_t, p.b_t, kTok, live, N, p.vec_bc);
+            stage_bc<kThreads, T::kN>(v.c, C + t0 * p.c_t, p.c_t, kTok, live, N, p.vec_bc);
         }
         ptx::cp_async_commit();
     };
