@@ -40,10 +40,10 @@ def _cuda(t: torch.Tensor, what: str, device: Optional[torch.device] = None) -> 
         raise DeltaCoreError(_abi.DC_EDEVICE, f"{what} is on {t.device}, the other tensors on {device}")
 
 
-def _whole(t: Optional[torch.Tensor], what: str, shape, dtype: torch.dtype, device: torch.device):
-    """The address of a contiguous tensor of this shape and dtype (None: no address)."""
+def _whole(t: Optional[torch.Tensor], what: str, shape, dtype: torch.dtype, device: torch.device) -> None:
+    """Refuse what is not a contiguous tensor of this shape and dtype (or None)."""
     if t is None:
-        return None
+        return
     _cuda(t, what, device)
     if t.dtype != dtype:
         raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"{what} must be {dtype}, got {t.dtype}")
@@ -51,7 +51,6 @@ def _whole(t: Optional[torch.Tensor], what: str, shape, dtype: torch.dtype, devi
         raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"{what} has shape {tuple(t.shape)}, want {tuple(shape)}")
     if not t.is_contiguous():
         raise DeltaCoreError(_abi.DC_EINVAL_ARG, f"{what} must be contiguous")
-    return t.data_ptr()
 
 
 def _row_stride(t: torch.Tensor, what: str) -> int:
@@ -85,25 +84,55 @@ def _strides(t: torch.Tensor, what: str, shape, dtype: torch.dtype, device: torc
     return t.stride(0), t.stride(1)
 
 
+# What a call's shapes, strides, dtypes and device decide (the checks, the C arguments without their addresses, the size of the
+# workspace) is worked out once and kept by those: a decode tick would otherwise spend three times its kernel's time on it.
+_PLANS: dict = {}
+_MOST_PLANS = 1024
+
+
+def _sig(t):
+    if t is None:
+        return None
+    try:
+        return t.shape, t.stride(), t.dtype, t.device
+    except AttributeError:
+        raise TypeError(f"a torch.Tensor is wanted, got {type(t).__name__}") from None
+
+
+def _planned(build, *key):
+    """build(), or what it returned for the same key before.  An error is not kept."""
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = build()
+        if len(_PLANS) >= _MOST_PLANS:
+            _PLANS.clear()
+        _PLANS[key] = plan
+    return plan
+
+
+def _on(device: torch.device, fn, *args):
+    """fn(*args) with `device` current."""
+    if torch.cuda.current_device() == device.index:
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
+
+
 def _call(fn, args, device: torch.device, what: str) -> None:
     """Run a C entry point on `device`'s current stream."""
-    if torch.cuda.current_device() == device.index:
-        status = fn(args, torch.cuda.current_stream(device).cuda_stream)
+    stream = torch._C._cuda_getCurrentRawStream(device.index)  # current_stream(device).cuda_stream without the object around it
+    if torch._C._cuda_getDevice() == device.index:
+        status = fn(args, stream)
     else:
         with torch.cuda.device(device):
-            status = fn(args, torch.cuda.current_stream(device).cuda_stream)
+            status = fn(args, stream)
     if status:
         _raise(status, what)
 
 
-def _workspace(size_fn, args, workspace: Optional[torch.Tensor], device: torch.device):
-    """Point `args` at a workspace of the size that `size_fn` asks for; returns the tensor, to be kept until the launch."""
+def _workspace(need: int, args, workspace: Optional[torch.Tensor], device: torch.device):
+    """Point `args` at a workspace of `need` bytes, or the caller's; returns the tensor, to be kept until the launch."""
     if workspace is None:
-        if torch.cuda.current_device() == device.index:
-            need = int(size_fn(args))
-        else:
-            with torch.cuda.device(device):
-                need = int(size_fn(args))
         if need == 0:
             return None
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
@@ -115,36 +144,77 @@ def _workspace(size_fn, args, workspace: Optional[torch.Tensor], device: torch.d
     return workspace
 
 
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
 # ------------------------------------------------------------------------------------------------ residual add + norm
-def _norm_args(x, weight, residual, eps, residual_dtype, residual_out):
-    """The fields that the two outputs' forms share; returns (args, residual_out or x)."""
+def _norm_plan(x, weight, residual, eps, out_dtype, residual_dtype, y_out, residual_out, group):
+    """(C arguments without addresses, dtype of y, dtype of the sum or None where it is x itself); group: None, or of the e4m3 form."""
     _cuda(x, "x")
     if x.dim() < 1:
         raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, "x must have at least one axis")
     width, dev = x.shape[-1], x.device
     a = _abi.RmsNormArgs()
     a.rows, a.width = x.numel() // width if width else 0, width
-    a.eps = float(eps)
-    a.weight = _whole(weight, "weight", (width,), torch.float32, dev)
-    a.x, a.x_dtype, a.x_stride = x.data_ptr(), _code(x.dtype, "x"), _row_stride(x, "x")
+    a.eps = eps
+    _cuda(weight, "weight")
+    _whole(weight, "weight", (width,), torch.float32, dev)
+    a.x_dtype, a.x_stride = _code(x.dtype, "x"), _row_stride(x, "x")
     r_dtype = residual_dtype or (residual.dtype if residual is not None else residual_out.dtype if residual_out is not None else x.dtype)
-    if residual is not None:
-        _cuda(residual, "residual", dev)
-        if residual.shape != x.shape:
-            raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"residual has shape {tuple(residual.shape)}, want {tuple(x.shape)}")
-        if residual.dtype != r_dtype:
-            raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"residual must be {r_dtype}, got {residual.dtype}")
-        a.residual_in, a.residual_in_stride = residual.data_ptr(), _row_stride(residual, "residual")
     a.residual_dtype = _code(r_dtype, "residual")
+    for t, what in ((residual, "residual"), (residual_out, "residual_out")):
+        if t is not None:
+            _cuda(t, what, dev)
+            if t.shape != x.shape:
+                raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"{what} has shape {tuple(t.shape)}, want {tuple(x.shape)}")
+            if t.dtype != r_dtype:
+                raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"{what} must be {r_dtype}, got {t.dtype}")
+    if residual is not None:
+        a.residual_in_stride = _row_stride(residual, "residual")
+    a.residual_out_stride = width if residual_out is None else _row_stride(residual_out, "residual_out")
     if residual is None and residual_out is None and r_dtype == x.dtype:
-        return a, x  # the sum is x itself
-    if residual_out is None:
-        residual_out = torch.empty(x.shape, device=dev, dtype=r_dtype)
-    _cuda(residual_out, "residual_out", dev)
-    if residual_out.shape != x.shape or residual_out.dtype != r_dtype:
-        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"residual_out must be {r_dtype}, shaped like x")
-    a.residual_out, a.residual_out_stride = residual_out.data_ptr(), _row_stride(residual_out, "residual_out")
-    return a, residual_out
+        r_dtype = None
+    if group is None:
+        y_dtype = y_out.dtype if y_out is not None else out_dtype or x.dtype
+        a.out_dtype, a.y_stride = _code(y_dtype, "y"), width
+        if y_out is not None:
+            _cuda(y_out, "y_out", dev)
+            if y_out.shape != x.shape or (out_dtype is not None and y_out.dtype != out_dtype):
+                raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, "y_out must be shaped like x, in out_dtype")
+            a.y_stride = _row_stride(y_out, "y_out")
+    else:
+        if group not in (0, 32, 64, 128, 256):
+            raise DeltaShapeError(_abi.DC_EINVAL_WIDTH, f"group must be 0, 32, 64, 128 or 256, got {group}")
+        if group and width % group:
+            raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"group {group} does not divide the width {width}")
+        y_dtype = torch.float8_e4m3fn
+        a.out_dtype, a.y_stride, a.group = _abi.DC_E4M3, width, group
+    return a, y_dtype, r_dtype
+
+
+def _norm(x, weight, residual, eps, out_dtype, residual_dtype, y_out, residual_out, group):
+    """add_rms_norm's and add_rms_norm_f8's call: (y, scale, r)."""
+    eps = float(eps)
+    proto, y_dtype, r_dtype = _planned(
+        lambda: _norm_plan(x, weight, residual, eps, out_dtype, residual_dtype, y_out, residual_out, group),
+        "norm", _sig(x), _sig(weight), _sig(residual), eps, out_dtype, residual_dtype, _sig(y_out), _sig(residual_out), group)
+    a = _abi.RmsNormArgs.from_buffer_copy(proto)
+    dev = x.device
+    y = torch.empty(x.shape, device=dev, dtype=y_dtype) if y_out is None else y_out
+    scale = None
+    if group is not None:
+        scale = torch.empty((*x.shape[:-1], x.shape[-1] // group if group else 1), device=dev, dtype=torch.float32)
+        a.scale = scale.data_ptr()
+    r = x
+    if r_dtype is not None:
+        r = torch.empty(x.shape, device=dev, dtype=r_dtype) if residual_out is None else residual_out
+        a.residual_out = r.data_ptr()
+    a.x, a.weight, a.y = x.data_ptr(), weight.data_ptr(), y.data_ptr()
+    if residual is not None:
+        a.residual_in = residual.data_ptr()
+    _call(_abi.lib().dc_rms_norm, a, dev, "dc_rms_norm")
+    return y, scale, r
 
 
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-5, *,
@@ -158,14 +228,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     sum in ``residual_dtype`` (default: ``residual``'s), the next layer's ``residual``; without a residual ``r`` is ``x``.
     ``y`` is made from the sum before ``r``'s rounding.  ``residual_out`` may be ``residual`` and ``y_out`` may be ``x``.
     """
-    a, r = _norm_args(x, weight, residual, eps, residual_dtype, residual_out)
-    y = y_out if y_out is not None else torch.empty(x.shape, device=x.device, dtype=out_dtype or x.dtype)
-    if y_out is not None:
-        _cuda(y, "y_out", x.device)
-        if y.shape != x.shape or (out_dtype is not None and y.dtype != out_dtype):
-            raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, "y_out must be shaped like x, in out_dtype")
-    a.y, a.out_dtype, a.y_stride = y.data_ptr(), _code(y.dtype, "y"), _row_stride(y, "y_out")
-    _call(_abi.lib().dc_rms_norm, a, x.device, "dc_rms_norm")
+    y, _, r = _norm(x, weight, residual, eps, out_dtype, residual_dtype, y_out, residual_out, None)
     return y, r
 
 
@@ -174,18 +237,34 @@ def add_rms_norm_f8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[to
     """:func:`add_rms_norm` with ``y`` in 8 bits: returns ``(q, scale, r)``, ``y = q * scale`` with ``q`` float8_e4m3fn shaped
     like ``x`` and one float32 scale, ``max|y| / 448``, per ``group`` consecutive columns (32, 64, 128 or 256 dividing the
     width; 0: per row).  ``scale`` is ``x``'s shape with the last axis ``width / group`` (1 per row)."""
-    a, r = _norm_args(x, weight, residual, eps, residual_dtype, residual_out)
-    width = x.shape[-1]
-    group = int(group)
-    if group not in (0, 32, 64, 128, 256):
-        raise DeltaShapeError(_abi.DC_EINVAL_WIDTH, f"group must be 0, 32, 64, 128 or 256, got {group}")
-    if group and width % group:
-        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"group {group} does not divide the width {width}")
-    q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
-    scale = torch.empty((*x.shape[:-1], width // group if group else 1), device=x.device, dtype=torch.float32)
-    a.y, a.out_dtype, a.y_stride, a.group, a.scale = q.data_ptr(), _abi.DC_E4M3, width, group, scale.data_ptr()
-    _call(_abi.lib().dc_rms_norm, a, x.device, "dc_rms_norm")
-    return q, scale, r
+    return _norm(x, weight, residual, eps, None, residual_dtype, None, residual_out, int(group))
+
+
+def _norm_bwd_plan(d_y, d_r, r, weight, eps, x_dtype):
+    """(C arguments without addresses, dtype of d_x or None where d_residual is it, bytes of workspace)."""
+    _cuda(r, "r")
+    dev, width = r.device, r.shape[-1]
+    _cuda(d_y, "d_y", dev)
+    if d_y.shape != r.shape or (d_r is not None and d_r.shape != r.shape):
+        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, "d_y and d_r must be shaped like r")
+    a = _abi.RmsNormBwdArgs()
+    a.rows, a.width, a.eps = r.numel() // width if width else 0, width, eps
+    _cuda(weight, "weight")
+    _whole(weight, "weight", (width,), torch.float32, dev)
+    a.r_dtype, a.r_stride = _code(r.dtype, "r"), _row_stride(r, "r")
+    a.y_dtype, a.d_y_stride = _code(d_y.dtype, "d_y"), _row_stride(d_y, "d_y")
+    if d_r is not None:
+        _cuda(d_r, "d_r", dev)
+        if d_r.dtype != r.dtype:
+            raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"d_r must be {r.dtype}, got {d_r.dtype}")
+        a.d_r_stride = _row_stride(d_r, "d_r")
+    a.d_residual_stride = width
+    other = x_dtype is not None and x_dtype != r.dtype
+    if other:
+        a.d_x_stride, a.x_dtype = width, _code(x_dtype, "x_dtype")
+    a.d_weight = 16  # stands for the buffer in the query
+    need = int(_on(dev, _abi.lib().dc_rms_norm_bwd_workspace_size, a))
+    return a, x_dtype if other else None, need
 
 
 def add_rms_norm_backward(d_y: torch.Tensor, d_r: Optional[torch.Tensor], r: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *,
@@ -193,32 +272,20 @@ def add_rms_norm_backward(d_y: torch.Tensor, d_r: Optional[torch.Tensor], r: tor
     """The backward of :func:`add_rms_norm` (``dc_rms_norm_bwd``) from its ``r``: returns ``(d_x, d_residual, d_weight)``,
     ``d_x`` in ``x_dtype`` (default: ``r``'s), ``d_residual`` in ``r``'s dtype (the same tensor where the dtypes are equal: the
     two gradients are), ``d_weight`` float32.  ``d_r`` is the gradient of the returned sum, in ``r``'s dtype (``None``: zero)."""
-    _cuda(r, "r")
-    dev, width = r.device, r.shape[-1]
-    _cuda(d_y, "d_y", dev)
-    if d_y.shape != r.shape or (d_r is not None and d_r.shape != r.shape):
-        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, "d_y and d_r must be shaped like r")
-    a = _abi.RmsNormBwdArgs()
-    a.rows, a.width, a.eps = r.numel() // width if width else 0, width, float(eps)
-    a.weight = _whole(weight, "weight", (width,), torch.float32, dev)
-    a.r, a.r_dtype, a.r_stride = r.data_ptr(), _code(r.dtype, "r"), _row_stride(r, "r")
-    a.d_y, a.y_dtype, a.d_y_stride = d_y.data_ptr(), _code(d_y.dtype, "d_y"), _row_stride(d_y, "d_y")
-    if d_r is not None:
-        _cuda(d_r, "d_r", dev)
-        if d_r.dtype != r.dtype:
-            raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"d_r must be {r.dtype}, got {d_r.dtype}")
-        a.d_r, a.d_r_stride = d_r.data_ptr(), _row_stride(d_r, "d_r")
-    d_residual = torch.empty(r.shape, device=dev, dtype=r.dtype)
-    a.d_residual, a.d_residual_stride = d_residual.data_ptr(), width
-    d_x = d_residual
-    if x_dtype is not None and x_dtype != r.dtype:
-        d_x = torch.empty(r.shape, device=dev, dtype=x_dtype)
-        a.d_x, a.d_x_stride, a.x_dtype = d_x.data_ptr(), width, _code(x_dtype, "x_dtype")
-    d_weight = torch.empty(width, device=dev, dtype=torch.float32)
-    a.d_weight = d_weight.data_ptr()
-    L = _abi.lib()
-    keep = _workspace(L.dc_rms_norm_bwd_workspace_size, a, workspace, dev)
-    _call(L.dc_rms_norm_bwd, a, dev, "dc_rms_norm_bwd")
+    eps = float(eps)
+    proto, other, need = _planned(lambda: _norm_bwd_plan(d_y, d_r, r, weight, eps, x_dtype),
+                                  "norm_bwd", _sig(d_y), _sig(d_r), _sig(r), _sig(weight), eps, x_dtype)
+    a = _abi.RmsNormBwdArgs.from_buffer_copy(proto)
+    dev = r.device
+    d_x = d_residual = torch.empty(r.shape, device=dev, dtype=r.dtype)
+    if other is not None:
+        d_x = torch.empty(r.shape, device=dev, dtype=other)
+        a.d_x = d_x.data_ptr()
+    d_weight = torch.empty(r.shape[-1], device=dev, dtype=torch.float32)
+    a.d_y, a.d_r, a.r, a.weight = d_y.data_ptr(), _ptr(d_r), r.data_ptr(), weight.data_ptr()
+    a.d_residual, a.d_weight = d_residual.data_ptr(), d_weight.data_ptr()
+    keep = _workspace(need, a, workspace, dev)
+    _call(_abi.lib().dc_rms_norm_bwd, a, dev, "dc_rms_norm_bwd")
     del keep
     return d_x, d_residual, d_weight
 
@@ -244,25 +311,57 @@ class AddRmsNormFunction(torch.autograd.Function):
 
 
 # ------------------------------------------------------------------------------------------------ causal convolution
-def _conv_args(a, x, weight, bias, window, silu, lengths):
-    """The forward's and the backward's common fields, for x [batch, seq, channels]."""
+def _conv_dims(a, x, weight, bias, window, silu, lengths):
+    """The forward's and the backward's common checks and fields, for x [batch, seq, channels]."""
     _cuda(x, "x")
     if x.dim() != 3:
         raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"x must be [batch, seq, channels], got {tuple(x.shape)}")
     b, s, c = x.shape
     dev = x.device
-    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+    if weight is None or weight.dim() != 2:
         raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"weight must be [{c}, taps]")
     k = weight.shape[1]
     a.batch, a.seq, a.channels, a.taps = b, s, c, k
     a.in_dtype = _code(x.dtype, "x")
     a.flags = _abi.DC_CONV_SILU if silu else 0
     a.x_batch_stride, a.x_token_stride = _strides(x, "x", (b, s, c), x.dtype, dev)
-    a.x = x.data_ptr()
-    a.weight = _whole(weight, "weight", (c, k), torch.float32, dev)
-    a.bias = _whole(bias, "bias", (c,), torch.float32, dev)
-    a.window_in = _whole(window, "window", (b, c, k), torch.float32, dev)
-    a.lengths = _whole(lengths, "lengths", (b,), torch.int32, dev)
+    _whole(weight, "weight", (c, k), torch.float32, dev)
+    _whole(bias, "bias", (c,), torch.float32, dev)
+    _whole(window, "window", (b, c, k), torch.float32, dev)
+    _whole(lengths, "lengths", (b,), torch.int32, dev)
+
+
+def _conv_plan(x, weight, bias, window, silu, lengths, out_dtype, y_out, window_out, step):
+    """(C arguments without addresses, dtype of y)."""
+    if step:
+        if x is None or x.dim() != 2:
+            raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, "x must be [batch, channels]")
+        x, y_out = x.unsqueeze(1), None if y_out is None else y_out.unsqueeze(1)
+    a = _abi.CausalConvArgs()
+    _conv_dims(a, x, weight, bias, window, silu, lengths)
+    b, s, c = x.shape
+    dtype = y_out.dtype if y_out is not None else out_dtype or x.dtype
+    if out_dtype is not None and dtype != out_dtype:
+        raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"y_out must be {out_dtype}")
+    a.y_batch_stride, a.y_token_stride = (s * c, c) if y_out is None else _strides(y_out, "y_out", (b, s, c), dtype, x.device)
+    a.out_dtype = _code(dtype, "y")
+    _whole(window_out, "window_out", (b, c, weight.shape[1]), torch.float32, x.device)
+    return a, dtype
+
+
+def _conv(x, weight, bias, window, silu, lengths, out_dtype, y_out, window_out, step):
+    """causal_conv's and causal_conv_step's call."""
+    proto, dtype = _planned(lambda: _conv_plan(x, weight, bias, window, silu, lengths, out_dtype, y_out, window_out, step),
+                            "conv", step, _sig(x), _sig(weight), _sig(bias), _sig(window), bool(silu), _sig(lengths), out_dtype,
+                            _sig(y_out), _sig(window_out))
+    a = _abi.CausalConvArgs.from_buffer_copy(proto)
+    dev = x.device
+    y = torch.empty(x.shape, device=dev, dtype=dtype) if y_out is None else y_out
+    nxt = torch.empty((a.batch, a.channels, a.taps), device=dev, dtype=torch.float32) if window_out is None else window_out
+    a.x, a.weight, a.bias, a.window_in, a.lengths = x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(window), _ptr(lengths)
+    a.y, a.window_out = y.data_ptr(), nxt.data_ptr()
+    _call(_abi.lib().dc_causal_conv, a, dev, "dc_causal_conv")
+    return y, nxt
 
 
 def causal_conv(x_bsc: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, window: Optional[torch.Tensor] = None, *,
@@ -275,19 +374,7 @@ def causal_conv(x_bsc: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.
     columns, as :func:`~.core.qkv_prologue`'s does.  ``lengths`` (int32 ``[batch]``) ends each sequence early: the padding is
     not read and its ``y`` is zero.  ``x`` may be a column slice.  Returns ``(y, next window)``.
     """
-    a = _abi.CausalConvArgs()
-    _conv_args(a, x_bsc, weight, bias, window, silu, lengths)
-    b, s, c = x_bsc.shape
-    dev = x_bsc.device
-    y = y_out if y_out is not None else torch.empty(b, s, c, device=dev, dtype=out_dtype or x_bsc.dtype)
-    if out_dtype is not None and y.dtype != out_dtype:
-        raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"y_out must be {out_dtype}")
-    nxt = window_out if window_out is not None else torch.empty(b, c, weight.shape[1], device=dev, dtype=torch.float32)
-    a.y_batch_stride, a.y_token_stride = _strides(y, "y_out", (b, s, c), y.dtype, dev)
-    a.y, a.out_dtype = y.data_ptr(), _code(y.dtype, "y")
-    a.window_out = _whole(nxt, "window_out", (b, c, weight.shape[1]), torch.float32, dev)
-    _call(_abi.lib().dc_causal_conv, a, dev, "dc_causal_conv")
-    return y, nxt
+    return _conv(x_bsc, weight, bias, window, silu, lengths, out_dtype, y_out, window_out, False)
 
 
 def causal_conv_step(x_bc: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, window: Optional[torch.Tensor] = None, *,
@@ -295,11 +382,20 @@ def causal_conv_step(x_bc: torch.Tensor, weight: torch.Tensor, bias: Optional[to
                      window_out: Optional[torch.Tensor] = None):
     """:func:`causal_conv` for one token per sequence: ``x [batch, channels]`` to ``(y [batch, channels], next window)``; pass
     ``window_out=window`` to roll the window in place."""
-    if not isinstance(x_bc, torch.Tensor) or x_bc.dim() != 2:
-        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, "x must be [batch, channels]")
-    y, nxt = causal_conv(x_bc.unsqueeze(1), weight, bias, window, silu=silu, out_dtype=out_dtype,
-                         y_out=None if y_out is None else y_out.unsqueeze(1), window_out=window_out)
-    return (y.squeeze(1) if y_out is None else y_out), nxt
+    return _conv(x_bc, weight, bias, window, silu, None, out_dtype, y_out, window_out, True)
+
+
+def _conv_bwd_plan(d_y, d_window_out, x, weight, bias, window, silu, lengths):
+    """(C arguments without addresses, bytes of workspace)."""
+    a = _abi.CausalConvBwdArgs()
+    _conv_dims(a, x, weight, bias, window, silu, lengths)
+    b, s, c = x.shape
+    _cuda(d_y, "d_y", x.device)
+    a.out_dtype = _code(d_y.dtype, "d_y")
+    a.d_y_batch_stride, a.d_y_token_stride = _strides(d_y, "d_y", (b, s, c), d_y.dtype, x.device)
+    _whole(d_window_out, "d_window_out", (b, c, weight.shape[1]), torch.float32, x.device)
+    a.d_x_batch_stride, a.d_x_token_stride = s * c, c
+    return a, int(_on(x.device, _abi.lib().dc_causal_conv_bwd_workspace_size, a))
 
 
 def causal_conv_backward(d_y: torch.Tensor, d_window_out: Optional[torch.Tensor], x_bsc: torch.Tensor, weight: torch.Tensor,
@@ -308,26 +404,20 @@ def causal_conv_backward(d_y: torch.Tensor, d_window_out: Optional[torch.Tensor]
     """The backward of :func:`causal_conv` (``dc_causal_conv_bwd``), given ``d_y`` and the gradient of the returned window
     (``None``: zero): returns ``(d_x, d_weight, d_bias, d_window)``, ``d_x`` in ``x``'s dtype, the others float32; ``d_bias`` and
     ``d_window`` are ``None`` where ``bias`` and ``window`` are."""
-    a = _abi.CausalConvBwdArgs()
-    _conv_args(a, x_bsc, weight, bias, window, silu, lengths)
-    b, s, c = x_bsc.shape
-    dev, k = x_bsc.device, weight.shape[1]
-    _cuda(d_y, "d_y", dev)
-    a.out_dtype = _code(d_y.dtype, "d_y")
-    a.d_y_batch_stride, a.d_y_token_stride = _strides(d_y, "d_y", (b, s, c), d_y.dtype, dev)
-    a.d_y = d_y.data_ptr()
-    a.d_window_out = _whole(d_window_out, "d_window_out", (b, c, k), torch.float32, dev)
-    d_x = torch.empty(b, s, c, device=dev, dtype=x_bsc.dtype)
-    d_weight = torch.empty(c, k, device=dev, dtype=torch.float32)
-    d_bias = None if bias is None else torch.empty(c, device=dev, dtype=torch.float32)
-    d_window = None if window is None else torch.empty(b, c, k, device=dev, dtype=torch.float32)
-    a.d_x, a.d_x_batch_stride, a.d_x_token_stride = d_x.data_ptr(), s * c, c
-    a.d_weight = d_weight.data_ptr()
-    a.d_bias = None if d_bias is None else d_bias.data_ptr()
-    a.d_window_in = None if d_window is None else d_window.data_ptr()
-    L = _abi.lib()
-    keep = _workspace(L.dc_causal_conv_bwd_workspace_size, a, workspace, dev)
-    _call(L.dc_causal_conv_bwd, a, dev, "dc_causal_conv_bwd")
+    proto, need = _planned(lambda: _conv_bwd_plan(d_y, d_window_out, x_bsc, weight, bias, window, silu, lengths),
+                           "conv_bwd", _sig(d_y), _sig(d_window_out), _sig(x_bsc), _sig(weight), _sig(bias), _sig(window), bool(silu),
+                           _sig(lengths))
+    a = _abi.CausalConvBwdArgs.from_buffer_copy(proto)
+    dev = x_bsc.device
+    d_x = torch.empty(x_bsc.shape, device=dev, dtype=x_bsc.dtype)
+    d_weight = torch.empty(weight.shape, device=dev, dtype=torch.float32)
+    d_bias = None if bias is None else torch.empty(bias.shape, device=dev, dtype=torch.float32)
+    d_window = None if window is None else torch.empty(window.shape, device=dev, dtype=torch.float32)
+    a.d_y, a.d_window_out, a.x, a.weight, a.bias = d_y.data_ptr(), _ptr(d_window_out), x_bsc.data_ptr(), weight.data_ptr(), _ptr(bias)
+    a.window_in, a.lengths = _ptr(window), _ptr(lengths)
+    a.d_x, a.d_weight, a.d_bias, a.d_window_in = d_x.data_ptr(), d_weight.data_ptr(), _ptr(d_bias), _ptr(d_window)
+    keep = _workspace(need, a, workspace, dev)
+    _call(_abi.lib().dc_causal_conv_bwd, a, dev, "dc_causal_conv_bwd")
     del keep
     return d_x, d_weight, d_bias, d_window
 
@@ -365,8 +455,8 @@ def _bc(t, what, b, s, dtype, dev):
     return g, n, t.stride(0), t.stride(1)
 
 
-def _scan_args(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths):
-    """dc_selective_scan_args but for the outputs, for u [batch, seq, channels]."""
+def _scan_dims(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths):
+    """dc_selective_scan_args without addresses and outputs, for u [batch, seq, channels]."""
     _cuda(u, "u")
     if u.dim() != 3:
         raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, f"u must be [batch, seq, channels], got {tuple(u.shape)}")
@@ -383,28 +473,64 @@ def _scan_args(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths):
     g.dt_batch_stride, g.dt_token_stride = _strides(dt, "dt", (bs, s, ch), dtype, dev)
     if z is not None:
         g.z_batch_stride, g.z_token_stride = _strides(z, "z", (bs, s, ch), dtype, dev)
-        g.z = z.data_ptr()
     g.flags = _abi.DC_SCAN_SOFTPLUS if softplus else 0
-    g.u, g.dt, g.b, g.c = u.data_ptr(), dt.data_ptr(), b.data_ptr(), c.data_ptr()
-    g.a = _whole(a, "a", (ch, n), torch.float32, dev)
-    g.d = _whole(d, "d", (ch,), torch.float32, dev)
-    g.dt_bias = _whole(dt_bias, "dt_bias", (ch,), torch.float32, dev)
-    g.state_in = _whole(state, "state", (bs, ch, n), torch.float32, dev)
-    g.lengths = _whole(lengths, "lengths", (bs,), torch.int32, dev)
+    _cuda(a, "a")
+    _whole(a, "a", (ch, n), torch.float32, dev)
+    _whole(d, "d", (ch,), torch.float32, dev)
+    _whole(dt_bias, "dt_bias", (ch,), torch.float32, dev)
+    _whole(state, "state", (bs, ch, n), torch.float32, dev)
+    _whole(lengths, "lengths", (bs,), torch.int32, dev)
     return g
 
 
-def _scan_outputs(g, u, out_dtype, y_out, state_out):
-    dev = u.device
-    shape = (g.batch, g.seq, g.channels)
-    y = y_out if y_out is not None else torch.empty(shape, device=dev, dtype=out_dtype or u.dtype)
-    if out_dtype is not None and y.dtype != out_dtype:
+def _scan_plan(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths, out_dtype, y_out, state_out, step):
+    """(C arguments without addresses, dtype of y, bytes of checkpoints, bytes of workspace)."""
+    if step:
+        if u is None or u.dim() != 2:
+            raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, "u must be [batch, channels]")
+        one = lambda t: None if t is None else t.unsqueeze(1)
+        u, dt, b, c, z, y_out = one(u), one(dt), one(b), one(c), one(z), one(y_out)
+    g = _scan_dims(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths)
+    dev, shape = u.device, (g.batch, g.seq, g.channels)
+    dtype = y_out.dtype if y_out is not None else out_dtype or u.dtype
+    if out_dtype is not None and dtype != out_dtype:
         raise DeltaCoreError(_abi.DC_EUNSUPPORTED_DTYPE, f"y_out must be {out_dtype}")
-    h = state_out if state_out is not None else torch.empty(g.batch, g.channels, g.state, device=dev, dtype=torch.float32)
-    g.y_batch_stride, g.y_token_stride = _strides(y, "y_out", shape, y.dtype, dev)
-    g.y, g.out_dtype = y.data_ptr(), _code(y.dtype, "y")
-    g.state_out = _whole(h, "state_out", (g.batch, g.channels, g.state), torch.float32, dev)
-    return y, h
+    strides = (g.seq * g.channels, g.channels) if y_out is None else _strides(y_out, "y_out", shape, dtype, dev)
+    g.y_batch_stride, g.y_token_stride = strides
+    g.out_dtype = _code(dtype, "y")
+    _whole(state_out, "state_out", (g.batch, g.channels, g.state), torch.float32, dev)
+    L = _abi.lib()
+    return g, dtype, int(L.dc_selective_scan_checkpoint_size(g)), 0 if step else int(_on(dev, L.dc_selective_scan_workspace_size, g))
+
+
+def _scan(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths, out_dtype, y_out, state_out, step, checkpoints, workspace):
+    """selective_scan's and selective_scan_step's call: (y, final state, checkpoints or None)."""
+    proto, dtype, saves, need = _planned(
+        lambda: _scan_plan(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths, out_dtype, y_out, state_out, step),
+        "scan", step, _sig(u), _sig(dt), _sig(a), _sig(b), _sig(c), _sig(d), _sig(z), _sig(dt_bias), _sig(state), bool(softplus),
+        _sig(lengths), out_dtype, _sig(y_out), _sig(state_out))
+    g = _abi.SelectiveScanArgs.from_buffer_copy(proto)
+    dev = u.device
+    y = torch.empty(u.shape, device=dev, dtype=dtype) if y_out is None else y_out
+    h = torch.empty((g.batch, g.channels, g.state), device=dev, dtype=torch.float32) if state_out is None else state_out
+    _scan_inputs(g, u, dt, a, b, c, d, z, dt_bias, state, lengths)
+    g.y, g.state_out = y.data_ptr(), h.data_ptr()
+    saved = keep = None
+    if checkpoints:
+        saved = torch.empty(saves // 4, device=dev, dtype=torch.float32)
+        g.checkpoints = saved.data_ptr()
+    if step:
+        _call(_abi.lib().dc_selective_scan_step, g, dev, "dc_selective_scan_step")
+    else:
+        keep = _workspace(need, g, workspace, dev)
+        _call(_abi.lib().dc_selective_scan, g, dev, "dc_selective_scan")
+    del keep
+    return y, h, saved
+
+
+def _scan_inputs(g, u, dt, a, b, c, d, z, dt_bias, state, lengths):
+    g.u, g.dt, g.a, g.b, g.c = u.data_ptr(), dt.data_ptr(), a.data_ptr(), b.data_ptr(), c.data_ptr()
+    g.d, g.z, g.dt_bias, g.state_in, g.lengths = _ptr(d), _ptr(z), _ptr(dt_bias), _ptr(state), _ptr(lengths)
 
 
 def selective_scan(u: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, d: Optional[torch.Tensor] = None,
@@ -426,16 +552,7 @@ def selective_scan(u: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
     ``(y, final state)``, with ``checkpoints=True`` also what :func:`selective_scan_backward` starts from.  ``state_out`` may be
     ``state``; ``softplus=False`` takes ``dt + dt_bias`` as it is.
     """
-    g = _scan_args(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths)
-    y, h = _scan_outputs(g, u, out_dtype, y_out, state_out)
-    L = _abi.lib()
-    saved = None
-    if checkpoints:
-        saved = torch.empty(int(L.dc_selective_scan_checkpoint_size(g)) // 4, device=u.device, dtype=torch.float32)
-        g.checkpoints = saved.data_ptr()
-    keep = _workspace(L.dc_selective_scan_workspace_size, g, workspace, u.device)
-    _call(L.dc_selective_scan, g, u.device, "dc_selective_scan")
-    del keep
+    y, h, saved = _scan(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths, out_dtype, y_out, state_out, False, checkpoints, workspace)
     return (y, h, saved) if checkpoints else (y, h)
 
 
@@ -446,13 +563,23 @@ def selective_scan_step(u: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: t
     """:func:`selective_scan` for one token per sequence (``dc_selective_scan_step``): ``u``, ``dt``, ``z [batch, channels]``, ``b``,
     ``c [batch, groups, state]`` or ``[batch, state]``; returns ``(y [batch, channels], next state)``.  Pass ``state_out=state`` to
     update the state in place."""
-    if not isinstance(u, torch.Tensor) or u.dim() != 2:
-        raise DeltaShapeError(_abi.DC_EINVAL_SHAPE, "u must be [batch, channels]")
-    one = lambda t: t.unsqueeze(1) if isinstance(t, torch.Tensor) else t
-    g = _scan_args(one(u), one(dt), a, one(b), one(c), d, one(z), dt_bias, state, softplus, None)
-    y, h = _scan_outputs(g, u, out_dtype, one(y_out), state_out)
-    _call(_abi.lib().dc_selective_scan_step, g, u.device, "dc_selective_scan_step")
-    return (y.squeeze(1) if y_out is None else y_out), h
+    y, h, _ = _scan(u, dt, a, b, c, d, z, dt_bias, state, softplus, None, out_dtype, y_out, state_out, True, False, None)
+    return y, h
+
+
+def _scan_bwd_plan(d_y, d_state, u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths, checkpoints):
+    """(C arguments without addresses, bytes of workspace)."""
+    g = _scan_dims(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths)
+    dev, shape = u.device, (g.batch, g.seq, g.channels)
+    L = _abi.lib()
+    _whole(checkpoints, "checkpoints", (int(L.dc_selective_scan_checkpoint_size(g)) // 4,), torch.float32, dev)
+    _cuda(d_y, "d_y", dev)
+    g.out_dtype = _code(d_y.dtype, "d_y")
+    w = _abi.SelectiveScanBwdArgs()
+    w.d_y_batch_stride, w.d_y_token_stride = _strides(d_y, "d_y", shape, d_y.dtype, dev)
+    _whole(d_state, "d_state", (g.batch, g.channels, g.state), torch.float32, dev)
+    w.fwd = g
+    return w, int(_on(dev, L.dc_selective_scan_bwd_workspace_size, w))
 
 
 def selective_scan_backward(d_y: torch.Tensor, d_state: Optional[torch.Tensor], u: torch.Tensor, dt: torch.Tensor, a: torch.Tensor,
@@ -466,30 +593,22 @@ def selective_scan_backward(d_y: torch.Tensor, d_state: Optional[torch.Tensor], 
     float32, ``None`` where the input is."""
     if checkpoints is None:
         checkpoints = selective_scan(u, dt, a, b, c, d, z, dt_bias, state, softplus=softplus, lengths=lengths, checkpoints=True)[2]
-    w = _abi.SelectiveScanBwdArgs()
-    g = _scan_args(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths)
+    proto, need = _planned(
+        lambda: _scan_bwd_plan(d_y, d_state, u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths, checkpoints),
+        "scan_bwd", _sig(d_y), _sig(d_state), _sig(u), _sig(dt), _sig(a), _sig(b), _sig(c), _sig(d), _sig(z), _sig(dt_bias), _sig(state),
+        bool(softplus), _sig(lengths), _sig(checkpoints))
+    w = _abi.SelectiveScanBwdArgs.from_buffer_copy(proto)
+    _scan_inputs(w.fwd, u, dt, a, b, c, d, z, dt_bias, state, lengths)
+    w.fwd.checkpoints = checkpoints.data_ptr()
     dev, dtype = u.device, u.dtype
-    shape = (g.batch, g.seq, g.channels)
-    L = _abi.lib()
-    g.checkpoints = _whole(checkpoints, "checkpoints", (int(L.dc_selective_scan_checkpoint_size(g)) // 4,), torch.float32, dev)
-    _cuda(d_y, "d_y", dev)
-    g.out_dtype = _code(d_y.dtype, "d_y")
-    w.d_y_batch_stride, w.d_y_token_stride = _strides(d_y, "d_y", shape, d_y.dtype, dev)
-    w.d_y = d_y.data_ptr()
-    w.d_state_out = _whole(d_state, "d_state", (g.batch, g.channels, g.state), torch.float32, dev)
-    new = lambda shape, dt=torch.float32: torch.empty(shape, device=dev, dtype=dt)
-    d_u, d_dt, d_z = new(shape, dtype), new(shape, dtype), None if z is None else new(shape, dtype)
-    d_b, d_c = new(b.shape, dtype), new(c.shape, dtype)
-    d_a = new((g.channels, g.state))
-    d_d, d_dt_bias = None if d is None else new(g.channels), None if dt_bias is None else new(g.channels)
-    d_state_in = None if state is None else new((g.batch, g.channels, g.state))
-    for name, t in (("d_u", d_u), ("d_dt", d_dt), ("d_a", d_a), ("d_b", d_b), ("d_c", d_c), ("d_d", d_d), ("d_z", d_z),
-                    ("d_dt_bias", d_dt_bias), ("d_state_in", d_state_in)):
-        if t is not None:
-            setattr(w, name, t.data_ptr())
-    w.fwd = g
-    keep = _workspace(L.dc_selective_scan_bwd_workspace_size, w, workspace, dev)
-    _call(L.dc_selective_scan_bwd, w, dev, "dc_selective_scan_bwd")
+    like = lambda t, dtype=torch.float32: None if t is None else torch.empty(t.shape, device=dev, dtype=dtype)
+    d_u, d_dt, d_z, d_b, d_c = like(u, dtype), like(dt, dtype), like(z, dtype), like(b, dtype), like(c, dtype)
+    d_a, d_d, d_dt_bias, d_state_in = like(a), like(d), like(dt_bias), like(state)
+    w.d_y, w.d_state_out = d_y.data_ptr(), _ptr(d_state)
+    w.d_u, w.d_dt, w.d_a, w.d_b, w.d_c, w.d_d = d_u.data_ptr(), d_dt.data_ptr(), d_a.data_ptr(), d_b.data_ptr(), d_c.data_ptr(), _ptr(d_d)
+    w.d_z, w.d_dt_bias, w.d_state_in = _ptr(d_z), _ptr(d_dt_bias), _ptr(d_state_in)
+    keep = _workspace(need, w, workspace, dev)
+    _call(_abi.lib().dc_selective_scan_bwd, w, dev, "dc_selective_scan_bwd")
     del keep
     return d_u, d_dt, d_a, d_b, d_c, d_d, d_z, d_dt_bias, d_state_in
 
