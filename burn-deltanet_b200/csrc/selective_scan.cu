@@ -107,7 +107,7 @@ extern "C" {
 
 uint64_t dc_selective_scan_checkpoint_size(const dc_selective_scan_args *a) {
     if (sc::validate_dims(a) != DC_OK) return 0;
-    return (uint64_t)a->batch * (uint64_t)ceil_div(a->seq, sc::tile_tokens(a->state)) * (uint64_t)a->channels * (uint64_t)a->state * 4;
+    return (uint64_t)a->batch * (uint64_t)ceil_div(a->seq, sc::kTile) * (uint64_t)a->channels * (uint64_t)a->state * 4;
 }
 
 uint64_t dc_selective_scan_workspace_size(const dc_selective_scan_args *a) {

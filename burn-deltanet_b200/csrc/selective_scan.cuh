@@ -29,19 +29,12 @@
 namespace dc {
 namespace scan {
 
-constexpr int kThreads = 256;  // of the step and the backward
-constexpr int kCh = 16;        // channels of a block in the backward
+constexpr int kThreads = 256;  // of the step
 constexpr int kK = 8;          // tokens of a segment
 constexpr int kS = 4;          // states of a thread
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// The backward's tile; the forward's checkpoints are at its first tokens.
-template <int P>
-struct Tile {
-    static constexpr int kSegs = kThreads / (kCh * P);  // 16 / P
-    static constexpr int kTokens = kSegs * kK;
-    static constexpr int kN = kS * P;  // padded states
-};
+constexpr int kTile = 16;  // tokens of the walk's and the backward's tiles, and between two checkpoints
 
 struct Params {
     int64_t batch, seq, channels, groups, per;  // per: channels of a group
@@ -200,55 +193,26 @@ __device__ __forceinline__ Place place_of(int64_t block, const Params &p, int wi
     return q;
 }
 
-// `rows` rows of CH channels (nch of them real) from src (row stride st) into dst [rows][CH], by NT threads; rows from
-// `live` on and missing channels are zeros.  The copies are asynchronous where vec says 16-byte copies are possible.
-template <int NT, int CH, typename TI>
-__device__ __forceinline__ void stage_x(TI *dst, const TI *src, int64_t st, int rows, int live, int nch, bool vec,
-                                        int tid = threadIdx.x) {
-    constexpr int kEl = 16 / sizeof(TI), kPer = CH / kEl;
-    if (vec && nch == CH && aligned16(src)) {
+// `rows` rows of W values (`width` of them real) from src (row stride st) into dst [rows][W], by NT threads of which this is
+// the tid-th; rows from `live` on and missing values are zeros.  Where vec says that rows start on 16-byte boundaries the
+// copies are asynchronous, and what a row lacks of its last copies is filled with zeros.
+template <int NT, int W, typename TI>
+__device__ __forceinline__ void stage(TI *dst, const TI *src, int64_t st, int rows, int live, int width, bool vec, int tid) {
+    constexpr int kEl = 16 / sizeof(TI), kPer = W >= kEl ? W / kEl : 1;
+    if (W % kEl == 0 && vec && aligned16(src)) {
 #pragma unroll 1
         for (int i = tid; i < rows * kPer; i += NT) {
-            const int r = i / kPer, q = i % kPer;
-            ptx::cp_async16(ptx::smem_u32(dst + i * kEl), src + (r < live ? r * st : 0) + q * kEl, r < live ? 16u : 0u);
+            const int r = i / kPer, q = i % kPer, left = (width - q * kEl) * (int)sizeof(TI);
+            const bool on = r < live && left > 0;
+            ptx::cp_async16(ptx::smem_u32(dst + i * kEl), on ? src + r * st + q * kEl : src, !on ? 0u : left > 16 ? 16u : (uint32_t)left);
         }
     } else {
 #pragma unroll 1
-        for (int i = tid; i < rows * CH; i += NT) {
-            const int r = i / CH, q = i % CH;
+        for (int i = tid; i < rows * W; i += NT) {
+            const int r = i / W, q = i % W;
             TI v;
             dc::st(&v, 0.f);
-            if (r < live && q < nch) v = src[r * st + q];
-            dst[i] = v;
-        }
-    }
-}
-// the same for `rows` rows of N states into dst [rows][NP] (columns from N on were zeroed once)
-template <int NT, int NP, typename TI>
-__device__ __forceinline__ void stage_bc(TI *dst, const TI *src, int64_t st, int rows, int live, int N, bool vec,
-                                         int tid = threadIdx.x) {
-    constexpr int kEl = 16 / sizeof(TI);
-    if (vec && N == NP && NP % kEl == 0 && aligned16(src)) {
-        constexpr int kPer = NP >= kEl ? NP / kEl : 1;
-#pragma unroll 1
-        for (int i = tid; i < rows * kPer; i += NT) {
-            const int r = i / kPer, q = i % kPer;
-            ptx::cp_async16(ptx::smem_u32(dst + i * kEl), src + (r < live ? r * st : 0) + q * kEl, r < live ? 16u : 0u);
-        }
-    } else if (vec && N % kEl == 0 && aligned16(src)) {
-        const int per = N / kEl;
-#pragma unroll 1
-        for (int i = tid; i < rows * per; i += NT) {
-            const int r = i / per, q = i % per;
-            ptx::cp_async16(ptx::smem_u32(dst + r * NP + q * kEl), src + (r < live ? r * st : 0) + q * kEl, r < live ? 16u : 0u);
-        }
-    } else {
-#pragma unroll 1
-        for (int i = tid; i < rows * NP; i += NT) {
-            const int r = i / NP, q = i % NP;
-            TI v;
-            dc::st(&v, 0.f);
-            if (r < live && q < N) v = src[r * st + q];
+            if (r < live && q < width) v = src[r * st + q];
             dst[i] = v;
         }
     }
@@ -287,12 +251,12 @@ struct Work {
     template <int NT, int TOK, bool FULL, typename Raw>
     __device__ __forceinline__ void load(Raw &w, int64_t t0, int tid) const {
         const int live = len - t0 < TOK ? (int)(len - t0) : TOK;
-        stage_x<NT, CH>(w.dt, D + t0 * p.dt_t, p.dt_t, TOK, live, at.nch, p.vec_x, tid);
-        stage_x<NT, CH>(w.u, U + t0 * p.u_t, p.u_t, TOK, live, at.nch, p.vec_x, tid);
-        stage_bc<NT, N4>(w.b, B + t0 * p.b_t, p.b_t, TOK, live, p.N, p.vec_bc, tid);
+        stage<NT, CH>(w.dt, D + t0 * p.dt_t, p.dt_t, TOK, live, at.nch, p.vec_x, tid);
+        stage<NT, CH>(w.u, U + t0 * p.u_t, p.u_t, TOK, live, at.nch, p.vec_x, tid);
+        stage<NT, N4>(w.b, B + t0 * p.b_t, p.b_t, TOK, live, p.N, p.vec_bc, tid);
         if (FULL) {
-            stage_bc<NT, N4>(w.c, C + t0 * p.c_t, p.c_t, TOK, live, p.N, p.vec_bc, tid);
-            if (Z) stage_x<NT, CH>(w.z, Z + t0 * p.z_t, p.z_t, TOK, live, at.nch, p.vec_x, tid);
+            stage<NT, N4>(w.c, C + t0 * p.c_t, p.c_t, TOK, live, p.N, p.vec_bc, tid);
+            if (Z) stage<NT, CH>(w.z, Z + t0 * p.z_t, p.z_t, TOK, live, at.nch, p.vec_x, tid);
         }
     }
 };
@@ -378,18 +342,8 @@ struct RawTile {
     TI b[TOK * N4], c[TOK * N4];
 };
 
-// b's and c's padding columns of every stage, zeroed once
-template <int NT, int TOK, int N4, int STAGES, typename Raw>
-__device__ __forceinline__ void clear_padding(Raw *raw, int N, int tid) {
-    if (N < N4)
-        for (int i = tid; i < TOK * N4; i += NT)
-            if (i % N4 >= N)
-#pragma unroll
-                for (int s = 0; s < STAGES; ++s) st(&raw[s].b[i], 0.f), st(&raw[s].c[i], 0.f);
-}
-
-__device__ __forceinline__ void checkpoint(const Params &p, const Place &at, int64_t t, int tokens, int64_t d, int q, F4 h) {
-    store4(p.ckpt + ((at.b * p.tiles + t / tokens) * p.channels + d) * p.N, kS * q, p.N, h);
+__device__ __forceinline__ void checkpoint(const Params &p, const Place &at, int64_t t, int64_t d, int q, F4 h) {
+    store4(p.ckpt + ((at.b * p.tiles + t / kTile) * p.channels + d) * p.N, kS * q, p.N, h);
 }
 
 // A thread's share of the 16-byte copies of a tile, where the rows start on 16-byte boundaries: the sources move on by one
@@ -460,7 +414,7 @@ constexpr int walk_ctas(int lanes) { return lanes == 4 ? 7 : lanes == 2 || lanes
 template <int P>
 struct WalkShape {
     static constexpr int kCh = walk_channels(P), kMain = kCh * P / 2, kHelp = 4 * kCh, kNT = kMain + kHelp;
-    static constexpr int kTok = 16, kStages = 4, kN = kS * P;
+    static constexpr int kTok = kTile, kStages = 4, kN = kS * P;
 };
 template <typename TI, int P>
 struct WalkSmem {
@@ -487,7 +441,6 @@ __global__ void __launch_bounds__(WalkShape<P>::kNT, walk_ctas(P)) scan_walk_ker
         const int tid = threadIdx.x - S::kMain;
         const Quads<TI, P, CH, kTok, S::kHelp> quads(p, at, tid);
         Stager<TI, CH, S::kN, kTok, S::kHelp, FULL> stager(wk, tid);
-        if (!stager.on) clear_padding<S::kHelp, kTok, S::kN, S::kStages>(sm.raw, p.N, tid);
         auto live = [&](int i) { return len - first - (int64_t)i * kTok < kTok ? (int)(len - first - (int64_t)i * kTok) : kTok; };
         auto prepare = [&](int i) {  // tile i's steps, b and c, once every helper's copies of it have landed
             const auto &w = sm.raw[i % S::kStages];
@@ -552,15 +505,12 @@ __global__ void __launch_bounds__(WalkShape<P>::kNT, walk_ctas(P)) scan_walk_ker
         const float2 *step = sm.step[i & 1] + ch;
         const float4 *b = sm.b[i & 1] + q, *c = sm.c[i & 1] + q;
         float *y = sm.y[i & 1] + q * CH + ch;
+        if (FULL && p.ckpt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (real[j]) checkpoint(p, at, first + (int64_t)i * kTok, d + j, q, h[j]);
 #pragma unroll 1
         for (int k0 = 0; k0 < kTok; k0 += kK) {
-            if (FULL && p.ckpt) {
-                const int64_t t = first + (int64_t)i * kTok + k0;
-                if (t < len && t % Tile<P>::kTokens == 0)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        if (real[j]) checkpoint(p, at, t, Tile<P>::kTokens, d + j, q, h[j]);
-            }
 #pragma unroll
             for (int k1 = 0; k1 < kK; k1 += kBatch) {
                 F4 av[kBatch][2], bv[kBatch][2];
@@ -630,7 +580,6 @@ __global__ void __launch_bounds__(SegShape<P>::kNT, 512 / SegShape<P>::kNT) scan
     const Place &at = wk.at;
     const int64_t len = wk.len;
     const Quads<TI, P, CH, kTok, kNT> quads(p, at, tid);
-    clear_padding<kNT, kTok, S::kN, 2>(sm.raw, N, tid);
     auto prepare = [&](int64_t t0, int s) {
         const auto &w = sm.raw[s];
         quads.steps(sm.step, w.dt, w.u, len - t0 < kTok ? (int)(len - t0) : kTok);
@@ -676,7 +625,7 @@ __global__ void __launch_bounds__(SegShape<P>::kNT, 512 / SegShape<P>::kNT) scan
                 if (i == seg) h = carry;
                 carry = fma(f4(sm.decay[i * kLanes + r]), carry, f4(sm.end[i * kLanes + r]));
             }
-            if (p.ckpt && real && k0 < live && (t0 + k0) % Tile<P>::kTokens == 0) checkpoint(p, at, t0 + k0, Tile<P>::kTokens, d, q, h);
+            if (p.ckpt && real && k0 < live && (t0 + k0) % kTile == 0) checkpoint(p, at, t0 + k0, d, q, h);
             float *y = sm.y + k0 * kLanes + r;
 #pragma unroll
             for (int k = 0; k < kK; ++k) {

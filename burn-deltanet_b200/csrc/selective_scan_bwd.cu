@@ -7,16 +7,7 @@ namespace {
 using namespace dc::host;
 namespace sc = dc::scan;
 
-// Blocks of 16 channels per CTA: as many as leave a CTA for every SM.
-int sub_blocks(const dc_selective_scan_args *f) {
-    const int64_t per = f->channels / f->groups;
-    int n = sc::kMaxSub;
-    while (n > 1 && f->batch * f->groups * ceil_div(per, (int64_t)sc::kCh * n) < sm_count()) n /= 2;
-    return n;
-}
-
 struct Layout {
-    int nsub;
     int64_t blocks;  // CTAs of a group
     uint64_t bc, a, d, bytes;
 };
@@ -24,8 +15,7 @@ struct Layout {
 Layout layout_of(const dc_selective_scan_args *f) {
     Layout l;
     const uint64_t al = 255;
-    l.nsub = sub_blocks(f);
-    l.blocks = ceil_div(f->channels / f->groups, (int64_t)sc::kCh * l.nsub);
+    l.blocks = ceil_div(f->channels / f->groups, sc::bwd_channels(sc::lanes_of(f->state)));
     l.bc = 0;
     l.a = ((uint64_t)f->batch * f->groups * l.blocks * f->seq * 2 * f->state * 4 + al) & ~al;
     l.d = l.a + (((uint64_t)f->batch * f->channels * f->state * 4 + al) & ~al);
@@ -69,7 +59,7 @@ struct Launch {
         static_assert(smem <= 227 * 1024, "shared memory of a CTA");
         const int st = sc::allow_smem(&sc::scan_bwd_kernel<TI, P>, smem);
         if (st != DC_OK) return st;
-        sc::scan_bwd_kernel<TI, P><<<ctas, sc::kThreads, smem, s>>>(p);
+        sc::scan_bwd_kernel<TI, P><<<ctas, sc::BwdShape<P>::kNT, smem, s>>>(p);
         return launched();
     }
 };
@@ -120,7 +110,6 @@ int dc_selective_scan_bwd(const dc_selective_scan_bwd_args *a, dc_stream_t strea
     if (st != DC_OK) return st;
     sc::BwdParams p{};
     p.f = sc::params_of(&a->fwd);
-    p.nsub = l.nsub;
     p.dy_b = a->d_y_batch_stride, p.dy_t = a->d_y_token_stride;
     p.f.vec_x = p.f.vec_x && (p.dy_t * (int64_t)dtype_size(a->fwd.out_dtype)) % 16 == 0;
     p.dy = a->d_y, p.dstate_out = a->d_state_out;

@@ -6,14 +6,17 @@
 //   d_step = u sum_n b g + sum_n a w,  w = g decay h_{t-1};   d_u = step sum_n b g + r d;   d_z = dy (sum_n c h + d u) silu'(z)
 // summed over the channels of a group: d_b = step u g, d_c = r h;  over tokens: d_a = step w, d_d = r u, d_dt_bias.
 //
-// The same tiles, segments and registers as the forward (selective_scan.cuh), whose checkpoints hold h at each tile's
-// first token: a tile's decays are taken once and serve the states' walk forward and the gradients' walk back; both
-// walks run once from zero for the exchange between the segments and once for good.
+// A thread of the recurrence has four states of two neighbouring channels, as in the forward's walk.  For a tile of 16
+// tokens it first walks forward from the forward's checkpoint and leaves the states before tokens 4, 8 and 12 in shared
+// memory; then, from the last four tokens to the first, it takes their decays and states once more, into registers, and
+// walks the gradients back through them.  So 1.75 exponentials per token and state; but the other way, segments of threads
+// that run their tokens from zero and exchange, takes twice the shared memory traffic, which is the bound here (measured at
+// 4 x 2048 x 2048 x 16: 690 us, with that traffic at 67 % of its peak).  Further threads stage the tiles, take the steps of
+// the next tile and write the gradients of the last one.
 //
-// d_b and d_c sum over channels, which lie across lanes: a token's eight sums of a thread (four states of each) are
-// halved lane by lane into one register per token (LaneSum), and a CTA takes up to four blocks of 16 channels one after
-// the other through each tile, so that those registers gather 64 channels before they leave for memory: the partial
-// sums are then 1/4 of what one block at a time would write and a second kernel read again.
+// d_b and d_c sum over channels, which lie across lanes: a token's eight sums of a thread (four states of each; its two
+// channels add up on the way) are halved lane by lane until a lane has one (LaneSum), and meet the other warps' in shared
+// memory; each CTA writes one line per token and a second kernel adds the CTAs' lines in order.
 #pragma once
 
 #include "selective_scan.cuh"
@@ -21,11 +24,8 @@
 namespace dc {
 namespace scan {
 
-constexpr int kMaxSub = 4;  // blocks of 16 channels of a CTA
-
 struct BwdParams {
     Params f;
-    int32_t nsub;        // blocks of 16 channels per CTA
     int64_t dy_b, dy_t;  // d_y's strides (f.y_dt is its type)
     const void *dy;
     const float *dstate_out;
@@ -36,307 +36,305 @@ struct BwdParams {
     float *d_part;   // [batch, 2, channels]: d_d, d_dt_bias
 };
 
-template <typename TI, int P>
-struct BwdSmem {
-    using T = Tile<P>;
-    static constexpr int kL = P == 1 ? 16 : 32 / P < 16 ? 32 / P : 16;  // channels whose sums meet in a warp
-    static constexpr int kSets = kCh / kL;
-    struct RawX {
-        TI u[T::kTokens * kCh], dt[T::kTokens * kCh], z[T::kTokens * kCh];
-        float dy[T::kTokens * kCh];  // or as many bfloat16
-    };
-    struct RawBC {
-        TI b[T::kTokens * T::kN], c[T::kTokens * T::kN];
-    };
-    RawX x[2];
-    RawBC bc[2];
-    float4 step[T::kTokens * kCh];  // (step, step * u, r, -)
-    float4 b[T::kTokens * P], c[T::kTokens * P];
-    float4 decay[kThreads], end[kThreads], back[kThreads];
-    float y[T::kTokens * kCh], gb[T::kTokens * kCh], aw[T::kTokens * kCh];
-    float sums[kSets][T::kTokens][2][T::kN];
-    // per block of 16 channels, carried from tile to tile
-    float4 a2[kMaxSub][kCh * P], g[kMaxSub][kCh * P];
-    float4 da[kMaxSub][kThreads], dd[kMaxSub][kThreads];
+constexpr int bwd_channels(int lanes) { return lanes <= 2 ? 64 / lanes : lanes == 16 ? 16 : 32; }  // of a CTA
+
+template <int P>
+struct BwdShape {
+    static constexpr int kCh = bwd_channels(P), kBlk = walk_channels(P);  // channels of a CTA, and of the threads of one block
+    static constexpr int kPairs = kBlk / 2, kSegT = kPairs * P, kBlocks = kCh / kBlk, kMain = kSegT * kBlocks;
+    static constexpr int kHelp = kTile * kCh / 4, kNT = kMain + kHelp, kN = kS * P, kT = 4;
+    // a token's sums over the states: a share per state group, or per four of them (added up by shuffles) where there are
+    // so many that the shares would not fit
+    static constexpr int kShares = P >= 8 ? P / 4 : P;
+    static_assert(kSegT % 32 == 0, "whole warps in a block");
 };
 
 template <typename TI, int P>
-__global__ void __launch_bounds__(kThreads, 2) scan_bwd_kernel(const BwdParams bp) {
-    using T = Tile<P>;
-    using Smem = BwdSmem<TI, P>;
-    using ChSum = LaneSum<Smem::kL, P>;
-    constexpr int kTok = T::kTokens, kLanes = kCh * P;
+struct BwdSmem {
+    using S = BwdShape<P>;
+    struct RawX {
+        TI u[kTile * S::kCh], dt[kTile * S::kCh], z[kTile * S::kCh];
+        float dy[kTile * S::kCh];  // or as many bfloat16
+        float h[S::kCh * S::kN];   // the states before the tile, [channel][N]
+    };
+    struct RawBC {
+        TI b[kTile * S::kN], c[kTile * S::kN];
+    };
+    RawX x[4];  // a tile's states are read while the next tile is prepared and the two after it land
+    RawBC bc[4];
+    float2 step[2][kTile * S::kCh];  // (step, step * u)
+    float r[2][kTile * S::kCh];
+    float4 b[2][kTile * P], c[2][kTile * P];
+    float y[kTile * S::kCh * S::kShares], gb[kTile * S::kCh * S::kShares], aw[kTile * S::kCh * S::kShares];  // [token][share][channel]
+    float sums[S::kBlocks][kTile][2][S::kN];  // d_b and d_c of a tile, by block
+    float4 mid[kTile / S::kT - 1][2][S::kMain];
+    float bias[S::kCh], skip[S::kCh];
+};
+
+template <typename TI, int P>
+__global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_kernel(const BwdParams bp) {
+    using S = BwdShape<P>;
+    using ChSum = LaneSum<S::kPairs, 1>;
+    constexpr int CH = S::kCh, kT = S::kT;
+    static_assert(ChSum::kOut == 1, "one sum a lane");
     const Params &p = bp.f;
     extern __shared__ __align__(16) unsigned char smem_bytes[];
-    Smem &sm = *reinterpret_cast<Smem *>(smem_bytes);
-    const int tid = threadIdx.x, seg = tid / kLanes, r = tid % kLanes, ch = r / P, q = r % P;
-    const Place at = place_of(blockIdx.x, p, kCh * bp.nsub);
-    const int nsub = (at.nch + kCh - 1) / kCh;
-    const int64_t len = length_of(p.lengths, at.b, p.seq);
-    const int64_t ntiles = (len + kTok - 1) / kTok;
+    BwdSmem<TI, P> &sm = *reinterpret_cast<BwdSmem<TI, P> *>(smem_bytes);
+    const Place at = place_of(blockIdx.x, p, CH);
     const int N = p.N;
-    const int64_t dy_size = p.y_dt ? 2 : 4;
-    const TI *U = static_cast<const TI *>(p.u) + at.b * p.u_b + at.d0, *D = static_cast<const TI *>(p.dt) + at.b * p.dt_b + at.d0;
-    const TI *Z = p.z ? static_cast<const TI *>(p.z) + at.b * p.z_b + at.d0 : nullptr;
-    const TI *B = static_cast<const TI *>(p.b) + at.b * p.b_b + at.e * N, *C = static_cast<const TI *>(p.c) + at.b * p.c_b + at.e * N;
-    const char *DY = static_cast<const char *>(bp.dy) + (at.b * bp.dy_b + at.d0) * dy_size;
+    const int64_t len = length_of(p.lengths, at.b, p.seq);
+    const int n = (int)((len + kTile - 1) / kTile);  // tiles; number i from the back
 
-    auto load = [&](int64_t it) {
-        const int64_t back = it / nsub, t0 = (ntiles - 1 - back) * kTok;
-        const int sub = (int)(it - back * nsub), c0 = sub * kCh;
-        const int nch = at.nch - c0 < kCh ? at.nch - c0 : kCh;
-        const int live = len - t0 < kTok ? (int)(len - t0) : kTok;
-        typename Smem::RawX &w = sm.x[it & 1];
-        stage_x<kThreads, kCh>(w.u, U + t0 * p.u_t + c0, p.u_t, kTok, live, nch, p.vec_x);
-        stage_x<kThreads, kCh>(w.dt, D + t0 * p.dt_t + c0, p.dt_t, kTok, live, nch, p.vec_x);
-        if (Z) stage_x<kThreads, kCh>(w.z, Z + t0 * p.z_t + c0, p.z_t, kTok, live, nch, p.vec_x);
-        if (p.y_dt)
-            stage_x<kThreads, kCh>(reinterpret_cast<__nv_bfloat16 *>(w.dy), reinterpret_cast<const __nv_bfloat16 *>(DY) + t0 * bp.dy_t + c0, bp.dy_t, kTok,
-                    live, nch, p.vec_x);
-        else
-            stage_x<kThreads, kCh>(w.dy, reinterpret_cast<const float *>(DY) + t0 * bp.dy_t + c0, bp.dy_t, kTok, live, nch, p.vec_x);
-        if (sub == 0) {
-            typename Smem::RawBC &v = sm.bc[back & 1];
-            stage_bc<kThreads, T::kN>(v.b, B + t0 * p.b_t, p.b_t, kTok, live, N, p.vec_bc);
-            stage_bc<kThreads, T::kN>(v.c, C + t0 * p.c_t, p.c_t, kTok, live, N, p.vec_bc);
-        }
-        ptx::cp_async_commit();
-    };
-    auto ld_dy = [&](const typename Smem::RawX &w, int i) {
-        return p.y_dt ? ld(reinterpret_cast<const __nv_bfloat16 *>(w.dy) + i) : w.dy[i];
-    };
-
-    for (int i = tid; i < kTok * T::kN; i += kThreads)
-        if (i % T::kN >= N)
+    if (threadIdx.x >= S::kMain) {
+        // ---------------------------------------------------------------- staging, steps, outputs
+        const int tid = threadIdx.x - S::kMain, oc = 4 * (tid % (CH / 4)), t = tid / (CH / 4);  // one quad of one token
+        const TI *U = static_cast<const TI *>(p.u) + at.b * p.u_b + at.d0, *D = static_cast<const TI *>(p.dt) + at.b * p.dt_b + at.d0;
+        const TI *Z = p.z ? static_cast<const TI *>(p.z) + at.b * p.z_b + at.d0 : nullptr;
+        const TI *B = static_cast<const TI *>(p.b) + at.b * p.b_b + at.e * N, *C = static_cast<const TI *>(p.c) + at.b * p.c_b + at.e * N;
+        const int64_t dy0 = at.b * bp.dy_b + at.d0;
+        const int64_t blocks = (p.per + CH - 1) / CH, blk = (at.d0 - at.e * p.per) / CH;
+        float *part = bp.bc_part + ((at.b * p.groups + at.e) * blocks + blk) * p.seq * 2 * N;
+        auto load = [&](int i) {
+            if (i < n) {
+                const int64_t tile = n - 1 - i, t0 = tile * kTile;
+                const int live = len - t0 < kTile ? (int)(len - t0) : kTile;
+                auto &w = sm.x[i & 3];
+                stage<S::kHelp, CH>(w.dt, D + t0 * p.dt_t, p.dt_t, kTile, live, at.nch, p.vec_x, tid);
+                stage<S::kHelp, CH>(w.u, U + t0 * p.u_t, p.u_t, kTile, live, at.nch, p.vec_x, tid);
+                if (Z) stage<S::kHelp, CH>(w.z, Z + t0 * p.z_t, p.z_t, kTile, live, at.nch, p.vec_x, tid);
+                if (p.y_dt)
+                    stage<S::kHelp, CH>(reinterpret_cast<__nv_bfloat16 *>(w.dy), static_cast<const __nv_bfloat16 *>(bp.dy) + dy0 + t0 * bp.dy_t,
+                                        bp.dy_t, kTile, live, at.nch, p.vec_x, tid);
+                else
+                    stage<S::kHelp, CH>(w.dy, static_cast<const float *>(bp.dy) + dy0 + t0 * bp.dy_t, bp.dy_t, kTile, live, at.nch, p.vec_x, tid);
+                stage<S::kHelp, CH * S::kN>(w.h, p.ckpt + ((at.b * p.tiles + tile) * p.channels + at.d0) * N, 0, 1, 1, at.nch * N, true, tid);
+                stage<S::kHelp, S::kN>(sm.bc[i & 3].b, B + t0 * p.b_t, p.b_t, kTile, live, N, p.vec_bc, tid);
+                stage<S::kHelp, S::kN>(sm.bc[i & 3].c, C + t0 * p.c_t, p.c_t, kTile, live, N, p.vec_bc, tid);
+            }
+            ptx::cp_async_commit();
+        };
+        // what this thread's four (token, channel) pairs of a tile need again when its sums come back
+        struct Kept {
+            float u[4], step[4], r[4], dz[4], slope[4];  // dz: d_z per read-out; slope: of softplus
+        };
+        Kept cur{}, nxt{};
+        auto prepare = [&](int i, Kept &k) {
+            const bool on = (int64_t)(n - 1 - i) * kTile + t < len;
+            const auto &w = sm.x[i & 3];
+            ptx::named_sync(1, S::kHelp);  // every helper's copies have landed
+            float v[4], z[4], gy[4];
+            vec::load<true>(w.u + t * CH + oc, k.u);
+            vec::load<true>(w.dt + t * CH + oc, v);
+            vec::load_as<true>(p.y_dt, w.dy, t * CH + oc, gy);
+            if (Z) vec::load<true>(w.z + t * CH + oc, z);
+            float bias[4];
+            vec::load<true>(sm.bias + oc, bias);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) st(&sm.bc[s].b[i], 0.f), st(&sm.bc[s].c[i], 0.f);
-    for (int sub = 0; sub < nsub; ++sub) {
-        sm.da[sub][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
-        sm.dd[sub][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (seg == 0) {
-            const bool real = sub * kCh + ch < at.nch;
-            const int64_t d = at.d0 + (real ? sub * kCh + ch : 0);
-            sm.a2[sub][r] = f4(real ? mul(kLog2e, load4(p.a + d * N, kS * q, N)) : zero4());
-            sm.g[sub][r] = f4(real && bp.dstate_out ? load4(bp.dstate_out + (at.b * p.channels + d) * N, kS * q, N) : zero4());
-        }
-    }
-    const int oc = 2 * (tid % (kCh / 2));  // the output phase's pair of channels within a block
-    float acc[kK][ChSum::kOut];
-#pragma unroll
-    for (int k = 0; k < kK; ++k)
-#pragma unroll
-        for (int j = 0; j < ChSum::kOut; ++j) acc[k][j] = 0.f;
-    const int64_t out0 = at.b * p.seq * p.channels + at.d0;
-    auto put = [&](void *o, int64_t t, int c, float v0, float v1) {  // channels c, c + 1 of token t
-        TI *w = static_cast<TI *>(o) + out0 + t * p.channels + c;
-        if (c + 1 < at.nch && (reinterpret_cast<uintptr_t>(w) % (2 * sizeof(TI))) == 0) {
-            if constexpr (sizeof(TI) == 2) *reinterpret_cast<uint32_t *>(w) = vec::pack(v0, v1);
-            else *reinterpret_cast<float2 *>(w) = make_float2(v0, v1);
-        } else {
-            if (c < at.nch) st(w, v0);
-            if (c + 1 < at.nch) st(w + 1, v1);
-        }
-    };
-
-    const int64_t items = ntiles * nsub;
-    if (items > 0) load(0);
-    for (int64_t it = 0; it < items; ++it) {
-        const int64_t back = it / nsub, tile = ntiles - 1 - back, t0 = tile * kTok;
-        const int sub = (int)(it - back * nsub), c0 = sub * kCh;
-        const int live = len - t0 < kTok ? (int)(len - t0) : kTok;
-        const bool real = c0 + ch < at.nch;
-        const int64_t d = at.d0 + (real ? c0 + ch : 0);
-        ptx::cp_async_wait<0>();
-        __syncthreads();  // this item's values have landed, and the last item's shared values are done with
-        if (it + 1 < items) load(it + 1);
-        const F4 h0 = real ? load4(p.ckpt + ((at.b * p.tiles + tile) * p.channels + d) * N, kS * q, N) : zero4();
-        const typename Smem::RawX &w = sm.x[it & 1];
-        {
-            const int pc = c0 + tid % kCh;
-            const float bias = p.dt_bias && pc < at.nch ? p.dt_bias[at.d0 + pc] : 0.f;
-            for (int i = tid; i < kTok * kCh; i += kThreads) {
-                float v = ld(&w.dt[i]) + bias, g = ld_dy(w, i);
-                if (p.softplus) v = softplus(v);
+            for (int j = 0; j < 4; ++j) {
+                v[j] += bias[j];
+                k.slope[j] = p.softplus ? sigmoid(v[j]) : 1.f;
+                k.r[j] = gy[j], k.dz[j] = 0.f;
                 if (Z) {
-                    const float z = ld(&w.z[i]);
-                    g *= z * sigmoid(z);
-                }
-                if (i / kCh >= live) v = 0.f, g = 0.f;
-                sm.step[i] = make_float4(v, v * ld(&w.u[i]), g, 0.f);
-            }
-        }
-        if (sub == 0) {
-            float *fb = reinterpret_cast<float *>(sm.b), *fc = reinterpret_cast<float *>(sm.c);
-            const typename Smem::RawBC &v = sm.bc[back & 1];
-            for (int i = tid; i < kTok * T::kN; i += kThreads) fb[i] = ld(&v.b[i]), fc[i] = ld(&v.c[i]);
-        }
-        __syncthreads();
-
-        const F4 a2 = f4(sm.a2[sub][r]);
-        F4 av[kK], hv[kK];  // hv: what is added at each token, then the states
-        F4 g_in = f4(sm.g[sub][r]), h_in = h0;
-        {
-            F4 prod = one4(), h = zero4();
-#pragma unroll
-            for (int k = 0; k < kK; ++k) {
-                const int t = seg * kK + k;
-                const float4 sd = sm.step[t * kCh + ch];
-                av[k] = ex2(mul(sd.x, a2));
-                hv[k] = mul(sd.y, f4(sm.b[t * P + q]));
-                if constexpr (T::kSegs > 1) {
-                    prod = mul(prod, av[k]);
-                    h = fma(av[k], h, hv[k]);
+                    const float s = sigmoid(z[j]);
+                    k.r[j] = gy[j] * (z[j] * s);
+                    k.dz[j] = gy[j] * s * fmaf(z[j], 1.f - s, 1.f);
                 }
             }
-            if constexpr (T::kSegs > 1) {
-                F4 g = zero4();
 #pragma unroll
-                for (int k = kK - 1; k >= 0; --k) {
-                    const int t = seg * kK + k;
-                    g = mul(av[k], fma(sm.step[t * kCh + ch].z, f4(sm.c[t * P + q]), g));
+            for (int j = 0; j < 4; j += 2) {
+                float2 f = make_float2(v[j], v[j + 1]);
+                if (p.softplus) f = softplus2(f);
+                k.step[j] = on ? f.x : 0.f, k.step[j + 1] = on ? f.y : 0.f;  // past the end: decay 1, nothing added
+            }
+            float4 *o = reinterpret_cast<float4 *>(sm.step[i & 1] + t * CH + oc);
+            o[0] = make_float4(k.step[0], k.step[0] * k.u[0], k.step[1], k.step[1] * k.u[1]);
+            o[1] = make_float4(k.step[2], k.step[2] * k.u[2], k.step[3], k.step[3] * k.u[3]);
+            vec::store<true>(sm.r[i & 1] + t * CH + oc, k.r);
+            widen<S::kHelp>(sm.b[i & 1], sm.bc[i & 3].b, kTile * S::kN, tid);
+            widen<S::kHelp>(sm.c[i & 1], sm.bc[i & 3].c, kTile * S::kN, tid);
+        };
+        const int64_t out0 = at.b * p.seq * p.channels + at.d0 + oc;
+        const int nput = at.nch - oc;  // channels of the quad that exist (<= 0: none)
+        const bool quad = nput >= 4 && out0 % 4 == 0 && p.channels % 4 == 0 && aligned16(bp.du) && aligned16(bp.ddt) && aligned16(bp.dz);
+        auto put = [&](void *o, int64_t token, const float (&v)[4]) {
+            TI *w = static_cast<TI *>(o) + out0 + token * p.channels;
+            if (quad) vec::store<true>(w, v);
+            else vec::store<false>(w, v, nput);
+        };
+        float sd[4] = {}, sb[4] = {};  // sums over this thread's tokens: d_d, d_dt_bias
+        auto finish = [&](int i, const Kept &k) {  // the gradients of tile i, from the recurrence's shares
+            const int64_t t0 = (int64_t)(n - 1 - i) * kTile, token = t0 + t;
+            float y[4] = {}, gb[4] = {}, aw[4] = {};
+#pragma unroll
+            for (int j = 0; j < S::kShares; ++j) {  // from another share on in each token, as in the forward
+                const int o = (t * S::kShares + ((j + t) & (S::kShares - 1))) * CH + oc;
+                const float4 f = *reinterpret_cast<const float4 *>(sm.gb + o), g = *reinterpret_cast<const float4 *>(sm.aw + o);
+                gb[0] += f.x, gb[1] += f.y, gb[2] += f.z, gb[3] += f.w;
+                aw[0] += g.x, aw[1] += g.y, aw[2] += g.z, aw[3] += g.w;
+                if (Z) {
+                    const float4 h = *reinterpret_cast<const float4 *>(sm.y + o);
+                    y[0] += h.x, y[1] += h.y, y[2] += h.z, y[3] += h.w;
                 }
-                sm.decay[tid] = f4(prod);
-                sm.end[tid] = f4(h);
-                sm.back[tid] = f4(g);
             }
-        }
-        __syncthreads();
-        if constexpr (T::kSegs > 1) {
+            if (token < len) {
+                float skip[4], du[4], ds[4], dz[4];
+                vec::load<true>(sm.skip + oc, skip);
 #pragma unroll
-            for (int i = 0; i < T::kSegs - 1; ++i) {
-                if (i < seg) h_in = fma(f4(sm.decay[i * kLanes + r]), h_in, f4(sm.end[i * kLanes + r]));
-                const int o = T::kSegs - 1 - i;
-                if (o > seg) g_in = fma(f4(sm.decay[o * kLanes + r]), g_in, f4(sm.back[o * kLanes + r]));
-            }
-        }
-        float y[kK], gb[kK], aw[kK];
-        {
-            F4 h = h_in;
-#pragma unroll
-            for (int k = 0; k < kK; ++k) {
-                h = fma(av[k], h, hv[k]);
-                hv[k] = h;
-                y[k] = dot(h, f4(sm.c[(seg * kK + k) * P + q]));
-            }
-        }
-        F4 da = f4(sm.da[sub][tid]);
-        F4 g = g_in;  // decay_{t+1} g_{t+1}
-#pragma unroll
-        for (int k = kK - 1; k >= 0; --k) {
-            const int t = seg * kK + k;
-            const float4 sd = sm.step[t * kCh + ch];
-            const F4 b = f4(sm.b[t * P + q]), c = f4(sm.c[t * P + q]);
-            const F4 dc = mul(sd.z, hv[k]);
-            g = fma(sd.z, c, g);
-            gb[k] = dot(g, b);
-            const F4 db = mul(sd.y, g);
-            g = mul(av[k], g);
-            const F4 wv = mul(g, k > 0 ? hv[k > 0 ? k - 1 : 0] : h_in);
-            aw[k] = dot(wv, a2);
-            da = fma(sd.x, wv, da);
-            float v[8] = {db.lo.x, db.lo.y, db.hi.x, db.hi.y, dc.lo.x, dc.lo.y, dc.hi.x, dc.hi.y};
-            ChSum::run(v, ch % Smem::kL);
-#pragma unroll
-            for (int j = 0; j < ChSum::kOut; ++j) acc[k][j] += v[j];
-        }
-        sm.da[sub][tid] = f4(da);
-        if (seg == 0) sm.g[sub][r] = f4(g);
-        LaneSum<P, 1>::run(gb, q);
-        LaneSum<P, 1>::run(aw, q);
-        LaneSum<P, 1>::run(y, q);
-        const int first = seg * kK + LaneSum<P, 1>::first(q);
-#pragma unroll
-        for (int k = 0; k < LaneSum<P, 1>::kOut; ++k) {
-            const int o = (first + k) * kCh + ch;
-            sm.gb[o] = gb[k], sm.aw[o] = aw[k], sm.y[o] = y[k];
-        }
-        if (sub == nsub - 1) {  // the tile's sums over this CTA's channels
-            const int j0 = ChSum::first(ch % Smem::kL), set = ch / Smem::kL;
-#pragma unroll
-            for (int k = 0; k < kK; ++k)
-#pragma unroll
-                for (int j = 0; j < ChSum::kOut; ++j) {
-                    sm.sums[set][seg * kK + k][(j0 + j) / kS][kS * q + (j0 + j) % kS] = acc[k][j];
-                    acc[k][j] = 0.f;
+                for (int j = 0; j < 4; ++j) {
+                    du[j] = fmaf(gb[j], k.step[j], k.r[j] * skip[j]);
+                    ds[j] = fmaf(gb[j], k.u[j], kLn2 * aw[j]) * k.slope[j];
+                    dz[j] = fmaf(skip[j], k.u[j], y[j]) * k.dz[j];
+                    sd[j] = fmaf(k.r[j], k.u[j], sd[j]);
+                    sb[j] += ds[j];
                 }
-        }
-        __syncthreads();
-        {
-            const int oa = c0 + oc;
-            const bool in0 = oa < at.nch, in1 = oa + 1 < at.nch;
-            const float dv0 = p.d && in0 ? p.d[at.d0 + oa] : 0.f, dv1 = p.d && in1 ? p.d[at.d0 + oa + 1] : 0.f;
-            const float bi0 = p.dt_bias && in0 ? p.dt_bias[at.d0 + oa] : 0.f, bi1 = p.dt_bias && in1 ? p.dt_bias[at.d0 + oa + 1] : 0.f;
-            float4 dd = sm.dd[sub][tid];
-            for (int i = tid; i < kTok * kCh / 2; i += kThreads) {
-                const int t = i / (kCh / 2);
-                if (t >= live) continue;
-                const int o = t * kCh + oc;
-                float du[2], ds[2], dz[2], sum_d[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float4 sd = sm.step[o + j];
-                    const float u = ld(&w.u[o + j]), dv = j ? dv1 : dv0;
-                    const float gbv = sm.gb[o + j];
-                    du[j] = fmaf(gbv, sd.x, sd.z * dv);
-                    ds[j] = fmaf(gbv, u, kLn2 * sm.aw[o + j]);
-                    if (p.softplus) ds[j] *= sigmoid(ld(&w.dt[o + j]) + (j ? bi1 : bi0));
-                    sum_d[j] = sd.z * u;
-                    if (Z) {
-                        const float z = ld(&w.z[o + j]), sg = sigmoid(z);
-                        dz[j] = ld_dy(w, o + j) * fmaf(dv, u, sm.y[o + j]) * sg * fmaf(z, 1.f - sg, 1.f);
-                    }
-                }
-                put(bp.du, t0 + t, oa, du[0], du[1]);
-                put(bp.ddt, t0 + t, oa, ds[0], ds[1]);
-                if (Z) put(bp.dz, t0 + t, oa, dz[0], dz[1]);
-                dd.x += sum_d[0], dd.y += sum_d[1], dd.z += ds[0], dd.w += ds[1];
+                put(bp.du, token, du);
+                put(bp.ddt, token, ds);
+                if (Z) put(bp.dz, token, dz);
             }
-            sm.dd[sub][tid] = dd;
-        }
-        if (sub == nsub - 1) {
-            const int64_t blocks = (p.per + kCh * bp.nsub - 1) / (kCh * bp.nsub);
-            const int64_t blk = (at.d0 - at.e * p.per) / (kCh * bp.nsub);
-            float *part = bp.bc_part + (((at.b * p.groups + at.e) * blocks + blk) * p.seq + t0) * 2 * N;
-            for (int i = tid; i < live * 2 * T::kN; i += kThreads) {
-                const int n = i % T::kN, j = i / T::kN;  // j: (token, which)
-                if (n < N) {
+            // the tile's lines of d_b and d_c: the blocks' sums in order
+            const int live = len - t0 < kTile ? (int)(len - t0) : kTile;
+            for (int j = tid; j < live * 2 * S::kN; j += S::kHelp) {
+                const int state = j % S::kN, row = j / S::kN;  // row: (token, which)
+                if (state < N) {
                     float v = 0.f;
 #pragma unroll
-                    for (int q2 = 0; q2 < Smem::kSets; ++q2) v += sm.sums[q2][j >> 1][j & 1][n];
-                    part[(int64_t)j * N + n] = v;
+                    for (int q = 0; q < S::kBlocks; ++q) v += (&sm.sums[q][0][0][0])[j];
+                    part[(t0 * 2 + row) * N + state] = v;
                 }
             }
+        };
+        for (int i = tid; i < CH; i += S::kHelp) {
+            sm.bias[i] = p.dt_bias && i < at.nch ? p.dt_bias[at.d0 + i] : 0.f;
+            sm.skip[i] = p.d && i < at.nch ? p.d[at.d0 + i] : 0.f;
         }
+        load(0);
+        load(1);
+        load(2);
+        ptx::cp_async_wait<2>();
+        if (n > 0) prepare(0, nxt);
+        __syncthreads();  // (1) the first tile is ready
+        Kept old{};
+        for (int i = 0; i < n; ++i) {
+            old = cur, cur = nxt;
+            if (i > 0) finish(i - 1, old);
+            __syncthreads();  // (2) the last tile's shares and sums are done with
+            ptx::cp_async_wait<1>();
+            if (i + 1 < n) prepare(i + 1, nxt);
+            load(i + 3);
+            __syncthreads();  // (3) this tile's shares and sums are complete, the next tile is ready
+        }
+        if (n > 0) finish(n - 1, cur);
+        // the sums over tokens: sixteen threads' in order, through the shares' memory
+        ptx::named_sync(1, S::kHelp);
+        vec::store<true>(sm.y + t * CH + oc, sd);
+        vec::store<true>(sm.gb + t * CH + oc, sb);
+        ptx::named_sync(1, S::kHelp);
+        if (tid < at.nch) {
+            float d = 0.f, b = 0.f;
+            for (int k = 0; k < kTile; ++k) d += sm.y[k * CH + tid], b += sm.gb[k * CH + tid];
+            float *o = bp.d_part + at.b * 2 * p.channels + at.d0 + tid;
+            o[0] = d;
+            o[p.channels] = b;
+        }
+        const float none[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int64_t token = len + t; token < p.seq; token += kTile) {
+            put(bp.du, token, none);
+            put(bp.ddt, token, none);
+            if (bp.dz) put(bp.dz, token, none);
+        }
+        return;
     }
-    __syncthreads();
-    for (int sub = 0; sub < nsub; ++sub) {
-        const int c0 = sub * kCh;
-        if (seg == 0 && c0 + ch < at.nch) {
-            const int64_t row = (at.b * p.channels + at.d0 + c0 + ch) * N;
-            F4 v = f4(sm.da[sub][r]);
-            for (int i = 1; i < T::kSegs; ++i) {
-                const F4 o = f4(sm.da[sub][i * kLanes + r]);
-                v = fma(1.f, o, v);
+
+    // -------------------------------------------------------------------- the recurrences
+    const int tid = threadIdx.x, block = tid / S::kSegT, r = tid % S::kSegT, pair = r % S::kPairs, q = r / S::kPairs;
+    const int ch = block * S::kBlk + 2 * pair;
+    bool real[2];
+    F4 a2[2], g[2], da[2];  // g: decay_{t+1} g_{t+1}
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        real[j] = ch + j < at.nch;
+        const int64_t d = at.d0 + ch + j;
+        a2[j] = real[j] ? mul(kLog2e, load4(p.a + d * N, kS * q, N)) : zero4();
+        g[j] = real[j] && bp.dstate_out ? load4(bp.dstate_out + (at.b * p.channels + d) * N, kS * q, N) : zero4();
+        da[j] = zero4();
+    }
+    // this lane's sum over channels: of d_b (0) or d_c (1), of which state; lanes that hold a copy leave nothing
+    const int value = ChSum::first(pair);
+    const bool leaves = pair % (S::kPairs / 8) == 0;
+    float *sums = &sm.sums[block][0][value / kS][kS * q + value % kS];
+    auto leave = [&](float *o, int t, float v0, float v1) {  // both channels' share of token t
+        if constexpr (S::kShares == P) {
+            *reinterpret_cast<float2 *>(o + (t * P + q) * CH + ch) = make_float2(v0, v1);
+        } else {  // the warp's four state groups, 8 lanes apart
+#pragma unroll
+            for (int x = 8; x <= 16; x *= 2) v0 += __shfl_xor_sync(0xffffffffu, v0, x), v1 += __shfl_xor_sync(0xffffffffu, v1, x);
+            if (q % 4 == 0) *reinterpret_cast<float2 *>(o + (t * S::kShares + q / 4) * CH + ch) = make_float2(v0, v1);
+        }
+    };
+    __syncthreads();  // (1)
+    for (int i = 0; i < n; ++i) {
+        const float2 *step = sm.step[i & 1] + ch;
+        const float *rr = sm.r[i & 1] + ch;
+        const float4 *bs = sm.b[i & 1] + q, *cs = sm.c[i & 1] + q;
+        const float *before = sm.x[i & 3].h;
+        auto first = [&](int j) { return real[j] ? load4(before + (ch + j) * N, kS * q, N) : zero4(); };
+        {
+            F4 h[2] = {first(0), first(1)};
+#pragma unroll 1
+            for (int m = 0; m < kTile / kT - 1; ++m) {
+#pragma unroll
+                for (int k = 0; k < kT; ++k) {
+                    const int t = m * kT + k;
+                    const float4 sd = *reinterpret_cast<const float4 *>(step + t * CH);
+                    const F4 b = f4(bs[t * P]);
+                    h[0] = fma(ex2(mul(sd.x, a2[0])), h[0], mul(sd.y, b));
+                    h[1] = fma(ex2(mul(sd.z, a2[1])), h[1], mul(sd.w, b));
+                }
+                sm.mid[m][0][tid] = f4(h[0]), sm.mid[m][1][tid] = f4(h[1]);
             }
-            store4(bp.a_part + row, kS * q, N, v);
-            if (bp.dstate_in) store4(bp.dstate_in + row, kS * q, N, f4(sm.g[sub][r]));
         }
-        if (tid < kCh && c0 + tid < at.nch) {
-            float sd = 0.f, sb = 0.f;
-            for (int i = tid / 2; i < kThreads; i += kCh / 2) {
-                const float4 v = sm.dd[sub][i];
-                sd += tid & 1 ? v.y : v.x;
-                sb += tid & 1 ? v.w : v.z;
+        __syncthreads();  // (2)
+#pragma unroll 1
+        for (int m = kTile / kT - 1; m >= 0; --m) {
+            F4 av[kT][2], hv[kT][2], h_in[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) h_in[j] = m ? f4(sm.mid[m ? m - 1 : 0][j][tid]) : first(j);
+#pragma unroll
+            for (int k = 0; k < kT; ++k) {
+                const int t = m * kT + k;
+                const float4 sd = *reinterpret_cast<const float4 *>(step + t * CH);
+                const F4 b = f4(bs[t * P]);
+                av[k][0] = ex2(mul(sd.x, a2[0])), av[k][1] = ex2(mul(sd.z, a2[1]));
+                hv[k][0] = fma(av[k][0], k ? hv[k ? k - 1 : 0][0] : h_in[0], mul(sd.y, b));
+                hv[k][1] = fma(av[k][1], k ? hv[k ? k - 1 : 0][1] : h_in[1], mul(sd.w, b));
             }
-            float *o = bp.d_part + at.b * 2 * p.channels + at.d0 + c0 + tid;
-            o[0] = sd;
-            o[p.channels] = sb;
+#pragma unroll
+            for (int k = kT - 1; k >= 0; --k) {
+                const int t = m * kT + k;
+                const float4 sd = *reinterpret_cast<const float4 *>(step + t * CH);
+                const float2 rv = *reinterpret_cast<const float2 *>(rr + t * CH);
+                const F4 b = f4(bs[t * P]), c = f4(cs[t * P]);
+                const F4 g0 = fma(rv.x, c, g[0]), g1 = fma(rv.y, c, g[1]);
+                const F4 dc = fma(rv.y, hv[k][1], mul(rv.x, hv[k][0])), db = fma(sd.w, g1, mul(sd.y, g0));
+                leave(sm.y, t, dot(hv[k][0], c), dot(hv[k][1], c));
+                leave(sm.gb, t, dot(g0, b), dot(g1, b));
+                g[0] = mul(av[k][0], g0), g[1] = mul(av[k][1], g1);
+                const F4 w0 = mul(g[0], k ? hv[k ? k - 1 : 0][0] : h_in[0]), w1 = mul(g[1], k ? hv[k ? k - 1 : 0][1] : h_in[1]);
+                leave(sm.aw, t, dot(w0, a2[0]), dot(w1, a2[1]));
+                da[0] = fma(sd.x, w0, da[0]), da[1] = fma(sd.z, w1, da[1]);
+                float v[8] = {db.lo.x, db.lo.y, db.hi.x, db.hi.y, dc.lo.x, dc.lo.y, dc.hi.x, dc.hi.y};
+                ChSum::run(v, pair);
+                if (leaves) sums[t * 2 * S::kN] = v[0];
+            }
         }
-        for (int64_t t = len + tid / (kCh / 2); t < p.seq; t += kThreads / (kCh / 2)) {
-            put(bp.du, t, c0 + oc, 0.f, 0.f);
-            put(bp.ddt, t, c0 + oc, 0.f, 0.f);
-            if (bp.dz) put(bp.dz, t, c0 + oc, 0.f, 0.f);
-        }
+        __syncthreads();  // (3)
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        if (!real[j]) continue;
+        const int64_t row = (at.b * p.channels + at.d0 + ch + j) * N;
+        store4(bp.a_part + row, kS * q, N, da[j]);
+        if (bp.dstate_in) store4(bp.dstate_in + row, kS * q, N, g[j]);
     }
 }
 

@@ -15,9 +15,6 @@ inline int lanes_of(int64_t state) {
     while (p * kS < state) p *= 2;
     return p;
 }
-// Tokens of a tile (Tile<P>::kTokens).
-inline int64_t tile_tokens(int64_t state) { return (int64_t)kK * (kThreads / (kCh * lanes_of(state))); }
-
 inline int validate_dims(const dc_selective_scan_args *a) {
     if (!a) return DC_EINVAL_ARG;
     if (a->batch < 0 || a->seq < 0 || a->channels < 0 || a->state < 1 || a->groups < 1) return DC_EINVAL_SHAPE;
@@ -60,7 +57,7 @@ inline Params params_of(const dc_selective_scan_args *a) {
     const int64_t is = host::dtype_size(a->in_dtype);
     p.vec_x = (p.u_t * is) % 16 == 0 && (p.dt_t * is) % 16 == 0 && (!a->z || (p.z_t * is) % 16 == 0);
     p.vec_bc = (p.b_t * is) % 16 == 0 && (p.c_t * is) % 16 == 0;
-    p.tiles = (int32_t)host::ceil_div(a->seq, tile_tokens(a->state));
+    p.tiles = (int32_t)host::ceil_div(a->seq, kTile);
     p.u = a->u, p.dt = a->dt, p.z = a->z, p.b = a->b, p.c = a->c;
     p.a = a->a, p.d = a->d, p.dt_bias = a->dt_bias, p.state_in = a->state_in, p.lengths = a->lengths;
     p.y = a->y, p.state_out = a->state_out, p.ckpt = a->checkpoints;

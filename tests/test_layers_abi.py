@@ -229,7 +229,7 @@ def test_scan_bwd_refusals(over, bwd, status):
 
 def test_sizes():
     L = abi.lib()
-    tile = {4: 128, 8: 64, 16: 32, 32: 16, 64: 8}  # tokens between checkpoints by state
+    tile = {4: 16, 8: 16, 16: 16, 32: 16, 64: 16}  # tokens between checkpoints by state
     for n, t in tile.items():
         for seq in (0, 1, t, t + 1, 1000):
             assert L.dc_selective_scan_checkpoint_size(scan(state=n, seq=seq)) == 2 * -(-seq // t) * 32 * n * 4
