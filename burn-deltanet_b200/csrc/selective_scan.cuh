@@ -133,42 +133,6 @@ __device__ __forceinline__ void store4(float *row, int n, int N, F4 v) {
     if (n + 3 < N) row[n + 3] = v.hi.y;
 }
 
-// Sums of eight values over L lanes that are STRIDE apart, all at once: at each step a lane hands half of the values it
-// holds to its partner and keeps the other half, while it holds more than one.  Lane q of the L (their order is q) is
-// left with values first(q) .. first(q) + kOut, at v[0 ..], each summed over the L lanes.
-template <int L, int STRIDE>
-struct LaneSum {
-    static constexpr int kOut = L >= 8 ? 1 : 8 / L;
-    __device__ static __forceinline__ int first(int q) {
-        int f = 0, w = 8;
-#pragma unroll
-        for (int o = L / 2; o >= 1; o >>= 1)
-            if (w > 1) {
-                w >>= 1;
-                if (q & o) f += w;
-            }
-        return f;
-    }
-    __device__ static __forceinline__ void run(float (&v)[8], int q) {
-        int w = 8;
-#pragma unroll
-        for (int o = L / 2; o >= 1; o >>= 1) {
-            if (w > 1) {
-                w >>= 1;
-                const bool upper = (q & o) != 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i < w) {
-                        const float send = upper ? v[i] : v[i + w], keep = upper ? v[i + w] : v[i];
-                        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o * STRIDE);
-                    }
-            } else {
-                v[0] += __shfl_xor_sync(0xffffffffu, v[0], o * STRIDE);
-            }
-        }
-    }
-};
-
 __device__ __forceinline__ int64_t length_of(const int32_t *lengths, int64_t b, int64_t seq) {
     if (!lengths) return seq;
     const int64_t n = lengths[b];

@@ -6,17 +6,17 @@
 //   d_step = u sum_n b g + sum_n a w,  w = g decay h_{t-1};   d_u = step sum_n b g + r d;   d_z = dy (sum_n c h + d u) silu'(z)
 // summed over the channels of a group: d_b = step u g, d_c = r h;  over tokens: d_a = step w, d_d = r u, d_dt_bias.
 //
-// A thread of the recurrence has four states of two neighbouring channels, as in the forward's walk.  For a tile of 16
-// tokens it first walks forward from the forward's checkpoint and leaves the states before tokens 4, 8 and 12 in shared
-// memory; then, from the last four tokens to the first, it takes their decays and states once more, into registers, and
-// walks the gradients back through them.  So 1.75 exponentials per token and state; but the other way, segments of threads
-// that run their tokens from zero and exchange, takes twice the shared memory traffic, which is the bound here (measured at
-// 4 x 2048 x 2048 x 16: 690 us, with that traffic at 67 % of its peak).  Further threads stage the tiles, take the steps of
-// the next tile and write the gradients of the last one.
+// A thread of the recurrence has four states of two neighbouring channels, as in the forward's walk.  From the last four
+// tokens of a tile of 16 to its first, it takes their decays and states once more, into registers, and walks the gradients
+// back through them.  The states before each four tokens come from a walk forward from the forward's checkpoint, which the
+// CTA's other threads make one tile ahead; these also stage the tiles, take the steps and write the gradients of the last
+// tile, so that the walk back, the longest chain, waits for nothing: one barrier per tile.  This takes 1.75 exponentials
+// per token and state; the other way, segments of threads that run their tokens from zero and exchange, takes one but twice
+// the shared memory traffic (measured at 4 x 2048 x 2048 x 16: 690 us, with that traffic at 67 % of its peak).
 //
-// d_b and d_c sum over channels, which lie across lanes: a token's eight sums of a thread (four states of each; its two
-// channels add up on the way) are halved lane by lane until a lane has one (LaneSum), and meet the other warps' in shared
-// memory; each CTA writes one line per token and a second kernel adds the CTAs' lines in order.
+// d_b and d_c sum over channels, which lie across lanes (a thread's two channels add up on the way): every four tokens a
+// warp turns its sums over in shared memory, so that each lane adds the eight pairs of channels of one token and four
+// states; the warps of a CTA meet in a line per token, and a second kernel adds the CTAs' lines in order.
 #pragma once
 
 #include "selective_scan.cuh"
@@ -52,31 +52,85 @@ struct BwdShape {
 template <typename TI, int P>
 struct BwdSmem {
     using S = BwdShape<P>;
-    struct RawX {
-        TI u[kTile * S::kCh], dt[kTile * S::kCh], z[kTile * S::kCh];
-        float dy[kTile * S::kCh];  // or as many bfloat16
-        float h[S::kCh * S::kN];   // the states before the tile, [channel][N]
+    struct Raw {  // d_y in the space of float32, whatever its type
+        TI u[kTile * S::kCh], dt[kTile * S::kCh], z[kTile * S::kCh], b[kTile * S::kN], c[kTile * S::kN];
+        float dy[kTile * S::kCh];
     };
-    struct RawBC {
-        TI b[kTile * S::kN], c[kTile * S::kN];
+    struct Shares {  // [token][share][channel]
+        float y[kTile * S::kCh * S::kShares], gb[kTile * S::kCh * S::kShares], aw[kTile * S::kCh * S::kShares];
+        float sums[S::kBlocks][kTile][2][S::kN];  // d_b and d_c of a tile, by block
     };
-    RawX x[4];  // a tile's states are read while the next tile is prepared and the two after it land
-    RawBC bc[4];
+    // all twofold: the walk back is at one tile while the next is prepared or the last is written
+    Raw raw[2];
     float2 step[2][kTile * S::kCh];  // (step, step * u)
     float r[2][kTile * S::kCh];
     float4 b[2][kTile * P], c[2][kTile * P];
-    float y[kTile * S::kCh * S::kShares], gb[kTile * S::kCh * S::kShares], aw[kTile * S::kCh * S::kShares];  // [token][share][channel]
-    float sums[S::kBlocks][kTile][2][S::kN];  // d_b and d_c of a tile, by block
-    float4 mid[kTile / S::kT - 1][2][S::kMain];
+    float4 mid[2][kTile / S::kT][2][S::kMain];  // the states before each four tokens
+    Shares share[2];
+    float4 turn[S::kMain / 32][S::kT * 2 * 32];  // a warp's sums of four tokens: [token][d_b, d_c][lane]
     float bias[S::kCh], skip[S::kCh];
+};
+
+// A helper's share of the 16-byte copies of a tile, where the rows start on 16-byte boundaries and d_y has the inputs' type:
+// the sources move back by one tile a call (the forward's Stager, the other way).
+template <typename TI, int P>
+struct BwdStager {
+    using S = BwdShape<P>;
+    using Raw = typename BwdSmem<TI, P>::Raw;
+    static constexpr int kEs = sizeof(TI), kEl = 16 / kEs, kXRow = S::kCh / kEl, kBRow = S::kN >= kEl ? S::kN / kEl : 1;
+    static constexpr int kX = kTile * kXRow, kB = kTile * kBRow, kAll = 4 * kX + 2 * kB, kEach = (kAll + S::kHelp - 1) / S::kHelp;
+    const char *src[kEach];
+    int64_t step[kEach];  // bytes a token
+    int dst[kEach], row[kEach], bytes[kEach];
+    bool on;
+
+    __device__ __forceinline__ BwdStager(const BwdParams &bp, const Place &at, int64_t t0, int tid) {
+        const Params &p = bp.f;
+        const struct {
+            const void *at;
+            int64_t batch, token, first;
+            int base;  // in copies
+        } in[6] = {{p.u, p.u_b, p.u_t, at.d0, 0},          {p.dt, p.dt_b, p.dt_t, at.d0, kX},        {p.z, p.z_b, p.z_t, at.d0, 2 * kX},
+                   {p.b, p.b_b, p.b_t, at.e * p.N, 3 * kX}, {p.c, p.c_b, p.c_t, at.e * p.N, 3 * kX + kB}, {bp.dy, bp.dy_b, bp.dy_t, at.d0, 3 * kX + 2 * kB}};
+        on = p.vec_x && p.vec_bc && S::kN % kEl == 0 && p.z && (p.y_dt ? 2 : 4) == kEs;
+#pragma unroll
+        for (int k = 0; k < 6; ++k) on = on && aligned16(static_cast<const TI *>(in[k].at) + at.b * in[k].batch + in[k].first);
+        if (!on) return;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const int c = tid + j * S::kHelp;
+            row[j] = kTile;  // a row that no tile has
+            bytes[j] = dst[j] = 0, step[j] = 0, src[j] = nullptr;
+#pragma unroll
+            for (int k = 0; k < 6; ++k) {
+                const int per = k == 3 || k == 4 ? kBRow : kXRow, width = k == 3 || k == 4 ? p.N : at.nch, q = (c - in[k].base) % per;
+                if (c >= in[k].base && c < in[k].base + kTile * per) {
+                    const int left = (width - q * kEl) * kEs;
+                    row[j] = (c - in[k].base) / per;
+                    bytes[j] = left < 0 ? 0 : left > 16 ? 16 : left;
+                    dst[j] = c * 16;
+                    step[j] = in[k].token * kEs;
+                    src[j] = reinterpret_cast<const char *>(static_cast<const TI *>(in[k].at) + at.b * in[k].batch + in[k].first + t0 * in[k].token +
+                                                            (bytes[j] ? q * kEl : 0));
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void copy(Raw &raw, int live) {  // src: the tile's first token
+        const uint32_t to = ptx::smem_u32(&raw);
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const bool in = row[j] < live;
+            if (row[j] < kTile) ptx::cp_async16(to + dst[j], src[j] + (in ? step[j] * row[j] : 0), in ? bytes[j] : 0);
+            src[j] -= step[j] * kTile;
+        }
+    }
 };
 
 template <typename TI, int P>
 __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_kernel(const BwdParams bp) {
     using S = BwdShape<P>;
-    using ChSum = LaneSum<S::kPairs, 1>;
     constexpr int CH = S::kCh, kT = S::kT;
-    static_assert(ChSum::kOut == 1, "one sum a lane");
     const Params &p = bp.f;
     extern __shared__ __align__(16) unsigned char smem_bytes[];
     BwdSmem<TI, P> &sm = *reinterpret_cast<BwdSmem<TI, P> *>(smem_bytes);
@@ -94,22 +148,26 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
         const int64_t dy0 = at.b * bp.dy_b + at.d0;
         const int64_t blocks = (p.per + CH - 1) / CH, blk = (at.d0 - at.e * p.per) / CH;
         float *part = bp.bc_part + ((at.b * p.groups + at.e) * blocks + blk) * p.seq * 2 * N;
+        BwdStager<TI, P> stager(bp, at, (int64_t)(n > 0 ? n - 1 : 0) * kTile, tid);
         auto load = [&](int i) {
             if (i < n) {
-                const int64_t tile = n - 1 - i, t0 = tile * kTile;
+                const int64_t t0 = (int64_t)(n - 1 - i) * kTile;
                 const int live = len - t0 < kTile ? (int)(len - t0) : kTile;
-                auto &w = sm.x[i & 3];
-                stage<S::kHelp, CH>(w.dt, D + t0 * p.dt_t, p.dt_t, kTile, live, at.nch, p.vec_x, tid);
-                stage<S::kHelp, CH>(w.u, U + t0 * p.u_t, p.u_t, kTile, live, at.nch, p.vec_x, tid);
-                if (Z) stage<S::kHelp, CH>(w.z, Z + t0 * p.z_t, p.z_t, kTile, live, at.nch, p.vec_x, tid);
-                if (p.y_dt)
-                    stage<S::kHelp, CH>(reinterpret_cast<__nv_bfloat16 *>(w.dy), static_cast<const __nv_bfloat16 *>(bp.dy) + dy0 + t0 * bp.dy_t,
-                                        bp.dy_t, kTile, live, at.nch, p.vec_x, tid);
-                else
-                    stage<S::kHelp, CH>(w.dy, static_cast<const float *>(bp.dy) + dy0 + t0 * bp.dy_t, bp.dy_t, kTile, live, at.nch, p.vec_x, tid);
-                stage<S::kHelp, CH * S::kN>(w.h, p.ckpt + ((at.b * p.tiles + tile) * p.channels + at.d0) * N, 0, 1, 1, at.nch * N, true, tid);
-                stage<S::kHelp, S::kN>(sm.bc[i & 3].b, B + t0 * p.b_t, p.b_t, kTile, live, N, p.vec_bc, tid);
-                stage<S::kHelp, S::kN>(sm.bc[i & 3].c, C + t0 * p.c_t, p.c_t, kTile, live, N, p.vec_bc, tid);
+                auto &w = sm.raw[i & 1];
+                if (stager.on) {
+                    stager.copy(w, live);
+                } else {
+                    stage<S::kHelp, CH>(w.dt, D + t0 * p.dt_t, p.dt_t, kTile, live, at.nch, p.vec_x, tid);
+                    stage<S::kHelp, CH>(w.u, U + t0 * p.u_t, p.u_t, kTile, live, at.nch, p.vec_x, tid);
+                    if (Z) stage<S::kHelp, CH>(w.z, Z + t0 * p.z_t, p.z_t, kTile, live, at.nch, p.vec_x, tid);
+                    if (p.y_dt)
+                        stage<S::kHelp, CH>(reinterpret_cast<__nv_bfloat16 *>(w.dy), static_cast<const __nv_bfloat16 *>(bp.dy) + dy0 + t0 * bp.dy_t,
+                                            bp.dy_t, kTile, live, at.nch, p.vec_x, tid);
+                    else
+                        stage<S::kHelp, CH>(w.dy, static_cast<const float *>(bp.dy) + dy0 + t0 * bp.dy_t, bp.dy_t, kTile, live, at.nch, p.vec_x, tid);
+                    stage<S::kHelp, S::kN>(w.b, B + t0 * p.b_t, p.b_t, kTile, live, N, p.vec_bc, tid);
+                    stage<S::kHelp, S::kN>(w.c, C + t0 * p.c_t, p.c_t, kTile, live, N, p.vec_bc, tid);
+                }
             }
             ptx::cp_async_commit();
         };
@@ -120,8 +178,7 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
         Kept cur{}, nxt{};
         auto prepare = [&](int i, Kept &k) {
             const bool on = (int64_t)(n - 1 - i) * kTile + t < len;
-            const auto &w = sm.x[i & 3];
-            ptx::named_sync(1, S::kHelp);  // every helper's copies have landed
+            const auto &w = sm.raw[i & 1];
             float v[4], z[4], gy[4];
             vec::load<true>(w.u + t * CH + oc, k.u);
             vec::load<true>(w.dt + t * CH + oc, v);
@@ -150,8 +207,8 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
             o[0] = make_float4(k.step[0], k.step[0] * k.u[0], k.step[1], k.step[1] * k.u[1]);
             o[1] = make_float4(k.step[2], k.step[2] * k.u[2], k.step[3], k.step[3] * k.u[3]);
             vec::store<true>(sm.r[i & 1] + t * CH + oc, k.r);
-            widen<S::kHelp>(sm.b[i & 1], sm.bc[i & 3].b, kTile * S::kN, tid);
-            widen<S::kHelp>(sm.c[i & 1], sm.bc[i & 3].c, kTile * S::kN, tid);
+            widen<S::kHelp>(sm.b[i & 1], w.b, kTile * S::kN, tid);
+            widen<S::kHelp>(sm.c[i & 1], w.c, kTile * S::kN, tid);
         };
         const int64_t out0 = at.b * p.seq * p.channels + at.d0 + oc;
         const int nput = at.nch - oc;  // channels of the quad that exist (<= 0: none)
@@ -163,16 +220,17 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
         };
         float sd[4] = {}, sb[4] = {};  // sums over this thread's tokens: d_d, d_dt_bias
         auto finish = [&](int i, const Kept &k) {  // the gradients of tile i, from the recurrence's shares
+            const auto &sh = sm.share[i & 1];
             const int64_t t0 = (int64_t)(n - 1 - i) * kTile, token = t0 + t;
             float y[4] = {}, gb[4] = {}, aw[4] = {};
 #pragma unroll
             for (int j = 0; j < S::kShares; ++j) {  // from another share on in each token, as in the forward
                 const int o = (t * S::kShares + ((j + t) & (S::kShares - 1))) * CH + oc;
-                const float4 f = *reinterpret_cast<const float4 *>(sm.gb + o), g = *reinterpret_cast<const float4 *>(sm.aw + o);
+                const float4 f = *reinterpret_cast<const float4 *>(sh.gb + o), g = *reinterpret_cast<const float4 *>(sh.aw + o);
                 gb[0] += f.x, gb[1] += f.y, gb[2] += f.z, gb[3] += f.w;
                 aw[0] += g.x, aw[1] += g.y, aw[2] += g.z, aw[3] += g.w;
                 if (Z) {
-                    const float4 h = *reinterpret_cast<const float4 *>(sm.y + o);
+                    const float4 h = *reinterpret_cast<const float4 *>(sh.y + o);
                     y[0] += h.x, y[1] += h.y, y[2] += h.z, y[3] += h.w;
                 }
             }
@@ -198,8 +256,49 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
                 if (state < N) {
                     float v = 0.f;
 #pragma unroll
-                    for (int q = 0; q < S::kBlocks; ++q) v += (&sm.sums[q][0][0][0])[j];
+                    for (int q = 0; q < S::kBlocks; ++q) v += (&sh.sums[q][0][0][0])[j];
                     part[(t0 * 2 + row) * N + state] = v;
+                }
+            }
+        };
+        // the states before each four tokens of a tile: thread v walks one channel (the j-th of a pair) of a thread of the
+        // recurrence; this thread is v = tid, tid + kHelp, ..
+        constexpr int kWalks = (2 * S::kMain + S::kHelp - 1) / S::kHelp;
+        F4 wa[kWalks], wh[kWalks];
+        int wch[kWalks], wq[kWalks];
+#pragma unroll
+        for (int x = 0; x < kWalks; ++x) {
+            const int v = tid + x * S::kHelp, of = v % S::kMain, r = of % S::kSegT;
+            wch[x] = v < 2 * S::kMain ? of / S::kSegT * S::kBlk + 2 * (r % S::kPairs) + v / S::kMain : CH, wq[x] = r / S::kPairs;
+            wa[x] = wch[x] < at.nch ? mul(kLog2e, load4(p.a + (at.d0 + wch[x]) * N, kS * wq[x], N)) : zero4();
+        }
+        auto fetch = [&](int i) {  // the checkpoints of tile i
+#pragma unroll
+            for (int x = 0; x < kWalks; ++x)
+                wh[x] = wch[x] < at.nch ? load4(p.ckpt + ((at.b * p.tiles + n - 1 - i) * p.channels + at.d0 + wch[x]) * N, kS * wq[x], N) : zero4();
+        };
+        auto walk = [&](int i) {
+#pragma unroll
+            for (int x = 0; x < kWalks; ++x) {
+                const int v = tid + x * S::kHelp;
+                if (v >= 2 * S::kMain) continue;
+                const float2 *step = sm.step[i & 1] + wch[x];
+                const float4 *bs = sm.b[i & 1] + wq[x];
+                float4 *mid = &sm.mid[i & 1][0][v / S::kMain][v % S::kMain];
+                F4 h = wh[x];
+                *mid = f4(h);
+#pragma unroll 1
+                for (int m = 1; m < kTile / kT; ++m) {
+                    F4 av[kT], bv[kT];
+#pragma unroll
+                    for (int k = 0; k < kT; ++k, step += CH, bs += P) {
+                        const float2 s = *step;
+                        av[k] = ex2(mul(s.x, wa[x]));
+                        bv[k] = mul(s.y, f4(*bs));
+                    }
+#pragma unroll
+                    for (int k = 0; k < kT; ++k) h = fma(av[k], h, bv[k]);
+                    mid[m * 2 * S::kMain] = f4(h);
                 }
             }
         };
@@ -208,30 +307,33 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
             sm.skip[i] = p.d && i < at.nch ? p.d[at.d0 + i] : 0.f;
         }
         load(0);
-        load(1);
-        load(2);
-        ptx::cp_async_wait<2>();
-        if (n > 0) prepare(0, nxt);
-        __syncthreads();  // (1) the first tile is ready
+        auto ahead = [&](int i) {  // make tile i ready
+            fetch(i);
+            ptx::cp_async_wait<0>();
+            ptx::named_sync(1, S::kHelp);  // every helper's copies of it have landed
+            load(i + 1);                   // into the other stage, which everyone has read
+            prepare(i, nxt);
+            ptx::named_sync(1, S::kHelp);
+            walk(i);
+        };
+        if (n > 0) ahead(0);
+        __syncthreads();  // the first tile is ready
         Kept old{};
         for (int i = 0; i < n; ++i) {
             old = cur, cur = nxt;
+            if (i + 1 < n) ahead(i + 1);
             if (i > 0) finish(i - 1, old);
-            __syncthreads();  // (2) the last tile's shares and sums are done with
-            ptx::cp_async_wait<1>();
-            if (i + 1 < n) prepare(i + 1, nxt);
-            load(i + 3);
-            __syncthreads();  // (3) this tile's shares and sums are complete, the next tile is ready
+            __syncthreads();  // tile i is done, i + 1 is ready
         }
         if (n > 0) finish(n - 1, cur);
         // the sums over tokens: sixteen threads' in order, through the shares' memory
         ptx::named_sync(1, S::kHelp);
-        vec::store<true>(sm.y + t * CH + oc, sd);
-        vec::store<true>(sm.gb + t * CH + oc, sb);
+        vec::store<true>(sm.share[0].y + t * CH + oc, sd);
+        vec::store<true>(sm.share[0].gb + t * CH + oc, sb);
         ptx::named_sync(1, S::kHelp);
         if (tid < at.nch) {
             float d = 0.f, b = 0.f;
-            for (int k = 0; k < kTile; ++k) d += sm.y[k * CH + tid], b += sm.gb[k * CH + tid];
+            for (int k = 0; k < kTile; ++k) d += sm.share[0].y[k * CH + tid], b += sm.share[0].gb[k * CH + tid];
             float *o = bp.d_part + at.b * 2 * p.channels + at.d0 + tid;
             o[0] = d;
             o[p.channels] = b;
@@ -258,10 +360,11 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
         g[j] = real[j] && bp.dstate_out ? load4(bp.dstate_out + (at.b * p.channels + d) * N, kS * q, N) : zero4();
         da[j] = zero4();
     }
-    // this lane's sum over channels: of d_b (0) or d_c (1), of which state; lanes that hold a copy leave nothing
-    const int value = ChSum::first(pair);
-    const bool leaves = pair % (S::kPairs / 8) == 0;
-    float *sums = &sm.sums[block][0][value / kS][kS * q + value % kS];
+    // this lane's part in turning sums over: token, which of d_b (0) and d_c (1), state group of the warp, first pair
+    constexpr int kGroups = 32 / S::kPairs, kPer = S::kPairs / 8;  // state groups of a warp, lanes that share a sum
+    const int lane = tid & 31, out = lane / kPer, out_t = out / (2 * kGroups), out_w = out / kGroups % 2, out_q = out % kGroups;
+    const int out_state = kS * (q / kGroups * kGroups + out_q);
+    float4 *turn = sm.turn[tid / 32];
     auto leave = [&](float *o, int t, float v0, float v1) {  // both channels' share of token t
         if constexpr (S::kShares == P) {
             *reinterpret_cast<float2 *>(o + (t * P + q) * CH + ch) = make_float2(v0, v1);
@@ -271,34 +374,16 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
             if (q % 4 == 0) *reinterpret_cast<float2 *>(o + (t * S::kShares + q / 4) * CH + ch) = make_float2(v0, v1);
         }
     };
-    __syncthreads();  // (1)
+    __syncthreads();  // the first tile is ready
     for (int i = 0; i < n; ++i) {
         const float2 *step = sm.step[i & 1] + ch;
         const float *rr = sm.r[i & 1] + ch;
         const float4 *bs = sm.b[i & 1] + q, *cs = sm.c[i & 1] + q;
-        const float *before = sm.x[i & 3].h;
-        auto first = [&](int j) { return real[j] ? load4(before + (ch + j) * N, kS * q, N) : zero4(); };
-        {
-            F4 h[2] = {first(0), first(1)};
-#pragma unroll 1
-            for (int m = 0; m < kTile / kT - 1; ++m) {
-#pragma unroll
-                for (int k = 0; k < kT; ++k) {
-                    const int t = m * kT + k;
-                    const float4 sd = *reinterpret_cast<const float4 *>(step + t * CH);
-                    const F4 b = f4(bs[t * P]);
-                    h[0] = fma(ex2(mul(sd.x, a2[0])), h[0], mul(sd.y, b));
-                    h[1] = fma(ex2(mul(sd.z, a2[1])), h[1], mul(sd.w, b));
-                }
-                sm.mid[m][0][tid] = f4(h[0]), sm.mid[m][1][tid] = f4(h[1]);
-            }
-        }
-        __syncthreads();  // (2)
+        auto &sh = sm.share[i & 1];
 #pragma unroll 1
         for (int m = kTile / kT - 1; m >= 0; --m) {
-            F4 av[kT][2], hv[kT][2], h_in[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) h_in[j] = m ? f4(sm.mid[m ? m - 1 : 0][j][tid]) : first(j);
+            F4 av[kT][2], hv[kT][2];
+            const F4 h_in[2] = {f4(sm.mid[i & 1][m][0][tid]), f4(sm.mid[i & 1][m][1][tid])};
 #pragma unroll
             for (int k = 0; k < kT; ++k) {
                 const int t = m * kT + k;
@@ -315,19 +400,32 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
                 const float2 rv = *reinterpret_cast<const float2 *>(rr + t * CH);
                 const F4 b = f4(bs[t * P]), c = f4(cs[t * P]);
                 const F4 g0 = fma(rv.x, c, g[0]), g1 = fma(rv.y, c, g[1]);
-                const F4 dc = fma(rv.y, hv[k][1], mul(rv.x, hv[k][0])), db = fma(sd.w, g1, mul(sd.y, g0));
-                leave(sm.y, t, dot(hv[k][0], c), dot(hv[k][1], c));
-                leave(sm.gb, t, dot(g0, b), dot(g1, b));
+                turn[(k * 2 + 0) * 32 + lane] = f4(fma(sd.w, g1, mul(sd.y, g0)));
+                turn[(k * 2 + 1) * 32 + lane] = f4(fma(rv.y, hv[k][1], mul(rv.x, hv[k][0])));
+                leave(sh.y, t, dot(hv[k][0], c), dot(hv[k][1], c));
+                leave(sh.gb, t, dot(g0, b), dot(g1, b));
                 g[0] = mul(av[k][0], g0), g[1] = mul(av[k][1], g1);
                 const F4 w0 = mul(g[0], k ? hv[k ? k - 1 : 0][0] : h_in[0]), w1 = mul(g[1], k ? hv[k ? k - 1 : 0][1] : h_in[1]);
-                leave(sm.aw, t, dot(w0, a2[0]), dot(w1, a2[1]));
+                leave(sh.aw, t, dot(w0, a2[0]), dot(w1, a2[1]));
                 da[0] = fma(sd.x, w0, da[0]), da[1] = fma(sd.z, w1, da[1]);
-                float v[8] = {db.lo.x, db.lo.y, db.hi.x, db.hi.y, dc.lo.x, dc.lo.y, dc.hi.x, dc.hi.y};
-                ChSum::run(v, pair);
-                if (leaves) sums[t * 2 * S::kN] = v[0];
             }
+            __syncwarp();
+            {
+                // eight pairs of channels, from another one on in each lane so that the reads meet in no bank
+                const float4 *from = turn + ((out_t * 2 + out_w) * kGroups + out_q) * S::kPairs + lane % kPer * 8;
+                F4 v = f4(from[out & 7]);
+#pragma unroll
+                for (int x = 1; x < 8; ++x) v = fma(1.f, f4(from[(out + x) & 7]), v);
+#pragma unroll
+                for (int o = kPer / 2; o >= 1; o /= 2) {
+                    v.lo.x += __shfl_xor_sync(0xffffffffu, v.lo.x, o), v.lo.y += __shfl_xor_sync(0xffffffffu, v.lo.y, o);
+                    v.hi.x += __shfl_xor_sync(0xffffffffu, v.hi.x, o), v.hi.y += __shfl_xor_sync(0xffffffffu, v.hi.y, o);
+                }
+                if (lane % kPer == 0) *reinterpret_cast<float4 *>(&sh.sums[block][m * kT + out_t][out_w][out_state]) = f4(v);
+            }
+            __syncwarp();
         }
-        __syncthreads();  // (3)
+        __syncthreads();  // tile i is done, i + 1 is ready
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
