@@ -29,14 +29,15 @@ int validate_dims(int64_t batch, int64_t seq, int64_t channels, int32_t taps, in
     return DC_OK;
 }
 
-bool vectors(const void *p, int64_t bs, int64_t ts, int64_t elem) {
-    return aligned(p, 16) && (bs * elem) % 16 == 0 && (ts * elem) % 16 == 0;
+// Whether every row of a tensor starts on a boundary of `n` elements.
+bool vectors(const void *p, int64_t bs, int64_t ts, int64_t elem, int64_t n) {
+    return aligned(p, (size_t)(elem * n)) && bs % n == 0 && ts % n == 0;
 }
 
 // Tokens per thread: as many as leave 16 warps for every SM (each run reads K - 1 tokens of its neighbour again, 5 %
-// at 64 tokens and 4 taps), between `least` and 64.
-int run_length(int64_t batch, int64_t seq, int64_t groups, int least) {
-    int run = 64;
+// at 64 tokens and 4 taps), between `least` and `most`.
+int run_length(int64_t batch, int64_t seq, int64_t groups, int least, int most) {
+    int run = most;
     while (run > least && batch * ceil_div(seq, run) * groups < (int64_t)sm_count() * 16) run /= 2;
     return run;
 }
@@ -70,13 +71,18 @@ int validate_conv(const dc_causal_conv_args *a) {
     return DC_OK;
 }
 
-template <typename TI, int VEC, bool ALIGNED>
+template <typename TI, typename TO, bool STAGED>
 void launch_conv(const cv::Params &p, dim3 grid, cudaStream_t s) {
+    const size_t smem = STAGED ? sizeof(typename cv::Ring<TI>::Buffer) * (cv::kThreads / 32) : 0;
+    auto go = [&](auto *kernel) {
+        if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        kernel<<<grid, cv::kThreads, smem, s>>>(p);
+    };
     switch (p.K) {
-        case 2: cv::conv_kernel<TI, VEC, ALIGNED, 2><<<grid, cv::kThreads, 0, s>>>(p); break;
-        case 3: cv::conv_kernel<TI, VEC, ALIGNED, 3><<<grid, cv::kThreads, 0, s>>>(p); break;
-        case 4: cv::conv_kernel<TI, VEC, ALIGNED, 4><<<grid, cv::kThreads, 0, s>>>(p); break;
-        default: cv::conv_kernel<TI, VEC, ALIGNED, cv::kMaxTaps><<<grid, cv::kThreads, 0, s>>>(p); break;
+        case 2: go(&cv::conv_kernel<TI, TO, STAGED, 2>); break;
+        case 3: go(&cv::conv_kernel<TI, TO, STAGED, 3>); break;
+        case 4: go(&cv::conv_kernel<TI, TO, STAGED, 4>); break;
+        default: go(&cv::conv_kernel<TI, TO, STAGED, cv::kMaxTaps>); break;
     }
 }
 
@@ -86,16 +92,22 @@ int run_conv(const dc_causal_conv_args *a, cv::Params p, cudaStream_t s) {
         cv::conv_step_kernel<TI><<<(unsigned)ceil_div(a->batch * a->channels, 256), 256, 0, s>>>(p);
         return launched();
     }
-    const int64_t is = sizeof(TI), os = dtype_size(a->out_dtype);
-    const bool vec = a->channels % 8 == 0 && vectors(a->x, p.x_b, p.x_t, is) && vectors(a->y, p.y_b, p.y_t, os);
-    const int64_t groups = ceil_div(a->channels, 32 * (vec ? 8 : 1));
-    p.run = run_length(a->batch, a->seq, groups, cv::kUnroll);
+    const int64_t el = 16 / (int64_t)sizeof(TI);
+    const bool staged = a->channels % el == 0 && vectors(a->x, p.x_b, p.x_t, sizeof(TI), el);
+    p.y_pair = vectors(a->y, p.y_b, p.y_t, dtype_size(a->out_dtype), cv::kVec);
+    const int64_t groups = ceil_div(a->channels, cv::kRow);
+    p.run = run_length(a->batch, a->seq, groups, cv::kStageTokens, 128);
     p.runs = (int32_t)(a->seq > 0 ? ceil_div(a->seq, p.run) : 1);
     const int64_t ctas = ceil_div(a->batch * p.runs, cv::kThreads / 32);
     if (ctas > 0x7fffffff) return DC_EUNSUPPORTED;
     const dim3 grid((unsigned)ctas, (unsigned)groups);
-    if (vec) launch_conv<TI, 8, true>(p, grid, s);
-    else launch_conv<TI, 1, false>(p, grid, s);
+    if (a->out_dtype == DC_BF16) {
+        if (staged) launch_conv<TI, __nv_bfloat16, true>(p, grid, s);
+        else launch_conv<TI, __nv_bfloat16, false>(p, grid, s);
+    } else {
+        if (staged) launch_conv<TI, float, true>(p, grid, s);
+        else launch_conv<TI, float, false>(p, grid, s);
+    }
     return launched();
 }
 
@@ -134,22 +146,34 @@ struct BwdShape {
 BwdShape bwd_shape(const dc_causal_conv_bwd_args *a) {
     const int64_t is = dtype_size(a->in_dtype), os = dtype_size(a->out_dtype);
     BwdShape b;
-    b.vec = a->channels % 8 == 0 && vectors(a->x, a->x_batch_stride, a->x_token_stride, is) &&
-            vectors(a->d_x, a->d_x_batch_stride, a->d_x_token_stride, is) && vectors(a->d_y, a->d_y_batch_stride, a->d_y_token_stride, os);
-    b.groups = ceil_div(a->channels, 32 * (b.vec ? 4 : 1));
-    b.run = run_length(a->batch, a->seq, b.groups, 16);
+    b.vec = a->channels % cv::kVec == 0 && vectors(a->x, a->x_batch_stride, a->x_token_stride, is, cv::kVec) &&
+            vectors(a->d_x, a->d_x_batch_stride, a->d_x_token_stride, is, cv::kVec) &&
+            vectors(a->d_y, a->d_y_batch_stride, a->d_y_token_stride, os, cv::kVec);
+    b.groups = ceil_div(a->channels, cv::kRow);
+    b.run = run_length(a->batch, a->seq, b.groups, 16, 64);
     b.runs = a->seq > 0 ? ceil_div(a->seq, b.run) : 1;
     b.ctas = ceil_div(a->batch * b.runs, cv::kBwdThreads / 32);
     return b;
 }
 
-template <typename TI, int VEC, bool ALIGNED>
+template <typename TI, typename TO, bool ALIGNED>
 void launch_bwd(const cv::BwdParams &p, dim3 grid, cudaStream_t s) {
     switch (p.K) {
-        case 2: cv::conv_bwd_kernel<TI, VEC, ALIGNED, 2><<<grid, cv::kBwdThreads, 0, s>>>(p); break;
-        case 3: cv::conv_bwd_kernel<TI, VEC, ALIGNED, 3><<<grid, cv::kBwdThreads, 0, s>>>(p); break;
-        case 4: cv::conv_bwd_kernel<TI, VEC, ALIGNED, 4><<<grid, cv::kBwdThreads, 0, s>>>(p); break;
-        default: cv::conv_bwd_kernel<TI, VEC, ALIGNED, cv::kMaxTaps><<<grid, cv::kBwdThreads, 0, s>>>(p); break;
+        case 2: cv::conv_bwd_kernel<TI, TO, ALIGNED, 2><<<grid, cv::kBwdThreads, 0, s>>>(p); break;
+        case 3: cv::conv_bwd_kernel<TI, TO, ALIGNED, 3><<<grid, cv::kBwdThreads, 0, s>>>(p); break;
+        case 4: cv::conv_bwd_kernel<TI, TO, ALIGNED, 4><<<grid, cv::kBwdThreads, 0, s>>>(p); break;
+        default: cv::conv_bwd_kernel<TI, TO, ALIGNED, cv::kMaxTaps><<<grid, cv::kBwdThreads, 0, s>>>(p); break;
+    }
+}
+
+template <typename TI>
+void launch_bwd_as(bool vec, const cv::BwdParams &p, dim3 grid, cudaStream_t s) {
+    if (p.y_dt) {
+        if (vec) launch_bwd<TI, __nv_bfloat16, true>(p, grid, s);
+        else launch_bwd<TI, __nv_bfloat16, false>(p, grid, s);
+    } else {
+        if (vec) launch_bwd<TI, float, true>(p, grid, s);
+        else launch_bwd<TI, float, false>(p, grid, s);
     }
 }
 
@@ -177,16 +201,7 @@ int dc_causal_conv(const dc_causal_conv_args *a, dc_stream_t stream) {
 
 uint64_t dc_causal_conv_bwd_workspace_size(const dc_causal_conv_bwd_args *a) {
     if (validate_bwd_dims(a) != DC_OK || a->batch == 0 || a->channels == 0) return 0;
-    // the larger of the aligned and the unaligned launch, so that the size depends on no pointer
-    dc_causal_conv_bwd_args q = *a;
-    uint64_t most = 0;
-    for (int i = 0; i < 2; ++i) {
-        q.x = q.d_x = reinterpret_cast<void *>((uintptr_t)(16 + i)), q.d_y = reinterpret_cast<void *>((uintptr_t)(16 + i));
-        q.x_batch_stride = q.x_token_stride = q.d_x_batch_stride = q.d_x_token_stride = q.d_y_batch_stride = q.d_y_token_stride = 8;
-        const uint64_t n = (uint64_t)bwd_shape(&q).ctas * (uint64_t)(a->taps + 1) * (uint64_t)a->channels * 4;
-        most = n > most ? n : most;
-    }
-    return most;
+    return (uint64_t)bwd_shape(a).ctas * (uint64_t)(a->taps + 1) * (uint64_t)a->channels * 4;
 }
 
 int dc_causal_conv_bwd(const dc_causal_conv_bwd_args *a, dc_stream_t stream) {
@@ -219,13 +234,8 @@ int dc_causal_conv_bwd(const dc_causal_conv_bwd_args *a, dc_stream_t stream) {
         p.dx = a->d_x, p.dwin_in = a->d_window_in;
         p.part = static_cast<float *>(a->workspace);
         const dim3 grid((unsigned)b.ctas, (unsigned)b.groups);
-        if (a->in_dtype == DC_BF16) {
-            if (b.vec) launch_bwd<__nv_bfloat16, 4, true>(p, grid, s);
-            else launch_bwd<__nv_bfloat16, 1, false>(p, grid, s);
-        } else {
-            if (b.vec) launch_bwd<float, 4, true>(p, grid, s);
-            else launch_bwd<float, 1, false>(p, grid, s);
-        }
+        if (a->in_dtype == DC_BF16) launch_bwd_as<__nv_bfloat16>(b.vec, p, grid, s);
+        else launch_bwd_as<float>(b.vec, p, grid, s);
         st = launched();
         if (st != DC_OK) return st;
     }

@@ -4,24 +4,30 @@
 //   pre_t = bias + sum_j w_j x_{t-K+1+j},  y_t = pre_t sigma(pre_t)  (or pre_t)
 //   backward, with e_t = dy_t dy/dpre:  dx_t = sum_j w_j e_{t+K-1-j},  dw_j = sum_t e_t x_{t-K+1+j},  db = sum_t e_t
 //
-// HBM-bound.  A thread owns a few adjacent channels and a run of tokens: it reads its channels' tokens one after the
-// other (a warp reads 32 such channel groups side by side, whole 128-byte lines), keeps the last K - 1 in registers,
-// and so reads each input once but for the K - 1 tokens before its run, which its neighbour's loads have just brought
-// into the caches.  The backward recomputes pre from x and carries the K unfinished sums of dx in registers the same
-// way; its run starts at its first token and ends K - 1 tokens past its last.
+// HBM-bound.  A thread owns a pair of adjacent channels, in two-wide arithmetic, and a run of tokens: it works on its
+// channels' tokens one after the other, keeps the last K - 1 in registers, and so reads each input once but for the K - 1
+// tokens before its run.  Where rows start on 16-byte boundaries each warp stages its 64 channels' tokens through a ring of
+// its own in shared memory (asynchronous copies, 48 tokens ahead, no barrier beyond the warp), so that the bytes in flight
+// do not depend on registers; loads into registers, eight tokens at a time, took 69 us at 8 x 4096 x 2048 bfloat16 where this
+// takes 62 (4.3 TB/s; the exponentials and reciprocals are next, at about half their rate).  The backward recomputes pre from x and carries the K unfinished sums of dx in registers the same way; its run
+// ends K - 1 tokens past its last.
 #pragma once
 
 #include "common.cuh"
+#include "ptx.cuh"
 #include "vec.cuh"
 
 namespace dc {
 namespace conv {
 
 constexpr int kMaxTaps = 8;
-constexpr int kThreads = 128;  // forward: four runs side by side
-constexpr int kUnroll = 8;     // tokens whose loads are in flight together
+constexpr int kThreads = 128;  // four runs side by side
+constexpr int kVec = 2;        // channels of a thread
+constexpr int kRow = 32 * kVec;
+constexpr int kStages = 4, kStageTokens = 16;  // of a warp's ring
+constexpr int kUnroll = 8;     // without it: tokens whose loads are in flight together
 constexpr int kBwdThreads = 256;
-constexpr int kBwdUnroll = 4;
+constexpr int kBwdUnroll = 8;
 
 struct Params {
     int64_t batch, seq, channels;
@@ -29,6 +35,7 @@ struct Params {
     int32_t K, silu, run;  // run: tokens per thread, a multiple of kUnroll
     int32_t runs;          // runs of a sequence
     int32_t y_dt;
+    int32_t y_pair;        // pairs of y's channels are aligned
     const void *x;
     const float *weight, *bias, *window_in;
     const int32_t *lengths;
@@ -36,8 +43,13 @@ struct Params {
     float *window_out;
 };
 
-// sigma(x) with the fast exponential (x -> -inf gives 0): a few ulp
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+// sigma(x) from the fast exponential and reciprocal (x -> -inf gives 0): a few ulp
+__device__ __forceinline__ float sigmoid(float x) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return r;
+}
 
 __device__ __forceinline__ int64_t length_of(const int32_t *lengths, int64_t b, int64_t seq) {
     if (!lengths) return seq;
@@ -52,86 +64,158 @@ __device__ __forceinline__ float token(const TI *x, int64_t x_t, const float *wi
     return win && t >= -K ? win[c * K + K + t] : 0.f;
 }
 
-// VEC channels per thread (with ALIGNED their loads and stores are whole vectors); KT: taps compiled in (the call's own,
-// or kMaxTaps with the first KT - K of them left out).
-template <typename TI, int VEC, bool ALIGNED, int KT>
+__device__ __forceinline__ float2 sigmoid2(float2 x) {
+    const float2 z = vec::mul2(x, vec::both(-1.4426950408889634f));
+    float2 e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(z.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(z.y));
+    e = vec::add2(e, vec::both(1.f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
+    return r;
+}
+// silu(x) or x, of a pair
+__device__ __forceinline__ float2 activate(float2 a, bool silu) { return silu ? vec::mul2(a, sigmoid2(a)) : a; }
+
+// A warp's ring: `count` tokens of 64 channels (nch of them real) from src on.
+template <typename T>
+struct Ring {
+    static constexpr int kPer = kRow * sizeof(T) / 16, kEl = 16 / sizeof(T);       // copies per row
+    static constexpr int kRows = 32 / kPer, kEach = kStageTokens / kRows;          // rows of a warp's pass, passes of a stage
+    using Buffer = T[kStages][kStageTokens][kRow];
+    const T *src;  // this lane's first copy of the next stage
+    int64_t stride;
+    uint32_t dst;
+    int left, row, s;  // tokens not yet asked for; stage
+    bool on;
+    __device__ __forceinline__ Ring(Buffer &buf, const T *from, int64_t stride, int count, int nch, int lane) : stride(stride), left(count), s(0) {
+        row = lane / kPer;
+        const int q = lane % kPer;
+        on = q * kEl < nch;
+        src = from + row * stride + (on ? q * kEl : 0);
+        dst = ptx::smem_u32(&buf[0][row][q * kEl]);
+    }
+    __device__ __forceinline__ void load() {  // the next stage (one commit whatever there is)
+        if (left > 0) {
+            const uint32_t to = dst + s * (int)sizeof(T) * kStageTokens * kRow;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const bool in = on && row + i * kRows < left;
+                ptx::cp_async16(to + i * (int)sizeof(T) * kRows * kRow, in ? src + i * kRows * stride : src - row * stride, in ? 16u : 0u);
+            }
+            src += kStageTokens * stride;
+            left -= kStageTokens;
+            s = s + 1 < kStages ? s + 1 : 0;
+        }
+        ptx::cp_async_commit();
+    }
+};
+
+// STAGED: rows start on 16-byte boundaries.  KT: taps compiled in (the call's own, or kMaxTaps with the first KT - K of
+// them left out).
+template <typename TI, typename TO, bool STAGED, int KT>
 __global__ void __launch_bounds__(kThreads) conv_kernel(const Params p) {
+    extern __shared__ __align__(16) unsigned char smem_bytes[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t item = (int64_t)blockIdx.x * (kThreads / 32) + warp;  // (sequence, run)
     if (item >= p.batch * p.runs) return;
     const int64_t b = item / p.runs, t0 = (item - b * p.runs) * (int64_t)p.run;
-    const int64_t c0 = ((int64_t)blockIdx.y * 32 + lane) * VEC;
-    if (c0 >= p.channels) return;
-    const int n = p.channels - c0 < VEC ? (int)(p.channels - c0) : VEC;
+    const int64_t c0 = (int64_t)blockIdx.y * kRow + lane * kVec;
+    const int n = c0 >= p.channels ? 0 : p.channels - c0 < kVec ? (int)(p.channels - c0) : kVec;
     const int K = KT == kMaxTaps ? p.K : KT;
     const int64_t len = length_of(p.lengths, b, p.seq);
     const int64_t t1 = t0 + p.run < p.seq ? t0 + p.run : p.seq;
     const int64_t live = t1 < len ? t1 : len;  // tokens from here on are zeros
     const TI *x = static_cast<const TI *>(p.x) + b * p.x_b;
     const float *win = p.window_in ? p.window_in + b * p.channels * K : nullptr;
-    const int64_t yb = b * p.y_b + c0;
+    TO *y = static_cast<TO *>(p.y) + b * p.y_b + c0;
+    const bool pair = n == kVec && p.y_pair;  // both channels in one store
 
     if (t0 < live) {
+        const int count = (int)(live - t0);
+        const int64_t row0 = (int64_t)blockIdx.y * kRow;
+        auto &buf = reinterpret_cast<typename Ring<TI>::Buffer *>(smem_bytes)[warp];
+        Ring<TI> ring(buf, x + t0 * p.x_t + row0, p.x_t, STAGED ? count : 0, (int)(p.channels - row0 < kRow ? p.channels - row0 : kRow), lane);
+        if (STAGED)
+#pragma unroll
+            for (int s = 0; s < kStages - 1; ++s) ring.load();
         // w[j] belongs to token t - (KT - 1) + j
-        float w[KT][VEC], bias[VEC], hist[KT - 1][VEC];
+        float2 w[KT], hist[KT - 1], bias = vec::both(0.f);
+        const int64_t ca = n > 0 ? c0 : 0, cb = n > 1 ? c0 + 1 : ca;
+        if (p.bias) bias = make_float2(p.bias[ca], p.bias[cb]);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const int64_t c = c0 + (e < n ? e : 0);
-#pragma unroll
-            for (int j = 0; j < KT; ++j) w[j][e] = j >= KT - K ? p.weight[c * K + j - (KT - K)] : 0.f;
-            bias[e] = p.bias ? p.bias[c] : 0.f;
-        }
+        for (int j = 0; j < KT; ++j)
+            w[j] = j >= KT - K ? make_float2(p.weight[ca * K + j - (KT - K)], p.weight[cb * K + j - (KT - K)]) : vec::both(0.f);
 #pragma unroll
         for (int j = 0; j < KT - 1; ++j) {
             const int64_t t = t0 - (KT - 1) + j;
-            if (t >= 0) {
-                vec::load<ALIGNED>(x + t * p.x_t + c0, hist[j], n);
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) hist[j][e] = e < n ? token(x, p.x_t, win, K, t, c0 + e) : 0.f;
-            }
+            hist[j] = j >= KT - K ? make_float2(token(x, p.x_t, win, K, t, ca), token(x, p.x_t, win, K, t, cb)) : vec::both(0.f);
         }
-        for (int64_t t = t0; t < live; t += kUnroll) {
-            float in[kUnroll][VEC];
+        TO *to = y + t0 * p.y_t;
+        auto next = [&](float2 v, TO *to) {  // one token's output, and the history one token on
+            float2 a = bias;
 #pragma unroll
-            for (int i = 0; i < kUnroll; ++i) {  // past the end: the last token again, not used
-                const int64_t ti = t + i < live ? t + i : live - 1;
-                vec::load<ALIGNED>(x + ti * p.x_t + c0, in[i], n);
-            }
+            for (int j = 0; j < KT - 1; ++j) a = vec::fma2(w[j], hist[j], a);
+            a = activate(vec::fma2(w[KT - 1], v, a), p.silu);
 #pragma unroll
-            for (int i = 0; i < kUnroll; ++i) {
-                if (t + i < live) {
-                    float out[VEC];
+            for (int j = 0; j < KT - 2; ++j) hist[j] = j >= KT - K ? hist[j + 1] : vec::both(0.f);
+            if (KT - 2 >= KT - K) hist[KT - 2] = v;
+            const float out[kVec] = {a.x, a.y};
+            if (pair) vec::store<true>(to, out);
+            else vec::store<false>(to, out, n);
+        };
+        if constexpr (STAGED) {
+            const TI *from = &buf[0][0][lane * kVec];
+            auto at = [&](int i) {
+                float v[kVec];
+                vec::load<true>(from + i * kRow, v);
+                return make_float2(v[0], v[1]);
+            };
+            for (int left = count, s = 0; left > 0; left -= kStageTokens) {
+                ptx::cp_async_wait<kStages - 2>();
+                __syncwarp();  // every lane's copies of this stage have landed, and the last stage has been read
+                ring.load();
+                if (left >= kStageTokens) {
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        float a = bias[e];
-#pragma unroll
-                        for (int j = 0; j < KT - 1; ++j)
-                            if (j >= KT - K) a = fmaf(w[j][e], hist[j][e], a);
-                        a = fmaf(w[KT - 1][e], in[i][e], a);
-                        out[e] = p.silu ? a * sigmoid(a) : a;
-                    }
-                    vec::store_as<ALIGNED>(p.y_dt, p.y, yb + (t + i) * p.y_t, out, n);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-#pragma unroll
-                        for (int j = 0; j < KT - 2; ++j) hist[j][e] = hist[j + 1][e];
-                        hist[KT - 2][e] = in[i][e];
-                    }
+                    for (int i = 0; i < kStageTokens; ++i) next(at(i), to + i * p.y_t);
+                } else {
+                    for (int i = 0; i < left; ++i) next(at(i), to + i * p.y_t);
                 }
+                to += kStageTokens * p.y_t;
+                s = s + 1 < kStages ? s + 1 : 0;
+                from = &buf[s][0][lane * kVec];
+            }
+            ptx::cp_async_wait<0>();
+        } else if (n > 0) {
+            const TI *from = x + t0 * p.x_t + c0;
+            int t = 0;
+            for (; t + kUnroll <= count; t += kUnroll, from += kUnroll * p.x_t) {
+                vec::Raw<TI, kVec> in[kUnroll];
+#pragma unroll
+                for (int i = 0; i < kUnroll; ++i) vec::load_raw<false>(from + i * p.x_t, in[i], n);
+#pragma unroll
+                for (int i = 0; i < kUnroll; ++i) next(vec::pair_of(in[i], 0), to + i * p.y_t);
+                to += kUnroll * p.y_t;
+            }
+            for (; t < count; ++t, from += p.x_t) {
+                vec::Raw<TI, kVec> in;
+                vec::load_raw<false>(from, in, n);
+                next(vec::pair_of(in, 0), to);
+                to += p.y_t;
             }
         }
     }
     if (t1 > live) {
-        float zero[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) zero[e] = 0.f;
-        for (int64_t t = t0 > live ? t0 : live; t < t1; ++t) vec::store_as<ALIGNED>(p.y_dt, p.y, yb + t * p.y_t, zero, n);
+        const float zero[kVec] = {0.f, 0.f};
+        for (int64_t t = t0 > live ? t0 : live; t < t1; ++t) {
+            if (pair) vec::store<true>(y + t * p.y_t, zero);
+            else vec::store<false>(y + t * p.y_t, zero, n);
+        }
     }
     // the next window, from the run that holds the last token (the first run when there is none)
     if (p.window_out && (len == 0 ? t0 == 0 : t0 < len && len <= t0 + p.run)) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
+        for (int e = 0; e < kVec; ++e)
             if (e < n)
                 for (int j = 0; j < K; ++j)
                     p.window_out[(b * p.channels + c0 + e) * K + j] = token(x, p.x_t, win, K, len - K + j, c0 + e);
@@ -183,24 +267,20 @@ struct BwdParams {
     float *part;  // [gridDim.x][K + 1][channels]: each CTA's sums of d_weight (K lines) and d_bias
 };
 
-// Channels of a warp: 32 * VEC.  The CTA's warps take consecutive runs of the same channels and add their sums in
-// order in shared memory.
-template <typename TI, int VEC, bool ALIGNED, int KT>
+// A pair of channels per thread (with ALIGNED as one access), 64 of a warp.  The CTA's warps take consecutive runs of the
+// same channels and add their sums in order in shared memory.
+template <typename TI, typename TO, bool ALIGNED, int KT>
 __global__ void __launch_bounds__(kBwdThreads) conv_bwd_kernel(const BwdParams p) {
-    constexpr int kWarps = kBwdThreads / 32;
-    __shared__ float sums[kWarps][32 * VEC];
+    constexpr int kWarps = kBwdThreads / 32, VEC = kVec;
+    __shared__ float2 sums[kWarps][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t item = (int64_t)blockIdx.x * kWarps + warp;
     const int64_t c0 = ((int64_t)blockIdx.y * 32 + lane) * VEC;
     const int n = c0 >= p.channels ? 0 : p.channels - c0 < VEC ? (int)(p.channels - c0) : VEC;
     const int K = KT == kMaxTaps ? p.K : KT;
-    float dw[KT][VEC], db[VEC];
+    float2 dw[KT], db = vec::both(0.f);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        db[e] = 0.f;
-#pragma unroll
-        for (int j = 0; j < KT; ++j) dw[j][e] = 0.f;
-    }
+    for (int j = 0; j < KT; ++j) dw[j] = vec::both(0.f);
     if (item < p.batch * p.runs && n > 0) {
         const int64_t b = item / p.runs, t0 = (item - b * p.runs) * (int64_t)p.run;
         const int64_t len = length_of(p.lengths, b, p.seq);
@@ -210,103 +290,114 @@ __global__ void __launch_bounds__(kBwdThreads) conv_bwd_kernel(const BwdParams p
         const float *win = p.window_in ? p.window_in + b * p.channels * K : nullptr;
         const float *dnext = p.dwin_out ? p.dwin_out + b * p.channels * K : nullptr;
         float *dwin = p.dwin_in ? p.dwin_in + b * p.channels * K : nullptr;
-        float w[KT][VEC], bias[VEC], hist[KT - 1][VEC], d[KT][VEC];
+        const int64_t c1 = n > 1 ? c0 + 1 : c0;
+        float2 w[KT], hist[KT - 1], d[KT];
+        const float2 bias = p.bias ? make_float2(p.bias[c0], p.bias[c1]) : vec::both(0.f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const int64_t c = c0 + (e < n ? e : 0);
-#pragma unroll
-            for (int j = 0; j < KT; ++j) {
-                w[j][e] = j >= KT - K ? p.weight[c * K + j - (KT - K)] : 0.f;
-                d[j][e] = 0.f;
-            }
-            bias[e] = p.bias ? p.bias[c] : 0.f;
+        for (int j = 0; j < KT; ++j) {
+            w[j] = j >= KT - K ? make_float2(p.weight[c0 * K + j - (KT - K)], p.weight[c1 * K + j - (KT - K)]) : vec::both(0.f);
+            d[j] = vec::both(0.f);
         }
 #pragma unroll
         for (int j = 0; j < KT - 1; ++j) {
             const int64_t t = t0 - (KT - 1) + j;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) hist[j][e] = 0.f;
+            hist[j] = vec::both(0.f);
             if (j >= KT - K && t < len) {
-                if (t >= 0) {
-                    vec::load<ALIGNED>(x + t * p.x_t + c0, hist[j], n);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) hist[j][e] = e < n ? token(x, p.x_t, win, K, t, c0 + e) : 0.f;
-                }
+                hist[j].x = token(x, p.x_t, win, K, t, c0);
+                if (n > 1) hist[j].y = token(x, p.x_t, win, K, t, c1);
             }
         }
-        // d[j] gathers dx of token t - (KT - 1) + j while e_t passes by; after token t, d[0] is complete
-        const int64_t end = t1 + KT - 1;  // tokens past t1 only finish the run's last sums
-        for (int64_t t = t0; t < end; t += kBwdUnroll) {
-            float in[kBwdUnroll][VEC], go[kBwdUnroll][VEC];
+        // d[j] gathers dx of token t - (KT - 1) + j while the gradient of pre_t passes by; after token t, d[0] is complete
+        const int count = (int)(t1 - t0), end = count + KT - 1;               // tokens past t1 only finish the run's last sums
+        const int live = len - t0 < 0 ? 0 : len - t0 < end ? (int)(len - t0) : end;  // tokens that are read
+        const TI *from = x + t0 * p.x_t + c0;
+        const TO *gfrom = static_cast<const TO *>(p.dy) + b * p.dy_b + t0 * p.dy_t + c0;
+        auto pass = [&](float2 v, float2 g, bool read, bool own) {  // token t: its gradients into d, and into dw and db if its own
+            float2 pre = bias;
+#pragma unroll
+            for (int j = 0; j < KT - 1; ++j) pre = vec::fma2(w[j], hist[j], pre);
+            pre = vec::fma2(w[KT - 1], v, pre);
+            if (p.silu && read) {
+                const float2 s = sigmoid2(pre);
+                const float2 slope = vec::fma2(vec::mul2(pre, s), vec::fma2(s, vec::both(-1.f), vec::both(1.f)), s);
+                g = vec::mul2(g, slope);
+            }
+#pragma unroll
+            for (int j = 0; j < KT; ++j) d[j] = vec::fma2(w[j], g, d[j]);
+            if (own) {
+                db = vec::add2(db, g);
+#pragma unroll
+                for (int j = 0; j < KT - 1; ++j) dw[j] = vec::fma2(g, hist[j], dw[j]);
+                dw[KT - 1] = vec::fma2(g, v, dw[KT - 1]);
+            }
+        };
+        auto shift = [&](float2 v) {
+#pragma unroll
+            for (int j = 0; j < KT - 1; ++j) d[j] = d[j + 1];
+            d[KT - 1] = vec::both(0.f);
+#pragma unroll
+            for (int j = 0; j < KT - 2; ++j) hist[j] = j >= KT - K ? hist[j + 1] : vec::both(0.f);
+            if (KT - 2 >= KT - K) hist[KT - 2] = v;
+        };
+        auto any = [&](int t) {  // a token of whatever place
+            const bool read = t < live;
+            float2 v = vec::both(0.f), g = vec::both(0.f);
+            if (read) {
+                vec::Raw<TI, VEC> in;
+                vec::Raw<TO, VEC> gin;
+                vec::load_raw<ALIGNED>(from + t * p.x_t, in, n);
+                vec::load_raw<ALIGNED>(gfrom + t * p.dy_t, gin, n);
+                v = vec::pair_of(in, 0), g = vec::pair_of(gin, 0);
+            }
+            pass(v, g, read, t < count);
+            const int64_t tau = t0 + t - (KT - 1);  // d[0]'s token
+            if (tau >= t0) {
+                if (dnext && tau < len && tau >= len - K) {
+                    d[0].x += dnext[c0 * K + (int)(tau - len + K)];
+                    if (n > 1) d[0].y += dnext[c1 * K + (int)(tau - len + K)];
+                }
+                const float out[VEC] = {d[0].x, d[0].y};
+                vec::store<ALIGNED>(dx + tau * p.dx_t, out, n);
+            } else if (dwin && tau < 0 && tau >= -(K - 1)) {  // t0 is 0: a token of the window
+                const int m = K + (int)tau;
+                const bool more = dnext && m >= len;
+                dwin[c0 * K + m] = d[0].x + (more ? dnext[c0 * K + m - (int)len] : 0.f);
+                if (n > 1) dwin[c1 * K + m] = d[0].y + (more ? dnext[c1 * K + m - (int)len] : 0.f);
+            }
+            shift(v);
+        };
+        // from `stop` on every sum is zero; a run that lies behind the sequence's end has none at all
+        const int stop = live == 0 && t0 > 0 ? 0 : live + KT - 1 < end ? live + KT - 1 : end;
+        int t = 0;
+        for (; t < KT - 1 && t < stop; ++t) any(t);
+        // whole groups of tokens that are read, the run's own, and finish tokens before the window's gradient reaches
+        const int plain_end = (int)min((int64_t)min(count, live), dnext ? len - K + (KT - 1) - t0 : (int64_t)count);
+        const TI *f = from + t * p.x_t;
+        const TO *gf = gfrom + t * p.dy_t;
+        TI *o = dx + t0 * p.dx_t;
+        for (; t + kBwdUnroll <= plain_end; t += kBwdUnroll, f += kBwdUnroll * p.x_t, gf += kBwdUnroll * p.dy_t, o += kBwdUnroll * p.dx_t) {
+            vec::Raw<TI, VEC> in[kBwdUnroll];
+            vec::Raw<TO, VEC> gin[kBwdUnroll];
 #pragma unroll
             for (int i = 0; i < kBwdUnroll; ++i) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) in[i][e] = 0.f, go[i][e] = 0.f;
-                if (t + i < len) {
-                    vec::load<ALIGNED>(x + (t + i) * p.x_t + c0, in[i], n);
-                    vec::load_as<ALIGNED>(p.y_dt, p.dy, b * p.dy_b + (t + i) * p.dy_t + c0, go[i], n);
-                }
+                vec::load_raw<ALIGNED>(f + i * p.x_t, in[i], n);
+                vec::load_raw<ALIGNED>(gf + i * p.dy_t, gin[i], n);
             }
 #pragma unroll
             for (int i = 0; i < kBwdUnroll; ++i) {
-                const int64_t ti = t + i;
-                if (ti < end) {
-                    const bool mine = ti < t1;
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        float pre = bias[e];
-#pragma unroll
-                        for (int j = 0; j < KT - 1; ++j) pre = fmaf(w[j][e], hist[j][e], pre);
-                        pre = fmaf(w[KT - 1][e], in[i][e], pre);
-                        float g = go[i][e];
-                        if (p.silu) {
-                            const float s = sigmoid(pre);
-                            g *= s * fmaf(pre, 1.f - s, 1.f);
-                        }
-                        if (ti >= len) g = 0.f;
-#pragma unroll
-                        for (int j = 0; j < KT; ++j) d[j][e] = fmaf(w[j][e], g, d[j][e]);
-                        if (mine) {
-                            db[e] += g;
-#pragma unroll
-                            for (int j = 0; j < KT - 1; ++j) dw[j][e] = fmaf(g, hist[j][e], dw[j][e]);
-                            dw[KT - 1][e] = fmaf(g, in[i][e], dw[KT - 1][e]);
-                        }
-                    }
-                    const int64_t tau = ti - (KT - 1);  // d[0]'s token
-                    if (tau >= t0 && tau < p.seq) {
-                        if (dnext && tau < len && tau >= len - K) {
-#pragma unroll
-                            for (int e = 0; e < VEC; ++e)
-                                if (e < n) d[0][e] += dnext[(c0 + e) * K + (int)(tau - len + K)];
-                        }
-                        vec::store<ALIGNED>(dx + tau * p.dx_t, d[0], n);
-                    } else if (dwin && tau < 0 && tau >= -(K - 1)) {  // t0 is 0: a token of the window
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e)
-                            if (e < n) {
-                                const int m = K + (int)tau;
-                                const float more = dnext && m >= len ? dnext[(c0 + e) * K + m - (int)len] : 0.f;
-                                dwin[(c0 + e) * K + m] = d[0][e] + more;
-                            }
-                    }
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-#pragma unroll
-                        for (int j = 0; j < KT - 1; ++j) d[j][e] = d[j + 1][e];
-                        d[KT - 1][e] = 0.f;
-#pragma unroll
-                        for (int j = 0; j < KT - 2; ++j) hist[j][e] = j >= KT - K ? hist[j + 1][e] : 0.f;
-                        if (KT - 2 >= KT - K) hist[KT - 2][e] = in[i][e];
-                    }
-                }
+                const float2 v = vec::pair_of(in[i], 0);
+                pass(v, vec::pair_of(gin[i], 0), true, true);
+                const float out[VEC] = {d[0].x, d[0].y};
+                vec::store<ALIGNED>(o + i * p.dx_t, out, n);
+                shift(v);
             }
         }
+        for (; t < stop; ++t) any(t);
+        const float none[VEC] = {0.f, 0.f};
+        for (int64_t tau = t0 + (stop > KT - 1 ? stop - (KT - 1) : 0); tau < t1; ++tau) vec::store<ALIGNED>(dx + tau * p.dx_t, none, n);
         if (dwin && t0 == 0) {  // column 0 reaches the output only as an unshifted window
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                if (e < n) dwin[(c0 + e) * K] = dnext && len == 0 ? dnext[(c0 + e) * K] : 0.f;
+            dwin[c0 * K] = dnext && len == 0 ? dnext[c0 * K] : 0.f;
+            if (n > 1) dwin[c1 * K] = dnext && len == 0 ? dnext[c1 * K] : 0.f;
         }
     }
     // the CTA's sums: the warps' in order, one tap at a time
@@ -315,15 +406,14 @@ __global__ void __launch_bounds__(kBwdThreads) conv_bwd_kernel(const BwdParams p
     for (int j = 0; j < KT + 1; ++j) {
         if (j < KT - K) continue;
         __syncthreads();
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) sums[warp][lane * VEC + e] = j < KT ? dw[j < KT ? j : 0][e] : db[e];
+        sums[warp][lane] = j < KT ? dw[j < KT ? j : 0] : db;
         __syncthreads();
-        for (int i = threadIdx.x; i < 32 * VEC; i += kBwdThreads) {
-            float v = sums[0][i];
+        if (warp == 0) {
+            float2 v = sums[0][lane];
 #pragma unroll
-            for (int q = 1; q < kWarps; ++q) v += sums[q][i];
-            const int64_t c = (int64_t)blockIdx.y * 32 * VEC + i;
-            if (c < p.channels) part[(int64_t)(j - (KT - K)) * p.channels + c] = v;
+            for (int q = 1; q < kWarps; ++q) v = vec::add2(v, sums[q][lane]);
+            if (n > 0) part[(int64_t)(j - (KT - K)) * p.channels + c0] = v.x;
+            if (n > 1) part[(int64_t)(j - (KT - K)) * p.channels + c0 + 1] = v.y;
         }
     }
 }

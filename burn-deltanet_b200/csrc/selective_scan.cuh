@@ -66,21 +66,9 @@ __device__ __forceinline__ float rcp(float x) {
 }
 __device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-kLog2e * x)); }
 
-// Pairs of float32 in one instruction (both lanes rounded as the single forms round them).
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
-        "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return r;
-}
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+using vec::both;
+using vec::fma2;
+using vec::mul2;
 
 // max(x, 0) + log(1 + e), e = exp(-|x|), with log(1 + e) = 2 atanh(s) at s = e / (2 + e) <= 1/3 by its series
 // s + s^3/3 + ... + s^11/11: full relative precision for small steps, where 1 + e would have rounded e away; the terms
