@@ -9,7 +9,7 @@ namespace {
 
 using namespace dc::host;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kMaxThreads = 512;
 
 bool valid_stride(int64_t stride, int64_t width, int64_t rows) { return rows <= 1 || stride >= width; }
 
@@ -24,20 +24,27 @@ struct Shape {
     int tpr, vpt, threads;
 };
 
-// Threads per row: two accesses of eight columns per thread where there are rows enough to fill the card (the
-// second access is in flight with the first), one where there are few rows and a row's own latency is all that
-// counts.
-Shape shape_of(int64_t rows, int64_t width, int max_tpr) {
+// Threads per row for `accesses` of eight columns per thread (the others are in flight with the first) where there are
+// rows enough to fill the card, and one where there are few rows and a row's own latency is all that counts.
+Shape shape_of(int64_t rows, int64_t width, int accesses) {
     const int64_t vecs = ceil_div(width, dc::rms::kVec);
-    const int want = rows <= 2 * (int64_t)sm_count() ? 1 : 2;
+    const int want = rows <= 2 * (int64_t)sm_count() ? 1 : accesses;
     Shape s;
     s.tpr = 32;
-    while (s.tpr < max_tpr && (int64_t)s.tpr * want < vecs) s.tpr *= 2;
+    while (s.tpr < kMaxThreads && (int64_t)s.tpr * want < vecs) s.tpr *= 2;
     s.vpt = (int)ceil_div(vecs, s.tpr);
     s.vpt = s.vpt <= 1 ? 1 : s.vpt <= 2 ? 2 : 4;
     s.threads = s.tpr > kThreads ? s.tpr : kThreads;
     return s;
 }
+
+// Two accesses; four for wide rows of 16-bit values, whose CTAs would otherwise be 512 threads (8192 x 8192 in bfloat16:
+// 86 us, 100 with two; with a float32 residual four no longer fit the registers).
+Shape fwd_shape(const dc_rms_norm_args *a) {
+    const bool narrow = a->x_dtype == DC_BF16 && (!a->residual_in || a->residual_dtype == DC_BF16);
+    return shape_of(a->rows, a->width, narrow && a->width > 4096 ? 4 : 2);
+}
+Shape bwd_shape(const dc_rms_norm_bwd_args *a) { return shape_of(a->rows, a->width, 2); }
 
 int validate_norm(const dc_rms_norm_args *a) {
     if (!a) return DC_EINVAL_ARG;
@@ -76,8 +83,18 @@ int validate_norm(const dc_rms_norm_args *a) {
 
 template <int VPT, bool F8>
 void launch_norm(bool vec, unsigned grid, const Shape &sh, const dc::rms::Params &p, cudaStream_t s) {
-    if (vec) dc::rms::rms_norm_kernel<VPT, true, F8><<<grid, sh.threads, 0, s>>>(p, sh.tpr);
-    else dc::rms::rms_norm_kernel<VPT, false, F8><<<grid, sh.threads, 0, s>>>(p, sh.tpr);
+    using bf16 = __nv_bfloat16;
+    if (!vec) dc::rms::rms_norm_kernel<VPT, F8><<<grid, sh.threads, 0, s>>>(p, sh.tpr);
+    else if (p.x_dt && p.r_dt) dc::rms::rms_norm_vec_kernel<bf16, bf16, VPT, F8><<<grid, sh.threads, 0, s>>>(p, sh.tpr);
+    else if (p.x_dt) dc::rms::rms_norm_vec_kernel<bf16, float, VPT, F8><<<grid, sh.threads, 0, s>>>(p, sh.tpr);
+    else if (p.r_dt) dc::rms::rms_norm_vec_kernel<float, bf16, VPT, F8><<<grid, sh.threads, 0, s>>>(p, sh.tpr);
+    else dc::rms::rms_norm_vec_kernel<float, float, VPT, F8><<<grid, sh.threads, 0, s>>>(p, sh.tpr);
+}
+
+// CTAs that stay: `per_sm` for every SM, never more than the rows give.
+unsigned grid_of(int64_t rows, const Shape &sh, int per_sm) {
+    const int64_t ctas = ceil_div(rows, sh.threads / sh.tpr), cap = (int64_t)sm_count() * per_sm;
+    return (unsigned)(ctas < cap ? ctas : cap);
 }
 
 // ---------------------------------------------------------------------------------------------- backward
@@ -110,21 +127,21 @@ int validate_norm_bwd_buffers(const dc_rms_norm_bwd_args *a) {
     return DC_OK;
 }
 
-// 512 threads per row at most: the row, its gradient and the d_weight sums are 96 registers a thread at four
-// accesses each.
-Shape bwd_shape(int64_t rows, int64_t width) { return shape_of(rows, width, 512); }
-
-// CTAs: the threads that fit an SM by registers (512: two 256-thread CTAs), never more than the rows give.
-unsigned bwd_grid(const dc_rms_norm_bwd_args *a, const Shape &sh) {
-    const int64_t per = sh.threads / sh.tpr, ctas = ceil_div(a->rows, per);
-    const int64_t cap = (int64_t)sm_count() * (sh.threads > 256 ? 1 : 2);
-    return (unsigned)(ctas < cap ? ctas : cap);
-}
+unsigned bwd_grid(const dc_rms_norm_bwd_args *a, const Shape &sh) { return grid_of(a->rows, sh, 512 / sh.threads); }
 
 template <int VPT>
 void launch_bwd(bool vec, unsigned grid, size_t smem, const Shape &sh, const dc::rms::BwdParams &p, cudaStream_t s) {
-    if (vec) dc::rms::rms_norm_bwd_kernel<VPT, true><<<grid, sh.threads, smem, s>>>(p, sh.tpr);
-    else dc::rms::rms_norm_bwd_kernel<VPT, false><<<grid, sh.threads, smem, s>>>(p, sh.tpr);
+    using bf16 = __nv_bfloat16;
+    if (!vec) {
+        dc::rms::rms_norm_bwd_kernel<VPT, false><<<grid, sh.threads, smem, s>>>(p, sh.tpr);
+    } else if constexpr (VPT == 4) {
+        dc::rms::rms_norm_bwd_kernel<VPT, true><<<grid, sh.threads, smem, s>>>(p, sh.tpr);
+    } else {
+        if (p.y_dt && p.r_dt) dc::rms::rms_norm_bwd_vec_kernel<bf16, bf16, VPT><<<grid, sh.threads, smem, s>>>(p, sh.tpr);
+        else if (p.y_dt) dc::rms::rms_norm_bwd_vec_kernel<bf16, float, VPT><<<grid, sh.threads, smem, s>>>(p, sh.tpr);
+        else if (p.r_dt) dc::rms::rms_norm_bwd_vec_kernel<float, bf16, VPT><<<grid, sh.threads, smem, s>>>(p, sh.tpr);
+        else dc::rms::rms_norm_bwd_vec_kernel<float, float, VPT><<<grid, sh.threads, smem, s>>>(p, sh.tpr);
+    }
 }
 
 }  // namespace
@@ -142,6 +159,8 @@ int dc_rms_norm(const dc_rms_norm_args *a, dc_stream_t stream) {
     p.rows = a->rows;
     p.width = (int32_t)a->width;
     p.group = a->group;
+    p.groups = a->group ? (int32_t)(a->width / a->group) : 1;
+    while (a->group && (dc::rms::kVec << p.group_shift) < a->group) ++p.group_shift;
     p.x_stride = a->x_stride, p.rin_stride = a->residual_in_stride, p.rout_stride = a->residual_out_stride, p.y_stride = a->y_stride;
     p.x_dt = a->x_dtype, p.r_dt = a->residual_dtype, p.y_dt = f8 ? 0 : a->out_dtype;
     p.eps = a->eps;
@@ -152,22 +171,23 @@ int dc_rms_norm(const dc_rms_norm_args *a, dc_stream_t stream) {
                      rows_aligned(a->residual_in, a->residual_in_stride, rs, a->rows) &&
                      rows_aligned(a->residual_out, a->residual_out_stride, rs, a->rows) &&
                      rows_aligned(a->y, a->y_stride, ys, a->rows) && aligned(a->weight, 16);
-    const Shape sh = shape_of(a->rows, a->width, 1024);
-    const int64_t ctas = ceil_div(a->rows, sh.threads / sh.tpr);
-    const unsigned grid = (unsigned)(ctas < 0x7fffffff ? ctas : 0x7fffffff);
+    const Shape sh = fwd_shape(a);
+    const unsigned grid = grid_of(a->rows, sh, 2048 / sh.threads);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     switch (sh.vpt * 2 + (f8 ? 1 : 0)) {
         case 2: launch_norm<1, false>(vec, grid, sh, p, s); break;
         case 3: launch_norm<1, true>(vec, grid, sh, p, s); break;
         case 4: launch_norm<2, false>(vec, grid, sh, p, s); break;
-        default: launch_norm<2, true>(vec, grid, sh, p, s); break;
+        case 5: launch_norm<2, true>(vec, grid, sh, p, s); break;
+        case 8: launch_norm<4, false>(vec, grid, sh, p, s); break;
+        default: launch_norm<4, true>(vec, grid, sh, p, s); break;
     }
     return launched();
 }
 
 uint64_t dc_rms_norm_bwd_workspace_size(const dc_rms_norm_bwd_args *a) {
     if (validate_norm_bwd(a) != DC_OK || !a->d_weight || a->rows == 0) return 0;
-    return (uint64_t)bwd_grid(a, bwd_shape(a->rows, a->width)) * (uint64_t)a->width * 4;
+    return (uint64_t)bwd_grid(a, bwd_shape(a)) * (uint64_t)a->width * 4;
 }
 
 int dc_rms_norm_bwd(const dc_rms_norm_bwd_args *a, dc_stream_t stream) {
@@ -200,7 +220,7 @@ int dc_rms_norm_bwd(const dc_rms_norm_bwd_args *a, dc_stream_t stream) {
                      rows_aligned(a->d_r, a->d_r_stride, rs, a->rows) && rows_aligned(a->r, a->r_stride, rs, a->rows) &&
                      rows_aligned(a->d_x, a->d_x_stride, xs, a->rows) && rows_aligned(a->d_residual, a->d_residual_stride, rs, a->rows) &&
                      aligned(a->weight, 16);
-    const Shape sh = bwd_shape(a->rows, a->width);
+    const Shape sh = bwd_shape(a);
     const unsigned grid = bwd_grid(a, sh);
     const size_t smem = (size_t)(sh.threads / sh.tpr - 1) * (size_t)a->width * 4;
     switch (sh.vpt) {

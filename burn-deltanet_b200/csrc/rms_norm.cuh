@@ -6,8 +6,9 @@
 //
 // HBM-bound: the forward reads x and the residual and writes the sum and y once, the backward reads dy, d_r and r
 // and writes d once; the row stays in registers between the reduction and its use.  A row is spread over TPR
-// threads (a power of two, 32 to 1024), eight consecutive columns per access, VPT accesses per thread; narrow
-// rows share a CTA.  The inverse root is recomputed in the backward from the row it reads anyway, so the forward
+// threads (a power of two, 32 to 512), eight consecutive columns per access, VPT accesses per thread; narrow
+// rows share a CTA.  CTAs stay and take row after row: the next row's loads are under way, as raw words, while this
+// one is reduced and written, and the weights stay in registers.  The inverse root is recomputed in the backward from the row it reads anyway, so the forward
 // saves nothing beside r.
 #pragma once
 
@@ -25,6 +26,7 @@ constexpr int kVec = 8;  // columns per access
 struct Params {
     int64_t rows;
     int32_t width, group;  // group: columns per scale (e4m3), 0 = the whole row
+    int32_t groups, group_shift;  // width / group; log2(group / kVec)
     int64_t x_stride, rin_stride, rout_stride, y_stride;
     int32_t x_dt, r_dt, y_dt;  // 0 float32, 1 bfloat16
     float eps;
@@ -34,9 +36,23 @@ struct Params {
     float *scale;
 };
 
-// Sum (or maximum) over the TPR threads of a row; every thread of the CTA calls it.  `red` holds one float per warp.
+// Sums (or maxima) over the TPR threads of a row; every thread of the CTA calls it.  `red` holds a pair per warp.
 template <bool MAX>
-__device__ __forceinline__ float row_reduce(float v, int tpr, float *red) {
+__device__ __forceinline__ float2 row_reduce(float2 v, int tpr, float2 *red) {
+    auto join = [](float2 a, float2 b) { return MAX ? make_float2(fmaxf(a.x, b.x), fmaxf(a.y, b.y)) : make_float2(a.x + b.x, a.y + b.y); };
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) v = join(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)));
+    if (tpr == 32) return v;
+    const int warp = threadIdx.x >> 5, per = tpr >> 5, first = warp & ~(per - 1);
+    __syncthreads();  // the last reduction's values have been read
+    if ((threadIdx.x & 31) == 0) red[warp] = v;
+    __syncthreads();
+    v = red[first];
+    for (int i = 1; i < per; ++i) v = join(v, red[first + i]);
+    return v;
+}
+template <bool MAX>
+__device__ __forceinline__ float row_reduce(float v, int tpr, float2 *red) {
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) {
         const float w = __shfl_xor_sync(0xffffffffu, v, o);
@@ -44,11 +60,11 @@ __device__ __forceinline__ float row_reduce(float v, int tpr, float *red) {
     }
     if (tpr == 32) return v;
     const int warp = threadIdx.x >> 5, per = tpr >> 5, first = warp & ~(per - 1);
-    __syncthreads();  // the last reduction's values have been read
-    if ((threadIdx.x & 31) == 0) red[warp] = v;
     __syncthreads();
-    v = red[first];
-    for (int i = 1; i < per; ++i) v = MAX ? fmaxf(v, red[first + i]) : v + red[first + i];
+    if ((threadIdx.x & 31) == 0) red[warp].x = v;
+    __syncthreads();
+    v = red[first].x;
+    for (int i = 1; i < per; ++i) v = MAX ? fmaxf(v, red[first + i].x) : v + red[first + i].x;
     return v;
 }
 
@@ -64,25 +80,152 @@ __device__ __forceinline__ uint2 to_e4m3(const float (&v)[kVec], float inv) {
     return make_uint2(w[0], w[1]);
 }
 
-// ALIGNED: width a multiple of 8 and every row of every tensor 16-byte aligned (8-byte for e4m3).
+// From the sum of one row on (s, n[i] columns of each access): its sum of squares, the stores, and y.  Every thread of the
+// CTA calls it, with s = 0 and on = false where it has no row.
 template <int VPT, bool ALIGNED, bool F8>
-__global__ void rms_norm_kernel(const Params p, int tpr) {
-    __shared__ float red[32];
-    const int tx = threadIdx.x & (tpr - 1), ty = threadIdx.x / tpr;
-    const int rows_per_cta = blockDim.x / tpr;
-    const float inv_width = 1.f / (float)p.width;
-    int n[VPT];  // columns of each access inside the row
+__device__ __forceinline__ void norm_row(const Params &p, float (&s)[VPT][kVec], const int (&n)[VPT], const float (&w)[VPT][kVec], int64_t row,
+                                         bool on, int tx, int tpr, float2 *red) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) ss = fmaf(s[i][e], s[i][e], ss);
+    if (p.rout && on) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+            if (n[i] > 0) vec::store_as<ALIGNED>(p.r_dt, p.rout, row * p.rout_stride + (tx + i * tpr) * kVec, s[i], n[i]);
+    }
+    ss = row_reduce<false>(ss, tpr, red);
+    const float inv = 1.f / sqrtf(fmaf(ss, 1.f / (float)p.width, p.eps));
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) s[i][e] *= inv * w[i][e];
+    if constexpr (!F8) {
+        if (on) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+                if (n[i] > 0) vec::store_as<ALIGNED>(p.y_dt, p.y, row * p.y_stride + (tx + i * tpr) * kVec, s[i], n[i]);
+        }
+    } else {
+        uint8_t *Y = static_cast<uint8_t *>(p.y);
+        float amax[VPT], all = 0.f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            amax[i] = 0.f;  // fmaxf drops a NaN: its row is NaN throughout, and keeps scale 1
+#pragma unroll
+            for (int e = 0; e < kVec; ++e)
+                if (ALIGNED || e < n[i]) amax[i] = fmaxf(amax[i], fabsf(s[i][e]));
+            all = fmaxf(all, amax[i]);
+        }
+        const int lanes = p.group ? p.group / kVec : 0;  // lanes of a group: 4 .. 32, a power of two
+        if (lanes) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1)
+                    if (o < lanes) amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], o));
+        } else {
+            all = row_reduce<true>(all, tpr, red);
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) amax[i] = all;
+        }
+        if (on) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                if (n[i] <= 0) continue;
+                const int v = tx + i * tpr;
+                const float scale = amax[i] > 0.f ? fmaxf(amax[i] * (1.f / 448.f), FLT_MIN) : 1.f;
+                if (lanes) {
+                    if ((v & (lanes - 1)) == 0) p.scale[row * p.groups + (v >> p.group_shift)] = scale;
+                } else if (v == 0) {
+                    p.scale[row] = scale;
+                }
+                const uint2 q = to_e4m3(s[i], __fdividef(1.f, scale));
+                uint8_t *o = Y + row * p.y_stride + v * kVec;
+                if constexpr (ALIGNED) {
+                    *reinterpret_cast<uint2 *>(o) = q;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e)
+                        if (e < n[i]) o[e] = (uint8_t)((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
+                }
+            }
+        }
+    }
+}
+
+// This thread's part of a row: columns of each access, and the weights.
+template <int VPT, bool ALIGNED>
+__device__ __forceinline__ void columns(int width, const float *weight, int tx, int tpr, int (&n)[VPT], float (&w)[VPT][kVec]) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-        const int left = p.width - (tx + i * tpr) * kVec;
+        const int left = width - (tx + i * tpr) * kVec;
         n[i] = left < 0 ? 0 : left > kVec ? kVec : left;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) w[i][e] = 0.f;
+        if (n[i] > 0) vec::load<ALIGNED>(weight + (tx + i * tpr) * kVec, w[i], n[i]);
     }
-    // every thread takes the same number of rounds, for the barriers in row_reduce
+}
+
+// Whole 16-byte accesses: width a multiple of 8 and every row of every tensor 16-byte aligned (8-byte for e4m3).  80
+// registers leave three CTAs of 256 an SM; two hold too few loads (16384 x 4096 into e4m3: 125 us, 140 at 96 registers).
+template <typename TX, typename TR, int VPT, bool F8>
+__global__ void __maxnreg__(VPT == 4 ? 128 : 80) rms_norm_vec_kernel(const Params p, int tpr) {
+    __shared__ float2 red[32];
+    const int tx = threadIdx.x & (tpr - 1), ty = threadIdx.x / tpr, rows_per_cta = blockDim.x / tpr;
+    int n[VPT];
+    float w[VPT][kVec];
+    columns<VPT, true>(p.width, p.weight, tx, tpr, n, w);
+    const TX *X = static_cast<const TX *>(p.x) + tx * kVec;
+    const TR *R = p.rin ? static_cast<const TR *>(p.rin) + tx * kVec : nullptr;
+    vec::Raw<TX, kVec> x[VPT];
+    vec::Raw<TR, kVec> r[VPT];
+    auto load = [&](int64_t row) {
+        if (row >= p.rows) return;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+            if (n[i] > 0) vec::load_raw<true>(X + row * p.x_stride + i * tpr * kVec, x[i], kVec);
+        if (R)
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+                if (n[i] > 0) vec::load_raw<true>(R + row * p.rin_stride + i * tpr * kVec, r[i], kVec);
+    };
+    const int64_t stride = (int64_t)gridDim.x * rows_per_cta;
+    int64_t row0 = (int64_t)blockIdx.x * rows_per_cta;
+    load(row0 + ty);
+    for (; row0 < p.rows; row0 += stride) {  // every thread takes the same number of rounds, for the barriers
+        const int64_t row = row0 + ty;
+        const bool on = row < p.rows;
+        float s[VPT][kVec];
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int e = 0; e < kVec; e += 2) {
+                float2 v = vec::both(0.f);
+                if (on && n[i] > 0) {
+                    v = vec::pair_of(x[i], e / 2);
+                    if (R) v = vec::add2(v, vec::pair_of(r[i], e / 2));
+                }
+                s[i][e] = v.x, s[i][e + 1] = v.y;
+            }
+        load(row + stride);
+        norm_row<VPT, true, F8>(p, s, n, w, row, on, tx, tpr, red);
+    }
+}
+
+// Any width, stride and alignment.
+template <int VPT, bool F8>
+__global__ void __launch_bounds__(512) rms_norm_kernel(const Params p, int tpr) {
+    __shared__ float2 red[32];
+    const int tx = threadIdx.x & (tpr - 1), ty = threadIdx.x / tpr, rows_per_cta = blockDim.x / tpr;
+    int n[VPT];
+    float w[VPT][kVec];
+    columns<VPT, false>(p.width, p.weight, tx, tpr, n, w);
     for (int64_t row0 = (int64_t)blockIdx.x * rows_per_cta; row0 < p.rows; row0 += (int64_t)gridDim.x * rows_per_cta) {
         const int64_t row = row0 + ty;
         const bool on = row < p.rows;
         float s[VPT][kVec];
-        float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int col = (tx + i * tpr) * kVec;
@@ -90,80 +233,13 @@ __global__ void rms_norm_kernel(const Params p, int tpr) {
 #pragma unroll
             for (int e = 0; e < kVec; ++e) s[i][e] = 0.f, r[e] = 0.f;
             if (on && n[i] > 0) {
-                vec::load_as<ALIGNED>(p.x_dt, p.x, row * p.x_stride + col, s[i], n[i]);
-                if (p.rin) vec::load_as<ALIGNED>(p.r_dt, p.rin, row * p.rin_stride + col, r, n[i]);
+                vec::load_as<false>(p.x_dt, p.x, row * p.x_stride + col, s[i], n[i]);
+                if (p.rin) vec::load_as<false>(p.r_dt, p.rin, row * p.rin_stride + col, r, n[i]);
             }
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) {
-                s[i][e] += r[e];
-                ss = fmaf(s[i][e], s[i][e], ss);
-            }
+            for (int e = 0; e < kVec; ++e) s[i][e] += r[e];
         }
-        if (p.rout && on) {
-#pragma unroll
-            for (int i = 0; i < VPT; ++i)
-                if (n[i] > 0) vec::store_as<ALIGNED>(p.r_dt, p.rout, row * p.rout_stride + (tx + i * tpr) * kVec, s[i], n[i]);
-        }
-        ss = row_reduce<false>(ss, tpr, red);
-        const float inv = 1.f / sqrtf(fmaf(ss, inv_width, p.eps));
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            if (n[i] > 0) {
-                float w[kVec];
-                vec::load<ALIGNED>(p.weight + (tx + i * tpr) * kVec, w, n[i]);
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) s[i][e] *= inv * w[e];
-            }
-        }
-        if constexpr (!F8) {
-            if (on) {
-#pragma unroll
-                for (int i = 0; i < VPT; ++i)
-                    if (n[i] > 0) vec::store_as<ALIGNED>(p.y_dt, p.y, row * p.y_stride + (tx + i * tpr) * kVec, s[i], n[i]);
-            }
-        } else {
-            uint8_t *Y = static_cast<uint8_t *>(p.y);
-            float amax[VPT], all = 0.f;
-#pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-                amax[i] = 0.f;  // fmaxf drops a NaN: its row is NaN throughout, and keeps scale 1
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) amax[i] = fmaxf(amax[i], fabsf(s[i][e]));
-                all = fmaxf(all, amax[i]);
-            }
-            const int lanes = p.group ? p.group / kVec : 0;  // lanes of a group: 4 .. 32, a power of two
-            if (lanes) {
-#pragma unroll
-                for (int i = 0; i < VPT; ++i)
-                    for (int o = lanes / 2; o >= 1; o >>= 1) amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], o));
-            } else {
-                all = row_reduce<true>(all, tpr, red);
-#pragma unroll
-                for (int i = 0; i < VPT; ++i) amax[i] = all;
-            }
-            if (on) {
-#pragma unroll
-                for (int i = 0; i < VPT; ++i) {
-                    if (n[i] <= 0) continue;
-                    const int v = tx + i * tpr;
-                    const float scale = amax[i] > 0.f ? fmaxf(amax[i] * (1.f / 448.f), FLT_MIN) : 1.f;
-                    if (lanes) {
-                        if (v % lanes == 0) p.scale[row * (p.width / p.group) + v / lanes] = scale;
-                    } else if (v == 0) {
-                        p.scale[row] = scale;
-                    }
-                    const uint2 q = to_e4m3(s[i], 1.f / scale);
-                    uint8_t *o = Y + row * p.y_stride + v * kVec;
-                    if constexpr (ALIGNED) {
-                        *reinterpret_cast<uint2 *>(o) = q;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < kVec; ++e)
-                            if (e < n[i]) o[e] = (uint8_t)((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
-                    }
-                }
-            }
-        }
+        norm_row<VPT, false, F8>(p, s, n, w, row, on, tx, tpr, red);
     }
 }
 
@@ -179,75 +255,48 @@ struct BwdParams {
     float *part;  // [gridDim.x, width] partial sums of d_weight, or null
 };
 
-// Persistent CTAs: each keeps its rows' share of d_weight in registers and writes it once, to its own line of
-// `part` (column_sum_kernel adds the lines in order).
-template <int VPT, bool ALIGNED>
-__global__ void __launch_bounds__(512) rms_norm_bwd_kernel(const BwdParams p, int tpr) {
-    __shared__ float red[32];
-    extern __shared__ float lines[];  // [rows per CTA - 1][width], when several rows share the CTA
-    const int tx = threadIdx.x & (tpr - 1), ty = threadIdx.x / tpr;
-    const int rows_per_cta = blockDim.x / tpr;
-    const float inv_width = 1.f / (float)p.width;
-    int n[VPT];
-    float dw[VPT][kVec];
+// From one row's r and dy on: the reductions, d, and the row's part of d_weight.  Every thread of the CTA calls it.
+// dr(i, d) and weight(i, w) give access i's d_r and weights.
+template <int VPT, bool ALIGNED, typename DR, typename W>
+__device__ __forceinline__ void bwd_row(const BwdParams &p, const float (&r)[VPT][kVec], const float (&g)[VPT][kVec], const int (&n)[VPT],
+                                        W &&weight, float (&dw)[VPT][kVec], DR &&dr, int64_t row, bool on, int tx, int tpr, float2 *red) {
+    float2 both = make_float2(0.f, 0.f);  // sum of r^2, sum of w dy r
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-        const int left = p.width - (tx + i * tpr) * kVec;
-        n[i] = left < 0 ? 0 : left > kVec ? kVec : left;
+        float w[kVec];
+        weight(i, w);
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) dw[i][e] = 0.f;
-    }
-    for (int64_t row0 = (int64_t)blockIdx.x * rows_per_cta; row0 < p.rows; row0 += (int64_t)gridDim.x * rows_per_cta) {
-        const int64_t row = row0 + ty;
-        const bool on = row < p.rows;
-        float r[VPT][kVec], g[VPT][kVec];
-        float ss = 0.f, dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) r[i][e] = 0.f, g[i][e] = 0.f;
-            if (on && n[i] > 0) {
-                const int col = (tx + i * tpr) * kVec;
-                vec::load_as<ALIGNED>(p.r_dt, p.r, row * p.r_stride + col, r[i], n[i]);
-                vec::load_as<ALIGNED>(p.y_dt, p.dy, row * p.dy_stride + col, g[i], n[i]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            float w[kVec];
-            if (n[i] > 0) vec::load<ALIGNED>(p.weight + (tx + i * tpr) * kVec, w, n[i]);
-            if (on && n[i] > 0) {
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                    ss = fmaf(r[i][e], r[i][e], ss);
-                    dot = fmaf(w[e] * g[i][e], r[i][e], dot);
-                }
-            }
-        }
-        ss = row_reduce<false>(ss, tpr, red);
-        dot = row_reduce<false>(dot, tpr, red);
-        const float inv = 1.f / sqrtf(fmaf(ss, inv_width, p.eps));
-        const float back = inv * inv * inv * (dot * inv_width);
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            if (!on || n[i] <= 0) continue;
-            const int col = (tx + i * tpr) * kVec;
-            float w[kVec], d[kVec];
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) d[e] = 0.f;
-            if (p.dr) vec::load_as<ALIGNED>(p.r_dt, p.dr, row * p.dr_stride + col, d, n[i]);
-            vec::load<ALIGNED>(p.weight + col, w, n[i]);
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) {
-                dw[i][e] = fmaf(g[i][e], r[i][e] * inv, dw[i][e]);
-                d[e] += fmaf(inv * w[e], g[i][e], -r[i][e] * back);
-            }
-            if (p.dx) vec::store_as<ALIGNED>(p.x_dt, p.dx, row * p.dx_stride + col, d, n[i]);
-            if (p.dres) vec::store_as<ALIGNED>(p.r_dt, p.dres, row * p.dres_stride + col, d, n[i]);
+        for (int e = 0; e < kVec; ++e) {
+            both.x = fmaf(r[i][e], r[i][e], both.x);
+            both.y = fmaf(w[e] * g[i][e], r[i][e], both.y);
         }
     }
+    both = row_reduce<false>(both, tpr, red);
+    const float inv_width = 1.f / (float)p.width;
+    const float inv = 1.f / sqrtf(fmaf(both.x, inv_width, p.eps));
+    const float back = inv * inv * inv * (both.y * inv_width);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        if (!on || n[i] <= 0) continue;
+        const int col = (tx + i * tpr) * kVec;
+        float d[kVec], w[kVec];
+        dr(i, d);
+        weight(i, w);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+            dw[i][e] = fmaf(g[i][e], r[i][e] * inv, dw[i][e]);
+            d[e] += fmaf(inv * w[e], g[i][e], -r[i][e] * back);
+        }
+        if (p.dx) vec::store_as<ALIGNED>(p.x_dt, p.dx, row * p.dx_stride + col, d, n[i]);
+        if (p.dres) vec::store_as<ALIGNED>(p.r_dt, p.dres, row * p.dres_stride + col, d, n[i]);
+    }
+}
+
+// The CTA's line of d_weight partial sums; rows that share the CTA: row group 0 adds the others' sums in order.
+template <int VPT>
+__device__ __forceinline__ void bwd_line(const BwdParams &p, const float (&dw)[VPT][kVec], const int (&n)[VPT], int tx, int ty, int tpr,
+                                         int rows_per_cta, float *lines) {
     if (!p.part) return;
-    // rows that share the CTA: row group 0 adds the others' sums in order
     if (rows_per_cta > 1) {
         if (ty > 0) {
 #pragma unroll
@@ -270,6 +319,116 @@ __global__ void __launch_bounds__(512) rms_norm_bwd_kernel(const BwdParams p, in
                     p.part[(int64_t)blockIdx.x * p.width + col] = v;
                 }
     }
+}
+
+// CTAs that stay: each keeps its rows' share of d_weight in registers and writes it once, to its own line of `part`
+// (column_sum_kernel adds the lines in order).  Whole 16-byte accesses, as in the forward.
+template <typename TY, typename TR, int VPT>
+__global__ void __launch_bounds__(512) rms_norm_bwd_vec_kernel(const BwdParams p, int tpr) {
+    __shared__ float2 red[32];
+    extern __shared__ float lines[];  // [rows per CTA - 1][width], when several rows share the CTA
+    const int tx = threadIdx.x & (tpr - 1), ty = threadIdx.x / tpr, rows_per_cta = blockDim.x / tpr;
+    int n[VPT];
+    float w[VPT][kVec], dw[VPT][kVec];
+    columns<VPT, true>(p.width, p.weight, tx, tpr, n, w);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) dw[i][e] = 0.f;
+    const TY *DY = static_cast<const TY *>(p.dy) + tx * kVec;
+    const TR *R = static_cast<const TR *>(p.r) + tx * kVec, *DR = p.dr ? static_cast<const TR *>(p.dr) + tx * kVec : nullptr;
+    vec::Raw<TY, kVec> gy[VPT];
+    vec::Raw<TR, kVec> rr[VPT], gr[VPT];
+    auto load = [&](int64_t row) {
+        if (row >= p.rows) return;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+            if (n[i] > 0) {
+                vec::load_raw<true>(R + row * p.r_stride + i * tpr * kVec, rr[i], kVec);
+                vec::load_raw<true>(DY + row * p.dy_stride + i * tpr * kVec, gy[i], kVec);
+            }
+    };
+    auto load_dr = [&](int64_t row) {
+        if (DR && row < p.rows)
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+                if (n[i] > 0) vec::load_raw<true>(DR + row * p.dr_stride + i * tpr * kVec, gr[i], kVec);
+    };
+    const int64_t stride = (int64_t)gridDim.x * rows_per_cta;
+    int64_t row0 = (int64_t)blockIdx.x * rows_per_cta;
+    load(row0 + ty);
+    for (; row0 < p.rows; row0 += stride) {
+        const int64_t row = row0 + ty;
+        const bool on = row < p.rows;
+        float r[VPT][kVec], g[VPT][kVec];
+        load_dr(row);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int e = 0; e < kVec; e += 2) {
+                const bool in = on && n[i] > 0;
+                const float2 a = in ? vec::pair_of(rr[i], e / 2) : vec::both(0.f), b = in ? vec::pair_of(gy[i], e / 2) : vec::both(0.f);
+                r[i][e] = a.x, r[i][e + 1] = a.y, g[i][e] = b.x, g[i][e + 1] = b.y;
+            }
+        load(row + stride);
+        auto dr = [&](int i, float (&d)[kVec]) {
+#pragma unroll
+            for (int e = 0; e < kVec; e += 2) {
+                const float2 v = DR ? vec::pair_of(gr[i], e / 2) : vec::both(0.f);
+                d[e] = v.x, d[e + 1] = v.y;
+            }
+        };
+        auto weight = [&](int i, float (&v)[kVec]) {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) v[e] = w[i][e];
+        };
+        bwd_row<VPT, true>(p, r, g, n, weight, dw, dr, row, on, tx, tpr, red);
+    }
+    bwd_line<VPT>(p, dw, n, tx, ty, tpr, rows_per_cta, lines);
+}
+
+// Any width, stride and alignment; and, ALIGNED, the widths whose rows leave no registers for loads under way and weights.
+template <int VPT, bool ALIGNED>
+__global__ void __launch_bounds__(512) rms_norm_bwd_kernel(const BwdParams p, int tpr) {
+    __shared__ float2 red[32];
+    extern __shared__ float lines[];
+    const int tx = threadIdx.x & (tpr - 1), ty = threadIdx.x / tpr, rows_per_cta = blockDim.x / tpr;
+    int n[VPT];
+    float dw[VPT][kVec];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int left = p.width - (tx + i * tpr) * kVec;
+        n[i] = left < 0 ? 0 : left > kVec ? kVec : left;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) dw[i][e] = 0.f;
+    }
+    for (int64_t row0 = (int64_t)blockIdx.x * rows_per_cta; row0 < p.rows; row0 += (int64_t)gridDim.x * rows_per_cta) {
+        const int64_t row = row0 + ty;
+        const bool on = row < p.rows;
+        float r[VPT][kVec], g[VPT][kVec];
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) r[i][e] = 0.f, g[i][e] = 0.f;
+            if (on && n[i] > 0) {
+                const int col = (tx + i * tpr) * kVec;
+                vec::load_as<ALIGNED>(p.r_dt, p.r, row * p.r_stride + col, r[i], n[i]);
+                vec::load_as<ALIGNED>(p.y_dt, p.dy, row * p.dy_stride + col, g[i], n[i]);
+            }
+        }
+        auto dr = [&](int i, float (&d)[kVec]) {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) d[e] = 0.f;
+            if (p.dr) vec::load_as<ALIGNED>(p.r_dt, p.dr, row * p.dr_stride + (tx + i * tpr) * kVec, d, n[i]);
+        };
+        auto weight = [&](int i, float (&v)[kVec]) {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) v[e] = 0.f;
+            if (n[i] > 0) vec::load<ALIGNED>(p.weight + (tx + i * tpr) * kVec, v, n[i]);
+        };
+        bwd_row<VPT, ALIGNED>(p, r, g, n, weight, dw, dr, row, on, tx, tpr, red);
+    }
+    bwd_line<VPT>(p, dw, n, tx, ty, tpr, rows_per_cta, lines);
 }
 
 }  // namespace rms
