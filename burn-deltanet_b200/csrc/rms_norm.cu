@@ -84,7 +84,8 @@ int validate_norm(const dc_rms_norm_args *a) {
 template <int VPT, bool F8>
 void launch_norm(bool vec, unsigned grid, const Shape &sh, const dc::rms::Params &p, cudaStream_t s) {
     using bf16 = __nv_bfloat16;
-    if (!vec) dc::rms::rms_norm_kernel<VPT, F8><<<grid, sh.threads, 0, s>>>(p, sh.tpr);
+    constexpr auto kAny = F8 ? dc::rms::Lay::kSide : dc::rms::Lay::kApart;  // the scales' groups are neighbouring columns
+    if (!vec) dc::rms::rms_norm_kernel<VPT, F8, kAny><<<grid, sh.threads, 0, s>>>(p, sh.tpr);
     else if (p.x_dt && p.r_dt) dc::rms::rms_norm_vec_kernel<bf16, bf16, VPT, F8><<<grid, sh.threads, 0, s>>>(p, sh.tpr);
     else if (p.x_dt) dc::rms::rms_norm_vec_kernel<bf16, float, VPT, F8><<<grid, sh.threads, 0, s>>>(p, sh.tpr);
     else if (p.r_dt) dc::rms::rms_norm_vec_kernel<float, bf16, VPT, F8><<<grid, sh.threads, 0, s>>>(p, sh.tpr);
@@ -133,9 +134,9 @@ template <int VPT>
 void launch_bwd(bool vec, unsigned grid, size_t smem, const Shape &sh, const dc::rms::BwdParams &p, cudaStream_t s) {
     using bf16 = __nv_bfloat16;
     if (!vec) {
-        dc::rms::rms_norm_bwd_kernel<VPT, false><<<grid, sh.threads, smem, s>>>(p, sh.tpr);
+        dc::rms::rms_norm_bwd_kernel<VPT, dc::rms::Lay::kApart><<<grid, sh.threads, smem, s>>>(p, sh.tpr);
     } else if constexpr (VPT == 4) {
-        dc::rms::rms_norm_bwd_kernel<VPT, true><<<grid, sh.threads, smem, s>>>(p, sh.tpr);
+        dc::rms::rms_norm_bwd_kernel<VPT, dc::rms::Lay::kAligned><<<grid, sh.threads, smem, s>>>(p, sh.tpr);
     } else {
         if (p.y_dt && p.r_dt) dc::rms::rms_norm_bwd_vec_kernel<bf16, bf16, VPT><<<grid, sh.threads, smem, s>>>(p, sh.tpr);
         else if (p.y_dt) dc::rms::rms_norm_bwd_vec_kernel<bf16, float, VPT><<<grid, sh.threads, smem, s>>>(p, sh.tpr);

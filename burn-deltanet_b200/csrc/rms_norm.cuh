@@ -23,6 +23,45 @@ namespace rms {
 
 constexpr int kVec = 8;  // columns per access
 
+// How an access's eight columns lie in a row: side by side, in aligned or single accesses, or (where rows start anywhere)
+// TPR columns apart, so that a warp's single accesses meet in few lines.
+enum class Lay { kAligned, kSide, kApart };
+
+template <Lay LAY>
+__device__ __forceinline__ int column(int i, int tx, int tpr) { return LAY == Lay::kApart ? i * tpr * kVec + tx : (tx + i * tpr) * kVec; }
+// columns of access i inside a row of `width`
+template <Lay LAY>
+__device__ __forceinline__ int inside(int i, int tx, int tpr, int width) {
+    const int left = width - column<LAY>(i, tx, tpr);
+    const int n = LAY == Lay::kApart ? (left + tpr - 1) / tpr : left;
+    return left <= 0 ? 0 : n > kVec ? kVec : n;
+}
+template <Lay LAY>
+__device__ __forceinline__ void load_cols(int dtype, const void *p, int64_t row, int i, int tx, int tpr, float (&v)[kVec], int n) {
+    const int64_t at = row + column<LAY>(i, tx, tpr);
+    if constexpr (LAY == Lay::kApart) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+            v[e] = e >= n ? 0.f : dtype ? ld(static_cast<const __nv_bfloat16 *>(p) + at + e * tpr) : static_cast<const float *>(p)[at + e * tpr];
+    } else {
+        vec::load_as<LAY == Lay::kAligned>(dtype, p, at, v, n);
+    }
+}
+template <Lay LAY>
+__device__ __forceinline__ void store_cols(int dtype, void *p, int64_t row, int i, int tx, int tpr, const float (&v)[kVec], int n) {
+    const int64_t at = row + column<LAY>(i, tx, tpr);
+    if constexpr (LAY == Lay::kApart) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+            if (e < n) {
+                if (dtype) st(static_cast<__nv_bfloat16 *>(p) + at + e * tpr, v[e]);
+                else static_cast<float *>(p)[at + e * tpr] = v[e];
+            }
+    } else {
+        vec::store_as<LAY == Lay::kAligned>(dtype, p, at, v, n);
+    }
+}
+
 struct Params {
     int64_t rows;
     int32_t width, group;  // group: columns per scale (e4m3), 0 = the whole row
@@ -82,7 +121,7 @@ __device__ __forceinline__ uint2 to_e4m3(const float (&v)[kVec], float inv) {
 
 // From the sum of one row on (s, n[i] columns of each access): its sum of squares, the stores, and y.  Every thread of the
 // CTA calls it, with s = 0 and on = false where it has no row.
-template <int VPT, bool ALIGNED, bool F8>
+template <int VPT, Lay LAY, bool F8>
 __device__ __forceinline__ void norm_row(const Params &p, float (&s)[VPT][kVec], const int (&n)[VPT], const float (&w)[VPT][kVec], int64_t row,
                                          bool on, int tx, int tpr, float2 *red) {
     float ss = 0.f;
@@ -93,7 +132,7 @@ __device__ __forceinline__ void norm_row(const Params &p, float (&s)[VPT][kVec],
     if (p.rout && on) {
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
-            if (n[i] > 0) vec::store_as<ALIGNED>(p.r_dt, p.rout, row * p.rout_stride + (tx + i * tpr) * kVec, s[i], n[i]);
+            if (n[i] > 0) store_cols<LAY>(p.r_dt, p.rout, row * p.rout_stride, i, tx, tpr, s[i], n[i]);
     }
     ss = row_reduce<false>(ss, tpr, red);
     const float inv = 1.f / sqrtf(fmaf(ss, 1.f / (float)p.width, p.eps));
@@ -105,7 +144,7 @@ __device__ __forceinline__ void norm_row(const Params &p, float (&s)[VPT][kVec],
         if (on) {
 #pragma unroll
             for (int i = 0; i < VPT; ++i)
-                if (n[i] > 0) vec::store_as<ALIGNED>(p.y_dt, p.y, row * p.y_stride + (tx + i * tpr) * kVec, s[i], n[i]);
+                if (n[i] > 0) store_cols<LAY>(p.y_dt, p.y, row * p.y_stride, i, tx, tpr, s[i], n[i]);
         }
     } else {
         uint8_t *Y = static_cast<uint8_t *>(p.y);
@@ -115,7 +154,7 @@ __device__ __forceinline__ void norm_row(const Params &p, float (&s)[VPT][kVec],
             amax[i] = 0.f;  // fmaxf drops a NaN: its row is NaN throughout, and keeps scale 1
 #pragma unroll
             for (int e = 0; e < kVec; ++e)
-                if (ALIGNED || e < n[i]) amax[i] = fmaxf(amax[i], fabsf(s[i][e]));
+                if (LAY == Lay::kAligned || e < n[i]) amax[i] = fmaxf(amax[i], fabsf(s[i][e]));
             all = fmaxf(all, amax[i]);
         }
         const int lanes = p.group ? p.group / kVec : 0;  // lanes of a group: 4 .. 32, a power of two
@@ -143,7 +182,7 @@ __device__ __forceinline__ void norm_row(const Params &p, float (&s)[VPT][kVec],
                 }
                 const uint2 q = to_e4m3(s[i], __fdividef(1.f, scale));
                 uint8_t *o = Y + row * p.y_stride + v * kVec;
-                if constexpr (ALIGNED) {
+                if constexpr (LAY == Lay::kAligned) {
                     *reinterpret_cast<uint2 *>(o) = q;
                 } else {
 #pragma unroll
@@ -156,15 +195,14 @@ __device__ __forceinline__ void norm_row(const Params &p, float (&s)[VPT][kVec],
 }
 
 // This thread's part of a row: columns of each access, and the weights.
-template <int VPT, bool ALIGNED>
+template <int VPT, Lay LAY>
 __device__ __forceinline__ void columns(int width, const float *weight, int tx, int tpr, int (&n)[VPT], float (&w)[VPT][kVec]) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-        const int left = width - (tx + i * tpr) * kVec;
-        n[i] = left < 0 ? 0 : left > kVec ? kVec : left;
+        n[i] = inside<LAY>(i, tx, tpr, width);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) w[i][e] = 0.f;
-        if (n[i] > 0) vec::load<ALIGNED>(weight + (tx + i * tpr) * kVec, w[i], n[i]);
+        if (n[i] > 0) load_cols<LAY>(0, weight, 0, i, tx, tpr, w[i], n[i]);
     }
 }
 
@@ -176,7 +214,7 @@ __global__ void __maxnreg__(VPT == 4 ? 128 : 80) rms_norm_vec_kernel(const Param
     const int tx = threadIdx.x & (tpr - 1), ty = threadIdx.x / tpr, rows_per_cta = blockDim.x / tpr;
     int n[VPT];
     float w[VPT][kVec];
-    columns<VPT, true>(p.width, p.weight, tx, tpr, n, w);
+    columns<VPT, Lay::kAligned>(p.width, p.weight, tx, tpr, n, w);
     const TX *X = static_cast<const TX *>(p.x) + tx * kVec;
     const TR *R = p.rin ? static_cast<const TR *>(p.rin) + tx * kVec : nullptr;
     vec::Raw<TX, kVec> x[VPT];
@@ -210,36 +248,35 @@ __global__ void __maxnreg__(VPT == 4 ? 128 : 80) rms_norm_vec_kernel(const Param
                 s[i][e] = v.x, s[i][e + 1] = v.y;
             }
         load(row + stride);
-        norm_row<VPT, true, F8>(p, s, n, w, row, on, tx, tpr, red);
+        norm_row<VPT, Lay::kAligned, F8>(p, s, n, w, row, on, tx, tpr, red);
     }
 }
 
 // Any width, stride and alignment.
-template <int VPT, bool F8>
+template <int VPT, bool F8, Lay LAY>
 __global__ void __launch_bounds__(512) rms_norm_kernel(const Params p, int tpr) {
     __shared__ float2 red[32];
     const int tx = threadIdx.x & (tpr - 1), ty = threadIdx.x / tpr, rows_per_cta = blockDim.x / tpr;
     int n[VPT];
     float w[VPT][kVec];
-    columns<VPT, false>(p.width, p.weight, tx, tpr, n, w);
+    columns<VPT, LAY>(p.width, p.weight, tx, tpr, n, w);
     for (int64_t row0 = (int64_t)blockIdx.x * rows_per_cta; row0 < p.rows; row0 += (int64_t)gridDim.x * rows_per_cta) {
         const int64_t row = row0 + ty;
         const bool on = row < p.rows;
         float s[VPT][kVec];
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const int col = (tx + i * tpr) * kVec;
             float r[kVec];
 #pragma unroll
             for (int e = 0; e < kVec; ++e) s[i][e] = 0.f, r[e] = 0.f;
             if (on && n[i] > 0) {
-                vec::load_as<false>(p.x_dt, p.x, row * p.x_stride + col, s[i], n[i]);
-                if (p.rin) vec::load_as<false>(p.r_dt, p.rin, row * p.rin_stride + col, r, n[i]);
+                load_cols<LAY>(p.x_dt, p.x, row * p.x_stride, i, tx, tpr, s[i], n[i]);
+                if (p.rin) load_cols<LAY>(p.r_dt, p.rin, row * p.rin_stride, i, tx, tpr, r, n[i]);
             }
 #pragma unroll
             for (int e = 0; e < kVec; ++e) s[i][e] += r[e];
         }
-        norm_row<VPT, false, F8>(p, s, n, w, row, on, tx, tpr, red);
+        norm_row<VPT, LAY, F8>(p, s, n, w, row, on, tx, tpr, red);
     }
 }
 
@@ -257,7 +294,7 @@ struct BwdParams {
 
 // From one row's r and dy on: the reductions, d, and the row's part of d_weight.  Every thread of the CTA calls it.
 // dr(i, d) and weight(i, w) give access i's d_r and weights.
-template <int VPT, bool ALIGNED, typename DR, typename W>
+template <int VPT, Lay LAY, typename DR, typename W>
 __device__ __forceinline__ void bwd_row(const BwdParams &p, const float (&r)[VPT][kVec], const float (&g)[VPT][kVec], const int (&n)[VPT],
                                         W &&weight, float (&dw)[VPT][kVec], DR &&dr, int64_t row, bool on, int tx, int tpr, float2 *red) {
     float2 both = make_float2(0.f, 0.f);  // sum of r^2, sum of w dy r
@@ -278,7 +315,6 @@ __device__ __forceinline__ void bwd_row(const BwdParams &p, const float (&r)[VPT
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
         if (!on || n[i] <= 0) continue;
-        const int col = (tx + i * tpr) * kVec;
         float d[kVec], w[kVec];
         dr(i, d);
         weight(i, w);
@@ -287,13 +323,13 @@ __device__ __forceinline__ void bwd_row(const BwdParams &p, const float (&r)[VPT
             dw[i][e] = fmaf(g[i][e], r[i][e] * inv, dw[i][e]);
             d[e] += fmaf(inv * w[e], g[i][e], -r[i][e] * back);
         }
-        if (p.dx) vec::store_as<ALIGNED>(p.x_dt, p.dx, row * p.dx_stride + col, d, n[i]);
-        if (p.dres) vec::store_as<ALIGNED>(p.r_dt, p.dres, row * p.dres_stride + col, d, n[i]);
+        if (p.dx) store_cols<LAY>(p.x_dt, p.dx, row * p.dx_stride, i, tx, tpr, d, n[i]);
+        if (p.dres) store_cols<LAY>(p.r_dt, p.dres, row * p.dres_stride, i, tx, tpr, d, n[i]);
     }
 }
 
 // The CTA's line of d_weight partial sums; rows that share the CTA: row group 0 adds the others' sums in order.
-template <int VPT>
+template <int VPT, Lay LAY>
 __device__ __forceinline__ void bwd_line(const BwdParams &p, const float (&dw)[VPT][kVec], const int (&n)[VPT], int tx, int ty, int tpr,
                                          int rows_per_cta, float *lines) {
     if (!p.part) return;
@@ -303,7 +339,7 @@ __device__ __forceinline__ void bwd_line(const BwdParams &p, const float (&dw)[V
             for (int i = 0; i < VPT; ++i)
 #pragma unroll
                 for (int e = 0; e < kVec; ++e)
-                    if (e < n[i]) lines[(int64_t)(ty - 1) * p.width + (tx + i * tpr) * kVec + e] = dw[i][e];
+                    if (e < n[i]) lines[(int64_t)(ty - 1) * p.width + column<LAY>(i, tx, tpr) + e * (LAY == Lay::kApart ? tpr : 1)] = dw[i][e];
         }
         __syncthreads();
     }
@@ -313,7 +349,7 @@ __device__ __forceinline__ void bwd_line(const BwdParams &p, const float (&dw)[V
 #pragma unroll
             for (int e = 0; e < kVec; ++e)
                 if (e < n[i]) {
-                    const int col = (tx + i * tpr) * kVec + e;
+                    const int col = column<LAY>(i, tx, tpr) + e * (LAY == Lay::kApart ? tpr : 1);
                     float v = dw[i][e];
                     for (int q = 1; q < rows_per_cta; ++q) v += lines[(int64_t)(q - 1) * p.width + col];
                     p.part[(int64_t)blockIdx.x * p.width + col] = v;
@@ -330,7 +366,7 @@ __global__ void __launch_bounds__(512) rms_norm_bwd_vec_kernel(const BwdParams p
     const int tx = threadIdx.x & (tpr - 1), ty = threadIdx.x / tpr, rows_per_cta = blockDim.x / tpr;
     int n[VPT];
     float w[VPT][kVec], dw[VPT][kVec];
-    columns<VPT, true>(p.width, p.weight, tx, tpr, n, w);
+    columns<VPT, Lay::kAligned>(p.width, p.weight, tx, tpr, n, w);
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
@@ -382,13 +418,13 @@ __global__ void __launch_bounds__(512) rms_norm_bwd_vec_kernel(const BwdParams p
 #pragma unroll
             for (int e = 0; e < kVec; ++e) v[e] = w[i][e];
         };
-        bwd_row<VPT, true>(p, r, g, n, weight, dw, dr, row, on, tx, tpr, red);
+        bwd_row<VPT, Lay::kAligned>(p, r, g, n, weight, dw, dr, row, on, tx, tpr, red);
     }
-    bwd_line<VPT>(p, dw, n, tx, ty, tpr, rows_per_cta, lines);
+    bwd_line<VPT, Lay::kAligned>(p, dw, n, tx, ty, tpr, rows_per_cta, lines);
 }
 
-// Any width, stride and alignment; and, ALIGNED, the widths whose rows leave no registers for loads under way and weights.
-template <int VPT, bool ALIGNED>
+// Any width, stride and alignment; and, aligned, the widths whose rows leave no registers for loads under way and weights.
+template <int VPT, Lay LAY>
 __global__ void __launch_bounds__(512) rms_norm_bwd_kernel(const BwdParams p, int tpr) {
     __shared__ float2 red[32];
     extern __shared__ float lines[];
@@ -397,8 +433,7 @@ __global__ void __launch_bounds__(512) rms_norm_bwd_kernel(const BwdParams p, in
     float dw[VPT][kVec];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-        const int left = p.width - (tx + i * tpr) * kVec;
-        n[i] = left < 0 ? 0 : left > kVec ? kVec : left;
+        n[i] = inside<LAY>(i, tx, tpr, p.width);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) dw[i][e] = 0.f;
     }
@@ -411,24 +446,23 @@ __global__ void __launch_bounds__(512) rms_norm_bwd_kernel(const BwdParams p, in
 #pragma unroll
             for (int e = 0; e < kVec; ++e) r[i][e] = 0.f, g[i][e] = 0.f;
             if (on && n[i] > 0) {
-                const int col = (tx + i * tpr) * kVec;
-                vec::load_as<ALIGNED>(p.r_dt, p.r, row * p.r_stride + col, r[i], n[i]);
-                vec::load_as<ALIGNED>(p.y_dt, p.dy, row * p.dy_stride + col, g[i], n[i]);
+                load_cols<LAY>(p.r_dt, p.r, row * p.r_stride, i, tx, tpr, r[i], n[i]);
+                load_cols<LAY>(p.y_dt, p.dy, row * p.dy_stride, i, tx, tpr, g[i], n[i]);
             }
         }
         auto dr = [&](int i, float (&d)[kVec]) {
 #pragma unroll
             for (int e = 0; e < kVec; ++e) d[e] = 0.f;
-            if (p.dr) vec::load_as<ALIGNED>(p.r_dt, p.dr, row * p.dr_stride + (tx + i * tpr) * kVec, d, n[i]);
+            if (p.dr) load_cols<LAY>(p.r_dt, p.dr, row * p.dr_stride, i, tx, tpr, d, n[i]);
         };
         auto weight = [&](int i, float (&v)[kVec]) {
 #pragma unroll
             for (int e = 0; e < kVec; ++e) v[e] = 0.f;
-            if (n[i] > 0) vec::load<ALIGNED>(p.weight + (tx + i * tpr) * kVec, v, n[i]);
+            if (n[i] > 0) load_cols<LAY>(0, p.weight, 0, i, tx, tpr, v, n[i]);
         };
-        bwd_row<VPT, ALIGNED>(p, r, g, n, weight, dw, dr, row, on, tx, tpr, red);
+        bwd_row<VPT, LAY>(p, r, g, n, weight, dw, dr, row, on, tx, tpr, red);
     }
-    bwd_line<VPT>(p, dw, n, tx, ty, tpr, rows_per_cta, lines);
+    bwd_line<VPT, LAY>(p, dw, n, tx, ty, tpr, rows_per_cta, lines);
 }
 
 }  // namespace rms

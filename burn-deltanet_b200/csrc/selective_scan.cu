@@ -94,9 +94,20 @@ struct LaunchStep {
     cudaStream_t s;
     template <int P>
     int operator()() const {
-        const int64_t ctas = ceil_div(p.batch * p.channels, sc::kThreads / P);
-        if (ctas > 0x7fffffff) return DC_EUNSUPPORTED;
-        sc::scan_step_kernel<TI, P><<<(unsigned)ctas, sc::kThreads, 0, s>>>(p);
+        // several sequences per thread where that still leaves two CTAs for every SM
+        const int64_t blocks = ceil_div(p.channels, sc::kThreads / P), seqs = ceil_div(p.batch, sc::kStepSeqs);
+        const bool many = blocks * seqs >= 2 * (int64_t)sm_count();
+        const int64_t rows = many ? seqs : p.batch;
+        if (blocks > 0x7fffffff || rows > 65535) return DC_EUNSUPPORTED;
+        const dim3 grid((unsigned)blocks, (unsigned)rows);
+        // every group of four states whole and aligned
+        const int64_t four = 4 * (int64_t)sizeof(TI);
+        const bool whole = p.N == 4 * P && aligned(p.a, 16) && aligned(p.state_in, 16) && aligned(p.state_out, 16) && aligned(p.b, four) &&
+                           aligned(p.c, four) && (p.batch == 1 || (p.b_b % 4 == 0 && p.c_b % 4 == 0));
+        if (many && whole) sc::scan_step_kernel<TI, P, sc::kStepSeqs, true><<<grid, sc::kThreads, 0, s>>>(p);
+        else if (many) sc::scan_step_kernel<TI, P, sc::kStepSeqs, false><<<grid, sc::kThreads, 0, s>>>(p);
+        else if (whole) sc::scan_step_kernel<TI, P, 1, true><<<grid, sc::kThreads, 0, s>>>(p);
+        else sc::scan_step_kernel<TI, P, 1, false><<<grid, sc::kThreads, 0, s>>>(p);
         return launched();
     }
 };

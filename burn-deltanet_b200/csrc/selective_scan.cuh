@@ -41,7 +41,7 @@ struct Params {
     int32_t N;
     int64_t u_b, u_t, dt_b, dt_t, z_b, z_t, b_b, b_t, c_b, c_t, y_b, y_t;
     int32_t softplus, y_dt;
-    int32_t vec_x, vec_bc;  // strides allow 16-byte copies of the channel rows / of the b and c rows
+    int32_t vec_x, vec_bc;  // how the channel rows / the b and c rows may be copied (kVectors, kWords, kScalar)
     int32_t tiles;          // checkpoints of a sequence
     int32_t pieces;         // pieces of the time axis, `piece` tokens each (a multiple of every tile's)
     int64_t piece;
@@ -145,27 +145,42 @@ __device__ __forceinline__ Place place_of(int64_t block, const Params &p, int wi
     return q;
 }
 
-// `rows` rows of W values (`width` of them real) from src (row stride st) into dst [rows][W], by NT threads of which this is
-// the tid-th; rows from `live` on and missing values are zeros.  Where vec says that rows start on 16-byte boundaries the
-// copies are asynchronous, and what a row lacks of its last copies is filled with zeros.
-template <int NT, int W, typename TI>
-__device__ __forceinline__ void stage(TI *dst, const TI *src, int64_t st, int rows, int live, int width, bool vec, int tid) {
-    constexpr int kEl = 16 / sizeof(TI), kPer = W >= kEl ? W / kEl : 1;
-    if (W % kEl == 0 && vec && aligned16(src)) {
+// How a tensor's rows may be copied, from their strides (and, for the first of these, a 16-byte first row).
+enum : int { kScalar = 0, kWords = 1, kVectors = 2 };  // one by one; asynchronously, 4 bytes or 16 at a time
+
+// ROWS rows of W values (`width` of them real) from src (row stride st) into dst [ROWS][W], by NT threads of which this is
+// the tid-th; rows from `live` on and missing values are zeros.
+template <int NT, int W, int ROWS, typename TI>
+__device__ __forceinline__ void stage(TI *dst, const TI *src, int64_t st, int live, int width, int how, int tid) {
+    constexpr int kEl = 16 / sizeof(TI), kPer = W >= kEl ? W / kEl : 1, kWord = 4 / sizeof(TI);
+    if (W % kEl == 0 && how == kVectors && aligned16(src)) {
 #pragma unroll 1
-        for (int i = tid; i < rows * kPer; i += NT) {
+        for (int i = tid; i < ROWS * kPer; i += NT) {
             const int r = i / kPer, q = i % kPer, left = (width - q * kEl) * (int)sizeof(TI);
             const bool on = r < live && left > 0;
             ptx::cp_async16(ptx::smem_u32(dst + i * kEl), on ? src + r * st + q * kEl : src, !on ? 0u : left > 16 ? 16u : (uint32_t)left);
         }
+    } else if (how >= kWords && (reinterpret_cast<uintptr_t>(src) & 3) == 0) {
+#pragma unroll 4
+        for (int i = tid; i < ROWS * W / kWord; i += NT) {
+            const int r = i / (W / kWord), q = i % (W / kWord), left = (width - q * kWord) * (int)sizeof(TI);
+            const bool on = r < live && left > 0;
+            ptx::cp_async4(ptx::smem_u32(dst + i * kWord), on ? src + r * st + q * kWord : src, !on ? 0u : left > 4 ? 4u : (uint32_t)left);
+        }
     } else {
+        constexpr int kBatch = 8;  // loads under way together
 #pragma unroll 1
-        for (int i = tid; i < rows * W; i += NT) {
-            const int r = i / W, q = i % W;
-            TI v;
-            dc::st(&v, 0.f);
-            if (r < live && q < width) v = src[r * st + q];
-            dst[i] = v;
+        for (int i0 = tid; i0 < ROWS * W; i0 += kBatch * NT) {
+            TI v[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int i = i0 + k * NT, r = i / W, q = i % W;
+                dc::st(&v[k], 0.f);
+                if (r < live && q < width) v[k] = src[r * st + q];
+            }
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k)
+                if (i0 + k * NT < ROWS * W) dst[i0 + k * NT] = v[k];
         }
     }
 }
@@ -203,12 +218,12 @@ struct Work {
     template <int NT, int TOK, bool FULL, typename Raw>
     __device__ __forceinline__ void load(Raw &w, int64_t t0, int tid) const {
         const int live = len - t0 < TOK ? (int)(len - t0) : TOK;
-        stage<NT, CH>(w.dt, D + t0 * p.dt_t, p.dt_t, TOK, live, at.nch, p.vec_x, tid);
-        stage<NT, CH>(w.u, U + t0 * p.u_t, p.u_t, TOK, live, at.nch, p.vec_x, tid);
-        stage<NT, N4>(w.b, B + t0 * p.b_t, p.b_t, TOK, live, p.N, p.vec_bc, tid);
+        stage<NT, CH, TOK>(w.dt, D + t0 * p.dt_t, p.dt_t, live, at.nch, p.vec_x, tid);
+        stage<NT, CH, TOK>(w.u, U + t0 * p.u_t, p.u_t, live, at.nch, p.vec_x, tid);
+        stage<NT, N4, TOK>(w.b, B + t0 * p.b_t, p.b_t, live, p.N, p.vec_bc, tid);
         if (FULL) {
-            stage<NT, N4>(w.c, C + t0 * p.c_t, p.c_t, TOK, live, p.N, p.vec_bc, tid);
-            if (Z) stage<NT, CH>(w.z, Z + t0 * p.z_t, p.z_t, TOK, live, at.nch, p.vec_x, tid);
+            stage<NT, N4, TOK>(w.c, C + t0 * p.c_t, p.c_t, live, p.N, p.vec_bc, tid);
+            if (Z) stage<NT, CH, TOK>(w.z, Z + t0 * p.z_t, p.z_t, live, at.nch, p.vec_x, tid);
         }
     }
 };
@@ -312,7 +327,7 @@ struct Stager {
 
     __device__ __forceinline__ Stager(const Work<TI, CH, N4> &wk, int tid) {
         const Params &p = wk.p;
-        on = p.vec_x && p.vec_bc && N4 % kEl == 0 && (!FULL || wk.Z) && aligned16(wk.U) && aligned16(wk.D) && aligned16(wk.B) &&
+        on = p.vec_x == kVectors && p.vec_bc == kVectors && N4 % kEl == 0 && (!FULL || wk.Z) && aligned16(wk.U) && aligned16(wk.D) && aligned16(wk.B) &&
              (!FULL || (aligned16(wk.Z) && aligned16(wk.C)));
         if (!on) return;
 #pragma unroll
@@ -596,39 +611,82 @@ __global__ void __launch_bounds__(SegShape<P>::kNT, 512 / SegShape<P>::kNT) scan
 }
 
 // ------------------------------------------------------------------------------------------------ one token
-// Four states per thread; HBM-bound (the state read and written once, 8 bytes per state, against 4 elements per channel).
-template <typename TI, int P>
+// four values n .. n + 3 of a row of N of type T (values past N are 0); WHOLE: all four there and aligned
+template <bool WHOLE, typename T>
+__device__ __forceinline__ F4 load4_as(const T *row, int n, int N) {
+    float v[4];
+    if (WHOLE) vec::load<true>(row + n, v);
+    else vec::load<false>(row + n, v, N - n);
+    return f4(make_float4(v[0], v[1], v[2], v[3]));
+}
+
+// Four states of one channel per thread, for SEQS sequences, whose states are all under way together; HBM-bound (the state
+// read and written once, 8 bytes per state, against 4 elements per channel).  A channel's P threads share out what is per
+// sequence: the step, the gate and the output.  256 x 2048 x 16 in place: 15 us (4.8 TB/s), 19 with four sequences, whose
+// registers halve the threads on an SM, and 26 with one and nothing shared.
+constexpr int kStepSeqs = 2;
+template <typename TI, int P, int SEQS, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) scan_step_kernel(const Params p) {
-    const int64_t i = (int64_t)blockIdx.x * (kThreads / P) + threadIdx.x / P;  // (sequence, channel)
+    constexpr int kOwn = P < SEQS ? SEQS / P : 1;  // sequences that a thread sees to: q, q + P, .. (modulo SEQS)
+    // (the channels fit 32 bits, and so do the strides' products with a sequence's number where they stay 64 bits wide)
+    const uint32_t at = blockIdx.x * (kThreads / P) + threadIdx.x / P, channels = (uint32_t)p.channels, d = at < channels ? at : channels - 1;
+    const uint32_t e = p.groups == 1 ? 0 : d / (uint32_t)p.per;
     const int q = threadIdx.x % P, N = p.N;
-    const bool on = i < p.batch * p.channels;
-    const int64_t j = on ? i : 0, b = j / p.channels, d = j - b * p.channels, e = d / p.per;
-    const F4 h0 = p.state_in ? load4(p.state_in + j * N, kS * q, N) : zero4();
-    const F4 a2 = mul(kLog2e, load4(p.a + d * N, kS * q, N));
-    const float u = ld(static_cast<const TI *>(p.u) + b * p.u_b + d);
-    float step = ld(static_cast<const TI *>(p.dt) + b * p.dt_b + d) + (p.dt_bias ? p.dt_bias[d] : 0.f);
-    if (p.softplus) step = softplus(step);
-    const TI *B = static_cast<const TI *>(p.b) + b * p.b_b + e * N, *C = static_cast<const TI *>(p.c) + b * p.c_b + e * N;
-    float bv[kS], cv[kS];
+    const int64_t b0 = (int64_t)blockIdx.y * SEQS;
+    const int left = p.batch - b0 < SEQS ? (int)(p.batch - b0) : SEQS;  // sequences that exist; the last one stands in for the others
+    const int64_t row0 = (b0 * channels + d) * N, row = (int64_t)channels * N;
+    const TI *B = static_cast<const TI *>(p.b) + b0 * p.b_b + e * (uint32_t)N, *C = static_cast<const TI *>(p.c) + b0 * p.c_b + e * (uint32_t)N;
+    F4 h[SEQS], bv[SEQS], cv[SEQS];
 #pragma unroll
-    for (int k = 0; k < kS; ++k) {
-        bv[k] = kS * q + k < N ? ld(B + kS * q + k) : 0.f;
-        cv[k] = kS * q + k < N ? ld(C + kS * q + k) : 0.f;
+    for (int k = 0; k < SEQS; ++k) {
+        const int b = k < left ? k : left - 1;
+        h[k] = p.state_in ? load4_as<WHOLE>(p.state_in + row0 + b * row, kS * q, N) : zero4();
+        bv[k] = load4_as<WHOLE>(B + b * p.b_b, kS * q, N);
+        cv[k] = load4_as<WHOLE>(C + b * p.c_b, kS * q, N);
     }
-    const F4 h = fma(ex2(mul(step, a2)), h0, mul(step * u, f4(make_float4(bv[0], bv[1], bv[2], bv[3]))));
-    float y = dot(h, f4(make_float4(cv[0], cv[1], cv[2], cv[3])));
+    float u[kOwn], step[kOwn], z[kOwn];
 #pragma unroll
-    for (int o = P / 2; o >= 1; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (!on) return;
-    if (p.state_out) store4(p.state_out + j * N, kS * q, N, h);
-    if (q == 0) {
-        if (p.d) y = fmaf(p.d[d], u, y);
-        if (p.z) {
-            const float z = ld(static_cast<const TI *>(p.z) + b * p.z_b + d);
-            y *= z * sigmoid(z);
+    for (int j = 0; j < kOwn; ++j) {
+        const int k = (q + j * P) % SEQS;
+        const int64_t b = b0 + (k < left ? k : left - 1);
+        u[j] = ld(static_cast<const TI *>(p.u) + b * p.u_b + d);
+        step[j] = ld(static_cast<const TI *>(p.dt) + b * p.dt_b + d);
+        z[j] = p.z ? ld(static_cast<const TI *>(p.z) + b * p.z_b + d) : 0.f;
+    }
+    const F4 a2 = mul(kLog2e, load4_as<WHOLE>(p.a + (int64_t)d * N, kS * q, N));
+    const float bias = p.dt_bias ? p.dt_bias[d] : 0.f, skip = p.d ? p.d[d] : 0.f;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+        step[j] += bias;
+        if (p.softplus) step[j] = softplus(step[j]);
+    }
+    float y[SEQS];
+#pragma unroll
+    for (int k = 0; k < SEQS; ++k) {
+        const float s = __shfl_sync(0xffffffffu, step[k / P % kOwn], k % P, P), su = __shfl_sync(0xffffffffu, step[k / P % kOwn] * u[k / P % kOwn], k % P, P);
+        h[k] = fma(ex2(mul(s, a2)), h[k], mul(su, bv[k]));
+        y[k] = dot(h[k], cv[k]);
+#pragma unroll
+        for (int o = P / 2; o >= 1; o >>= 1) y[k] += __shfl_xor_sync(0xffffffffu, y[k], o);
+        if (p.state_out && at < channels && k < left) {
+            float *o = p.state_out + row0 + k * row;
+            if (WHOLE) *reinterpret_cast<float4 *>(o + kS * q) = f4(h[k]);
+            else store4(o, kS * q, N, h[k]);
         }
-        if (p.y_dt) st(static_cast<__nv_bfloat16 *>(p.y) + b * p.y_b + d, y);
-        else st(static_cast<float *>(p.y) + b * p.y_b + d, y);
+    }
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+        const int k = (q + j * P) % SEQS;
+        float v = y[0];
+#pragma unroll
+        for (int x = 1; x < SEQS; ++x) v = x == k ? y[x] : v;
+        v = fmaf(skip, u[j], v);
+        if (p.z) v *= z[j] * sigmoid(z[j]);
+        if (at < channels && k < left && q < SEQS) {
+            const int64_t o = (b0 + k) * p.y_b + d;
+            if (p.y_dt) st(static_cast<__nv_bfloat16 *>(p.y) + o, v);
+            else st(static_cast<float *>(p.y) + o, v);
+        }
     }
 }
 

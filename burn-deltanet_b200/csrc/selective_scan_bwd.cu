@@ -111,7 +111,8 @@ int dc_selective_scan_bwd(const dc_selective_scan_bwd_args *a, dc_stream_t strea
     sc::BwdParams p{};
     p.f = sc::params_of(&a->fwd);
     p.dy_b = a->d_y_batch_stride, p.dy_t = a->d_y_token_stride;
-    p.f.vec_x = p.f.vec_x && (p.dy_t * (int64_t)dtype_size(a->fwd.out_dtype)) % 16 == 0;
+    const int64_t dy_bytes = p.dy_t * (int64_t)dtype_size(a->fwd.out_dtype);
+    if (dy_bytes % 16) p.f.vec_x = dy_bytes % 4 ? sc::kScalar : p.f.vec_x < sc::kWords ? p.f.vec_x : sc::kWords;
     p.dy = a->d_y, p.dstate_out = a->d_state_out;
     p.du = a->d_u, p.ddt = a->d_dt, p.dz = a->fwd.z ? a->d_z : nullptr, p.dstate_in = a->d_state_in;
     char *ws = static_cast<char *>(a->workspace);

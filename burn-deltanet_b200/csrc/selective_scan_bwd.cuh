@@ -92,7 +92,7 @@ struct BwdStager {
             int base;  // in copies
         } in[6] = {{p.u, p.u_b, p.u_t, at.d0, 0},          {p.dt, p.dt_b, p.dt_t, at.d0, kX},        {p.z, p.z_b, p.z_t, at.d0, 2 * kX},
                    {p.b, p.b_b, p.b_t, at.e * p.N, 3 * kX}, {p.c, p.c_b, p.c_t, at.e * p.N, 3 * kX + kB}, {bp.dy, bp.dy_b, bp.dy_t, at.d0, 3 * kX + 2 * kB}};
-        on = p.vec_x && p.vec_bc && S::kN % kEl == 0 && p.z && (p.y_dt ? 2 : 4) == kEs;
+        on = p.vec_x == kVectors && p.vec_bc == kVectors && S::kN % kEl == 0 && p.z && (p.y_dt ? 2 : 4) == kEs;
 #pragma unroll
         for (int k = 0; k < 6; ++k) on = on && aligned16(static_cast<const TI *>(in[k].at) + at.b * in[k].batch + in[k].first);
         if (!on) return;
@@ -157,16 +157,16 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
                 if (stager.on) {
                     stager.copy(w, live);
                 } else {
-                    stage<S::kHelp, CH>(w.dt, D + t0 * p.dt_t, p.dt_t, kTile, live, at.nch, p.vec_x, tid);
-                    stage<S::kHelp, CH>(w.u, U + t0 * p.u_t, p.u_t, kTile, live, at.nch, p.vec_x, tid);
-                    if (Z) stage<S::kHelp, CH>(w.z, Z + t0 * p.z_t, p.z_t, kTile, live, at.nch, p.vec_x, tid);
+                    stage<S::kHelp, CH, kTile>(w.dt, D + t0 * p.dt_t, p.dt_t, live, at.nch, p.vec_x, tid);
+                    stage<S::kHelp, CH, kTile>(w.u, U + t0 * p.u_t, p.u_t, live, at.nch, p.vec_x, tid);
+                    if (Z) stage<S::kHelp, CH, kTile>(w.z, Z + t0 * p.z_t, p.z_t, live, at.nch, p.vec_x, tid);
                     if (p.y_dt)
-                        stage<S::kHelp, CH>(reinterpret_cast<__nv_bfloat16 *>(w.dy), static_cast<const __nv_bfloat16 *>(bp.dy) + dy0 + t0 * bp.dy_t,
-                                            bp.dy_t, kTile, live, at.nch, p.vec_x, tid);
+                        stage<S::kHelp, CH, kTile>(reinterpret_cast<__nv_bfloat16 *>(w.dy), static_cast<const __nv_bfloat16 *>(bp.dy) + dy0 + t0 * bp.dy_t,
+                                            bp.dy_t, live, at.nch, p.vec_x, tid);
                     else
-                        stage<S::kHelp, CH>(w.dy, static_cast<const float *>(bp.dy) + dy0 + t0 * bp.dy_t, bp.dy_t, kTile, live, at.nch, p.vec_x, tid);
-                    stage<S::kHelp, S::kN>(w.b, B + t0 * p.b_t, p.b_t, kTile, live, N, p.vec_bc, tid);
-                    stage<S::kHelp, S::kN>(w.c, C + t0 * p.c_t, p.c_t, kTile, live, N, p.vec_bc, tid);
+                        stage<S::kHelp, CH, kTile>(w.dy, static_cast<const float *>(bp.dy) + dy0 + t0 * bp.dy_t, bp.dy_t, live, at.nch, p.vec_x, tid);
+                    stage<S::kHelp, S::kN, kTile>(w.b, B + t0 * p.b_t, p.b_t, live, N, p.vec_bc, tid);
+                    stage<S::kHelp, S::kN, kTile>(w.c, C + t0 * p.c_t, p.c_t, live, N, p.vec_bc, tid);
                 }
             }
             ptx::cp_async_commit();

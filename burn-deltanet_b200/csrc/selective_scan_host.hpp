@@ -55,8 +55,10 @@ inline Params params_of(const dc_selective_scan_args *a) {
     p.softplus = (a->flags & DC_SCAN_SOFTPLUS) ? 1 : 0;
     p.y_dt = a->out_dtype;
     const int64_t is = host::dtype_size(a->in_dtype);
-    p.vec_x = (p.u_t * is) % 16 == 0 && (p.dt_t * is) % 16 == 0 && (!a->z || (p.z_t * is) % 16 == 0);
-    p.vec_bc = (p.b_t * is) % 16 == 0 && (p.c_t * is) % 16 == 0;
+    auto how = [](int64_t bytes) { return bytes % 16 == 0 ? kVectors : bytes % 4 == 0 ? kWords : kScalar; };
+    auto least = [](int a, int b) { return a < b ? a : b; };
+    p.vec_x = least(least(how(p.u_t * is), how(p.dt_t * is)), a->z ? how(p.z_t * is) : kVectors);
+    p.vec_bc = least(how(p.b_t * is), how(p.c_t * is));
     p.tiles = (int32_t)host::ceil_div(a->seq, kTile);
     p.u = a->u, p.dt = a->dt, p.z = a->z, p.b = a->b, p.c = a->c;
     p.a = a->a, p.d = a->d, p.dt_bias = a->dt_bias, p.state_in = a->state_in, p.lengths = a->lengths;
