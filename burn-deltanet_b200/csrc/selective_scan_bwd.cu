@@ -8,18 +8,37 @@ using namespace dc::host;
 namespace sc = dc::scan;
 
 struct Layout {
-    int64_t blocks;  // CTAs of a group
-    uint64_t bc, a, d, bytes;
+    int64_t blocks;  // CTAs of a group, for one piece
+    int64_t pieces, piece;
+    uint64_t bc, a, d, out, step, bytes;
 };
 
+// Pieces of the time axis: as many as the card has room for, 256 tokens each at least (1 x 4096 x 1024 x 16, forward and
+// backward: 233 us with nine of them, 773 us in one).
 Layout layout_of(const dc_selective_scan_args *f) {
+    constexpr int64_t kLeast = 256;
+    const int lanes = sc::lanes_of(f->state);
     Layout l;
-    const uint64_t al = 255;
-    l.blocks = ceil_div(f->channels / f->groups, sc::bwd_channels(sc::lanes_of(f->state)));
-    l.bc = 0;
-    l.a = ((uint64_t)f->batch * f->groups * l.blocks * f->seq * 2 * f->state * 4 + al) & ~al;
-    l.d = l.a + (((uint64_t)f->batch * f->channels * f->state * 4 + al) & ~al);
-    l.bytes = l.d + (uint64_t)f->batch * 2 * f->channels * 4;
+    l.blocks = ceil_div(f->channels / f->groups, sc::bwd_channels(lanes));
+    const int64_t ctas = f->batch * f->groups * l.blocks, room = (int64_t)sm_count() * sc::bwd_ctas(lanes);
+    const int64_t want = room / ctas, most = f->seq / kLeast, pieces = want < most ? want : most;
+    l.pieces = 1, l.piece = f->seq;
+    if (pieces > 1) {
+        l.piece = ceil_div(ceil_div(f->seq, pieces), sc::kTile) * sc::kTile;
+        l.pieces = ceil_div(f->seq, l.piece);
+    }
+    uint64_t at = 0;
+    auto take = [&](int64_t floats) {
+        const uint64_t from = at;
+        at += ((uint64_t)floats * 4 + 255) & ~(uint64_t)255;
+        return from;
+    };
+    l.bc = take(f->batch * f->groups * l.blocks * f->seq * 2 * f->state);
+    l.a = take(f->batch * l.pieces * f->channels * f->state);
+    l.d = take(f->batch * l.pieces * 2 * f->channels);
+    l.out = take(f->batch * (l.pieces - 1) * f->channels * f->state);
+    l.step = take(f->batch * (l.pieces - 1) * f->channels);
+    l.bytes = at;
     return l;
 }
 
@@ -51,16 +70,22 @@ int validate(const dc_selective_scan_bwd_args *a) {
 template <typename TI>
 struct Launch {
     const sc::BwdParams &p;
-    unsigned ctas;
+    int64_t ctas;  // of one piece
     cudaStream_t s;
-    template <int P>
-    int operator()() const {
+    template <int P, bool FULL>
+    int go(int64_t n) const {
         constexpr size_t smem = sizeof(sc::BwdSmem<TI, P>);
         static_assert(smem <= 227 * 1024, "shared memory of a CTA");
-        const int st = sc::allow_smem(&sc::scan_bwd_kernel<TI, P>, smem);
+        if (n > 0x7fffffff) return DC_EUNSUPPORTED;
+        const int st = sc::allow_smem(&sc::scan_bwd_kernel<TI, P, FULL>, smem);
         if (st != DC_OK) return st;
-        sc::scan_bwd_kernel<TI, P><<<ctas, sc::BwdShape<P>::kNT, smem, s>>>(p);
+        sc::scan_bwd_kernel<TI, P, FULL><<<(unsigned)n, sc::BwdShape<P>::kNT, smem, s>>>(p);
         return launched();
+    }
+    template <int P>
+    int operator()() const {
+        const int st = p.f.pieces > 1 ? go<P, false>(ctas * (p.f.pieces - 1)) : DC_OK;
+        return st == DC_OK ? go<P, true>(ctas * p.f.pieces) : st;
     }
 };
 
@@ -70,8 +95,8 @@ int run(const dc_selective_scan_bwd_args *a, const sc::BwdParams &p, int64_t blo
     if (f->batch > 0) {
         const int64_t ctas = f->batch * f->groups * blocks;
         const int64_t bc = ceil_div(f->batch * f->groups * f->seq * 2 * f->state, 256);
-        if (ctas > 0x7fffffff || bc > 0x7fffffff) return DC_EUNSUPPORTED;
-        int st = sc::for_lanes(f->state, Launch<TI>{p, (unsigned)ctas, s});
+        if (bc > 0x7fffffff) return DC_EUNSUPPORTED;
+        int st = sc::for_lanes(f->state, Launch<TI>{p, ctas, s});
         if (st != DC_OK) return st;
         if (bc > 0) {
             sc::scan_bwd_bc_kernel<TI><<<(unsigned)bc, 256, 0, s>>>(p.bc_part, f->batch, f->seq, f->groups, blocks, (int)f->state, f->lengths,
@@ -81,7 +106,7 @@ int run(const dc_selective_scan_bwd_args *a, const sc::BwdParams &p, int64_t blo
         }
     }
     const int64_t n = f->channels * (f->state + 2);
-    sc::scan_bwd_batch_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(p.a_part, p.d_part, f->batch, f->channels, (int)f->state, a->d_a, a->d_d,
+    sc::scan_bwd_batch_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(p.a_part, p.d_part, f->batch * p.f.pieces, f->channels, (int)f->state, a->d_a, a->d_d,
                                                                         a->d_dt_bias);
     return launched();
 }
@@ -101,8 +126,10 @@ int dc_selective_scan_bwd(const dc_selective_scan_bwd_args *a, dc_stream_t strea
     if (st == DC_OK) st = validate(a);
     if (st != DC_OK) return st;
     if (a->fwd.channels == 0) return DC_OK;
-    const Layout l = layout_of(&a->fwd);
+    Layout l{};
+    l.pieces = 1;
     if (a->fwd.batch > 0) {
+        l = layout_of(&a->fwd);
         if (a->workspace_bytes < l.bytes) return DC_EWORKSPACE;
         if (!a->workspace || !aligned(a->workspace, 16)) return DC_EINVAL_ARG;
     }
@@ -117,6 +144,8 @@ int dc_selective_scan_bwd(const dc_selective_scan_bwd_args *a, dc_stream_t strea
     p.du = a->d_u, p.ddt = a->d_dt, p.dz = a->fwd.z ? a->d_z : nullptr, p.dstate_in = a->d_state_in;
     char *ws = static_cast<char *>(a->workspace);
     p.bc_part = reinterpret_cast<float *>(ws + l.bc), p.a_part = reinterpret_cast<float *>(ws + l.a), p.d_part = reinterpret_cast<float *>(ws + l.d);
+    p.piece_out = reinterpret_cast<float *>(ws + l.out), p.piece_step = reinterpret_cast<float *>(ws + l.step);
+    p.f.pieces = (int32_t)l.pieces, p.f.piece = l.piece;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     return a->fwd.in_dtype == DC_BF16 ? run<__nv_bfloat16>(a, p, l.blocks, s) : run<float>(a, p, l.blocks, s);
 }

@@ -14,6 +14,10 @@
 // per token and state; the other way, segments of threads that run their tokens from zero and exchange, takes one but twice
 // the shared memory traffic (measured at 4 x 2048 x 2048 x 16: 690 us, with that traffic at 67 % of its peak).
 //
+// With few channels the time axis is cut into pieces, as in the forward: a first launch walks back through each piece but
+// the first from zero, for the gradient that leaves it and its sum of steps, and the second starts each piece from what the
+// pieces after it give.
+//
 // d_b and d_c sum over channels, which lie across lanes (a thread's two channels add up on the way): every four tokens a
 // warp turns its sums over in shared memory, so that each lane adds the eight pairs of channels of one token and four
 // states; the warps of a CTA meet in a line per token, and a second kernel adds the CTAs' lines in order.
@@ -32,11 +36,15 @@ struct BwdParams {
     void *du, *ddt, *dz;  // [batch, seq, channels]
     float *dstate_in;
     float *bc_part;  // [batch, groups, CTAs of a group, seq, 2, N]
-    float *a_part;   // [batch, channels, N]
-    float *d_part;   // [batch, 2, channels]: d_d, d_dt_bias
+    float *a_part;   // [batch, pieces, channels, N]
+    float *d_part;   // [batch, pieces, 2, channels]: d_d, d_dt_bias
+    // with pieces (f.pieces, f.piece; the first has none): the gradients that leave them from zero, their sums of steps
+    float *piece_out;   // [batch, pieces - 1, channels, N]
+    float *piece_step;  // [batch, pieces - 1, channels]
 };
 
 constexpr int bwd_channels(int lanes) { return lanes <= 2 ? 64 / lanes : lanes == 16 ? 16 : 32; }  // of a CTA
+constexpr int bwd_ctas(int lanes) { return lanes == 2 || lanes == 4 ? 2 : 1; }  // of an SM, by their registers and shared memory
 
 template <int P>
 struct BwdShape {
@@ -127,17 +135,22 @@ struct BwdStager {
     }
 };
 
-template <typename TI, int P>
-__global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_kernel(const BwdParams bp) {
+// FULL: the whole backward; else only the gradient that leaves the piece, and its sum of steps.
+template <typename TI, int P, bool FULL>
+__global__ void __launch_bounds__(BwdShape<P>::kNT, bwd_ctas(P)) scan_bwd_kernel(const BwdParams bp) {
     using S = BwdShape<P>;
     constexpr int CH = S::kCh, kT = S::kT;
     const Params &p = bp.f;
     extern __shared__ __align__(16) unsigned char smem_bytes[];
     BwdSmem<TI, P> &sm = *reinterpret_cast<BwdSmem<TI, P> *>(smem_bytes);
-    const Place at = place_of(blockIdx.x, p, CH);
+    const int64_t pieces = FULL ? p.pieces : p.pieces - 1;
+    const int64_t piece = (pieces > 1 ? blockIdx.x % pieces : 0) + (FULL ? 0 : 1);
+    const Place at = place_of(pieces > 1 ? blockIdx.x / pieces : blockIdx.x, p, CH);
     const int N = p.N;
-    const int64_t len = length_of(p.lengths, at.b, p.seq);
-    const int n = (int)((len + kTile - 1) / kTile);  // tiles; number i from the back
+    const int64_t first = p.pieces > 1 ? piece * p.piece : 0, last = p.pieces > 1 && first + p.piece < p.seq ? first + p.piece : p.seq;
+    const int64_t all = length_of(p.lengths, at.b, p.seq), len = all < last ? all : last;  // this CTA's tokens: first .. len
+    const int n = len > first ? (int)((len - first + kTile - 1) / kTile) : 0;              // tiles; number i from the back
+    const int64_t tile_end = first / kTile + n;
 
     if (threadIdx.x >= S::kMain) {
         // ---------------------------------------------------------------- staging, steps, outputs
@@ -148,10 +161,10 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
         const int64_t dy0 = at.b * bp.dy_b + at.d0;
         const int64_t blocks = (p.per + CH - 1) / CH, blk = (at.d0 - at.e * p.per) / CH;
         float *part = bp.bc_part + ((at.b * p.groups + at.e) * blocks + blk) * p.seq * 2 * N;
-        BwdStager<TI, P> stager(bp, at, (int64_t)(n > 0 ? n - 1 : 0) * kTile, tid);
+        BwdStager<TI, P> stager(bp, at, (n > 0 ? tile_end - 1 : 0) * kTile, tid);
         auto load = [&](int i) {
             if (i < n) {
-                const int64_t t0 = (int64_t)(n - 1 - i) * kTile;
+                const int64_t t0 = (tile_end - 1 - i) * kTile;
                 const int live = len - t0 < kTile ? (int)(len - t0) : kTile;
                 auto &w = sm.raw[i & 1];
                 if (stager.on) {
@@ -177,7 +190,7 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
         };
         Kept cur{}, nxt{};
         auto prepare = [&](int i, Kept &k) {
-            const bool on = (int64_t)(n - 1 - i) * kTile + t < len;
+            const bool on = (tile_end - 1 - i) * kTile + t < len;
             const auto &w = sm.raw[i & 1];
             float v[4], z[4], gy[4];
             vec::load<true>(w.u + t * CH + oc, k.u);
@@ -221,7 +234,7 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
         float sd[4] = {}, sb[4] = {};  // sums over this thread's tokens: d_d, d_dt_bias
         auto finish = [&](int i, const Kept &k) {  // the gradients of tile i, from the recurrence's shares
             const auto &sh = sm.share[i & 1];
-            const int64_t t0 = (int64_t)(n - 1 - i) * kTile, token = t0 + t;
+            const int64_t t0 = (tile_end - 1 - i) * kTile, token = t0 + t;
             float y[4] = {}, gb[4] = {}, aw[4] = {};
 #pragma unroll
             for (int j = 0; j < S::kShares; ++j) {  // from another share on in each token, as in the forward
@@ -275,7 +288,7 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
         auto fetch = [&](int i) {  // the checkpoints of tile i
 #pragma unroll
             for (int x = 0; x < kWalks; ++x)
-                wh[x] = wch[x] < at.nch ? load4(p.ckpt + ((at.b * p.tiles + n - 1 - i) * p.channels + at.d0 + wch[x]) * N, kS * wq[x], N) : zero4();
+                wh[x] = wch[x] < at.nch ? load4(p.ckpt + ((at.b * p.tiles + tile_end - 1 - i) * p.channels + at.d0 + wch[x]) * N, kS * wq[x], N) : zero4();
         };
         auto walk = [&](int i) {
 #pragma unroll
@@ -308,13 +321,13 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
         }
         load(0);
         auto ahead = [&](int i) {  // make tile i ready
-            fetch(i);
+            if (FULL) fetch(i);
             ptx::cp_async_wait<0>();
             ptx::named_sync(1, S::kHelp);  // every helper's copies of it have landed
             load(i + 1);                   // into the other stage, which everyone has read
             prepare(i, nxt);
             ptx::named_sync(1, S::kHelp);
-            walk(i);
+            if (FULL) walk(i);
         };
         if (n > 0) ahead(0);
         __syncthreads();  // the first tile is ready
@@ -322,9 +335,10 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
         for (int i = 0; i < n; ++i) {
             old = cur, cur = nxt;
             if (i + 1 < n) ahead(i + 1);
-            if (i > 0) finish(i - 1, old);
+            if (FULL && i > 0) finish(i - 1, old);
             __syncthreads();  // tile i is done, i + 1 is ready
         }
+        if (!FULL) return;
         if (n > 0) finish(n - 1, cur);
         // the sums over tokens: sixteen threads' in order, through the shares' memory
         ptx::named_sync(1, S::kHelp);
@@ -334,12 +348,12 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
         if (tid < at.nch) {
             float d = 0.f, b = 0.f;
             for (int k = 0; k < kTile; ++k) d += sm.share[0].y[k * CH + tid], b += sm.share[0].gb[k * CH + tid];
-            float *o = bp.d_part + at.b * 2 * p.channels + at.d0 + tid;
+            float *o = bp.d_part + (at.b * p.pieces + piece) * 2 * p.channels + at.d0 + tid;
             o[0] = d;
             o[p.channels] = b;
         }
         const float none[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int64_t token = len + t; token < p.seq; token += kTile) {
+        for (int64_t token = (len > first ? len : first) + t; token < last; token += kTile) {
             put(bp.du, token, none);
             put(bp.ddt, token, none);
             if (bp.dz) put(bp.dz, token, none);
@@ -357,8 +371,41 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
         real[j] = ch + j < at.nch;
         const int64_t d = at.d0 + ch + j;
         a2[j] = real[j] ? mul(kLog2e, load4(p.a + d * N, kS * q, N)) : zero4();
-        g[j] = real[j] && bp.dstate_out ? load4(bp.dstate_out + (at.b * p.channels + d) * N, kS * q, N) : zero4();
+        g[j] = FULL && real[j] && bp.dstate_out ? load4(bp.dstate_out + (at.b * p.channels + d) * N, kS * q, N) : zero4();
         da[j] = zero4();
+        if (FULL && real[j])
+#pragma unroll 4
+            for (int64_t k = p.pieces - 1; k > piece; --k) {  // what the pieces after this one make of it
+                const int64_t row = (at.b * (p.pieces - 1) + k - 1) * p.channels + d;
+                g[j] = fma(ex2(mul(bp.piece_step[row], a2[j])), g[j], load4(bp.piece_out + row * N, kS * q, N));
+            }
+    }
+    if constexpr (!FULL) {
+        float steps[2] = {0.f, 0.f};
+        __syncthreads();  // the first tile is ready
+        for (int i = 0; i < n; ++i) {
+            const float2 *step = sm.step[i & 1] + ch;
+            const float *rr = sm.r[i & 1] + ch;
+            const float4 *cs = sm.c[i & 1] + q;
+#pragma unroll 4
+            for (int t = kTile - 1; t >= 0; --t) {
+                const float4 sd = *reinterpret_cast<const float4 *>(step + t * CH);
+                const float2 rv = *reinterpret_cast<const float2 *>(rr + t * CH);
+                const F4 c = f4(cs[t * P]);
+                g[0] = mul(ex2(mul(sd.x, a2[0])), fma(rv.x, c, g[0]));
+                g[1] = mul(ex2(mul(sd.z, a2[1])), fma(rv.y, c, g[1]));
+                steps[0] += sd.x, steps[1] += sd.z;
+            }
+            __syncthreads();  // tile i is done, i + 1 is ready
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if (!real[j]) continue;
+            const int64_t row = (at.b * (p.pieces - 1) + piece - 1) * p.channels + at.d0 + ch + j;
+            store4(bp.piece_out + row * N, kS * q, N, g[j]);
+            if (q == 0) bp.piece_step[row] = steps[j];
+        }
+        return;
     }
     // this lane's part in turning sums over: token, which of d_b (0) and d_c (1), state group of the warp, first pair
     constexpr int kGroups = 32 / S::kPairs, kPer = S::kPairs / 8;  // state groups of a warp, lanes that share a sum
@@ -430,9 +477,9 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, P == 4 ? 2 : 1) scan_bwd_ker
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         if (!real[j]) continue;
-        const int64_t row = (at.b * p.channels + at.d0 + ch + j) * N;
-        store4(bp.a_part + row, kS * q, N, da[j]);
-        if (bp.dstate_in) store4(bp.dstate_in + row, kS * q, N, g[j]);
+        const int64_t d = at.d0 + ch + j;
+        store4(bp.a_part + ((at.b * p.pieces + piece) * p.channels + d) * N, kS * q, N, da[j]);
+        if (bp.dstate_in && piece == 0) store4(bp.dstate_in + (at.b * p.channels + d) * N, kS * q, N, g[j]);
     }
 }
 

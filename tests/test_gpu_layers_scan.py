@@ -125,6 +125,40 @@ def test_lengths_and_what_is_behind_them(n, dtype):
     assert torch.equal(y, y2) and torch.equal(h, h2)
 
 
+@pytest.mark.parametrize("n", [4, 8, 16, 24, 64])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_long_sequences_of_few_channels(n, dtype):
+    """Sequences long enough for the time axis to be cut into pieces, whole and with lengths that end inside each of them, the
+    state in place; in one piece where there is no workspace."""
+    check(inputs(1, 1000, 24, n, dtype=dtype, seed=n))
+    t = inputs(5, 700, 20, n, dtype=dtype, seed=n + 1)
+    lens = [0, 1, 130, 699, 700]
+    want = check(t, lens)
+    args = [t[k].clone() if k == "state" else t[k] for k in NAMES]
+    y, h = dn.selective_scan(*args, lengths=int32(lens), state_out=args[-1])
+    assert torch.equal(y, want[0]) and torch.equal(h, want[1]) and h.data_ptr() == args[-1].data_ptr()
+
+
+def test_without_a_workspace():
+    """The C entry point with workspace NULL walks the sequence in one piece."""
+    abi = importlib.import_module("burn-deltanet_b200._abi")
+    layers = importlib.import_module("burn-deltanet_b200.layers")
+    t = inputs(1, 600, 24, 16, seed=7)
+    want = dn.selective_scan(*(t[k] for k in NAMES))
+    g = layers._scan_dims(*(t[k] for k in NAMES), True, None)
+    assert abi.lib().dc_selective_scan_workspace_size(g) > 0
+    layers._scan_inputs(g, *(t[k] for k in NAMES), None)
+    y, h = torch.empty_like(t["u"]), torch.empty_like(t["state"])
+    g.y, g.state_out, g.y_batch_stride, g.y_token_stride = y.data_ptr(), h.data_ptr(), 600 * 24, 24
+    assert abi.lib().dc_selective_scan(g, torch.cuda.current_stream().cuda_stream) == 0
+    sy, sh = ol.selective_scan(**magnitudes(clean(t, None)))
+    close("y", y, f64(want[0]), np.abs(sy), 2 * (3e-7 * 600 + 4e-6))
+    close("state", h, f64(want[1]), np.abs(sh), 2 * (3e-7 * 600 + 4e-6))
+    workspace = torch.empty(64, dtype=torch.uint8, device="cuda")
+    g.workspace, g.workspace_bytes = workspace.data_ptr(), 64
+    assert abi.lib().dc_selective_scan(g, torch.cuda.current_stream().cuda_stream) == abi.DC_EWORKSPACE
+
+
 def test_no_tokens_and_no_sequences():
     t = inputs(2, 0, 8, 16, seed=1)
     y, h = dn.selective_scan(*(t[k] for k in NAMES))
@@ -294,6 +328,14 @@ def test_backward_with_lengths(n, dtype):
         for k in ("u", "dt", "b", "c", "z"):
             t[k][i, m:] = float("nan")
     check_backward(t, lens)
+
+
+@pytest.mark.parametrize("n", [4, 8, 16, 24, 64])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_backward_of_long_sequences_of_few_channels(n, dtype):
+    """The time axis in pieces, lengths that end inside each of them."""
+    check_backward(inputs(1, 900, 24, n, dtype=dtype, seed=n))
+    check_backward(inputs(5, 600, 20, n, 2, dtype, seed=n + 1), lens=[0, 1, 130, 599, 600])
 
 
 def test_backward_of_no_tokens():
