@@ -34,11 +34,12 @@ bool vectors(const void *p, int64_t bs, int64_t ts, int64_t elem, int64_t n) {
     return aligned(p, (size_t)(elem * n)) && bs % n == 0 && ts % n == 0;
 }
 
-// Tokens per thread: as many as leave 16 warps for every SM (each run reads K - 1 tokens of its neighbour again, 5 %
-// at 64 tokens and 4 taps), between `least` and `most`.
+// Tokens per thread: as many as leave 24 warps for every SM, between `least` and `most`.  Each run reads K - 1 tokens of
+// its neighbour again (5 % at 64 tokens and 4 taps); ragged 6 x 2049 x 1536 takes 19 us at 24 warps and 23 at
+// 16; at 48 the runs of the backward get too short.
 int run_length(int64_t batch, int64_t seq, int64_t groups, int least, int most) {
     int run = most;
-    while (run > least && batch * ceil_div(seq, run) * groups < (int64_t)sm_count() * 16) run /= 2;
+    while (run > least && batch * ceil_div(seq, run) * groups < (int64_t)sm_count() * 24) run /= 2;
     return run;
 }
 
@@ -72,17 +73,21 @@ int validate_conv(const dc_causal_conv_args *a) {
 }
 
 template <typename TI, typename TO, bool STAGED>
-void launch_conv(const cv::Params &p, dim3 grid, cudaStream_t s) {
-    const size_t smem = STAGED ? sizeof(typename cv::Ring<TI>::Buffer) * (cv::kThreads / 32) : 0;
+int launch_conv(const cv::Params &p, dim3 grid, cudaStream_t s) {
+    const size_t smem = STAGED ? sizeof(typename cv::FwdRing<TI>::Buffer) * (cv::kThreads / 32) : 0;
     auto go = [&](auto *kernel) {
-        if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (smem > 48 * 1024) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e != cudaSuccess) return cuda_fail(e);
+        }
         kernel<<<grid, cv::kThreads, smem, s>>>(p);
+        return launched();
     };
     switch (p.K) {
-        case 2: go(&cv::conv_kernel<TI, TO, STAGED, 2>); break;
-        case 3: go(&cv::conv_kernel<TI, TO, STAGED, 3>); break;
-        case 4: go(&cv::conv_kernel<TI, TO, STAGED, 4>); break;
-        default: go(&cv::conv_kernel<TI, TO, STAGED, cv::kMaxTaps>); break;
+        case 2: return go(&cv::conv_kernel<TI, TO, STAGED, 2>);
+        case 3: return go(&cv::conv_kernel<TI, TO, STAGED, 3>);
+        case 4: return go(&cv::conv_kernel<TI, TO, STAGED, 4>);
+        default: return go(&cv::conv_kernel<TI, TO, STAGED, cv::kMaxTaps>);
     }
 }
 
@@ -101,14 +106,9 @@ int run_conv(const dc_causal_conv_args *a, cv::Params p, cudaStream_t s) {
     const int64_t ctas = ceil_div(a->batch * p.runs, cv::kThreads / 32);
     if (ctas > 0x7fffffff) return DC_EUNSUPPORTED;
     const dim3 grid((unsigned)ctas, (unsigned)groups);
-    if (a->out_dtype == DC_BF16) {
-        if (staged) launch_conv<TI, __nv_bfloat16, true>(p, grid, s);
-        else launch_conv<TI, __nv_bfloat16, false>(p, grid, s);
-    } else {
-        if (staged) launch_conv<TI, float, true>(p, grid, s);
-        else launch_conv<TI, float, false>(p, grid, s);
-    }
-    return launched();
+    if (a->out_dtype == DC_BF16)
+        return staged ? launch_conv<TI, __nv_bfloat16, true>(p, grid, s) : launch_conv<TI, __nv_bfloat16, false>(p, grid, s);
+    return staged ? launch_conv<TI, float, true>(p, grid, s) : launch_conv<TI, float, false>(p, grid, s);
 }
 
 // ---------------------------------------------------------------------------------------------- backward
@@ -138,7 +138,7 @@ int validate_bwd(const dc_causal_conv_bwd_args *a) {
 }
 
 struct BwdShape {
-    bool vec;
+    bool staged, pair;  // x and d_y through rings; pairs of d_x's channels aligned
     int run;
     int64_t runs, groups, ctas;
 };
@@ -146,9 +146,9 @@ struct BwdShape {
 BwdShape bwd_shape(const dc_causal_conv_bwd_args *a) {
     const int64_t is = dtype_size(a->in_dtype), os = dtype_size(a->out_dtype);
     BwdShape b;
-    b.vec = a->channels % cv::kVec == 0 && vectors(a->x, a->x_batch_stride, a->x_token_stride, is, cv::kVec) &&
-            vectors(a->d_x, a->d_x_batch_stride, a->d_x_token_stride, is, cv::kVec) &&
-            vectors(a->d_y, a->d_y_batch_stride, a->d_y_token_stride, os, cv::kVec);
+    b.staged = a->channels % (16 / is) == 0 && vectors(a->x, a->x_batch_stride, a->x_token_stride, is, 16 / is) &&
+               a->channels % (16 / os) == 0 && vectors(a->d_y, a->d_y_batch_stride, a->d_y_token_stride, os, 16 / os);
+    b.pair = vectors(a->d_x, a->d_x_batch_stride, a->d_x_token_stride, is, cv::kVec);
     b.groups = ceil_div(a->channels, cv::kRow);
     b.run = run_length(a->batch, a->seq, b.groups, 16, 64);
     b.runs = a->seq > 0 ? ceil_div(a->seq, b.run) : 1;
@@ -156,25 +156,29 @@ BwdShape bwd_shape(const dc_causal_conv_bwd_args *a) {
     return b;
 }
 
-template <typename TI, typename TO, bool ALIGNED>
-void launch_bwd(const cv::BwdParams &p, dim3 grid, cudaStream_t s) {
+template <typename TI, typename TO, bool STAGED>
+int launch_bwd(const cv::BwdParams &p, dim3 grid, cudaStream_t s) {
+    const size_t smem = STAGED ? sizeof(cv::BwdRings<TI, TO>) * (cv::kBwdThreads / 32) : 0;
+    auto go = [&](auto *kernel) {
+        if (smem > 48 * 1024) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e != cudaSuccess) return cuda_fail(e);
+        }
+        kernel<<<grid, cv::kBwdThreads, smem, s>>>(p);
+        return launched();
+    };
     switch (p.K) {
-        case 2: cv::conv_bwd_kernel<TI, TO, ALIGNED, 2><<<grid, cv::kBwdThreads, 0, s>>>(p); break;
-        case 3: cv::conv_bwd_kernel<TI, TO, ALIGNED, 3><<<grid, cv::kBwdThreads, 0, s>>>(p); break;
-        case 4: cv::conv_bwd_kernel<TI, TO, ALIGNED, 4><<<grid, cv::kBwdThreads, 0, s>>>(p); break;
-        default: cv::conv_bwd_kernel<TI, TO, ALIGNED, cv::kMaxTaps><<<grid, cv::kBwdThreads, 0, s>>>(p); break;
+        case 2: return go(&cv::conv_bwd_kernel<TI, TO, STAGED, 2>);
+        case 3: return go(&cv::conv_bwd_kernel<TI, TO, STAGED, 3>);
+        case 4: return go(&cv::conv_bwd_kernel<TI, TO, STAGED, 4>);
+        default: return go(&cv::conv_bwd_kernel<TI, TO, STAGED, cv::kMaxTaps>);
     }
 }
 
 template <typename TI>
-void launch_bwd_as(bool vec, const cv::BwdParams &p, dim3 grid, cudaStream_t s) {
-    if (p.y_dt) {
-        if (vec) launch_bwd<TI, __nv_bfloat16, true>(p, grid, s);
-        else launch_bwd<TI, __nv_bfloat16, false>(p, grid, s);
-    } else {
-        if (vec) launch_bwd<TI, float, true>(p, grid, s);
-        else launch_bwd<TI, float, false>(p, grid, s);
-    }
+int launch_bwd_as(bool staged, const cv::BwdParams &p, dim3 grid, cudaStream_t s) {
+    if (p.y_dt) return staged ? launch_bwd<TI, __nv_bfloat16, true>(p, grid, s) : launch_bwd<TI, __nv_bfloat16, false>(p, grid, s);
+    return staged ? launch_bwd<TI, float, true>(p, grid, s) : launch_bwd<TI, float, false>(p, grid, s);
 }
 
 }  // namespace
@@ -227,16 +231,14 @@ int dc_causal_conv_bwd(const dc_causal_conv_bwd_args *a, dc_stream_t stream) {
         p.dx_b = a->d_x_batch_stride, p.dx_t = a->d_x_token_stride;
         p.K = a->taps;
         p.silu = (a->flags & DC_CONV_SILU) ? 1 : 0;
-        p.run = b.run, p.runs = (int32_t)b.runs;
+        p.run = b.run, p.runs = (int32_t)b.runs, p.dx_pair = b.pair;
         p.y_dt = a->out_dtype;
         p.dy = a->d_y, p.x = a->x, p.dwin_out = a->d_window_out, p.weight = a->weight, p.bias = a->bias, p.window_in = a->window_in;
         p.lengths = a->lengths;
         p.dx = a->d_x, p.dwin_in = a->d_window_in;
         p.part = static_cast<float *>(a->workspace);
         const dim3 grid((unsigned)b.ctas, (unsigned)b.groups);
-        if (a->in_dtype == DC_BF16) launch_bwd_as<__nv_bfloat16>(b.vec, p, grid, s);
-        else launch_bwd_as<float>(b.vec, p, grid, s);
-        st = launched();
+        st = a->in_dtype == DC_BF16 ? launch_bwd_as<__nv_bfloat16>(b.staged, p, grid, s) : launch_bwd_as<float>(b.staged, p, grid, s);
         if (st != DC_OK) return st;
     }
     cv::conv_bwd_sum_kernel<<<dim3((unsigned)ceil_div(a->channels, 32), (unsigned)(a->taps + 1)), 256, 0, s>>>(

@@ -9,8 +9,13 @@
 // tokens before its run.  Where rows start on 16-byte boundaries each warp stages its 64 channels' tokens through a ring of
 // its own in shared memory (asynchronous copies, 48 tokens ahead, no barrier beyond the warp), so that the bytes in flight
 // do not depend on registers; loads into registers, eight tokens at a time, took 69 us at 8 x 4096 x 2048 bfloat16 where this
-// takes 62 (4.3 TB/s; the exponentials and reciprocals are next, at about half their rate).  The backward recomputes pre from x and carries the K unfinished sums of dx in registers the same way; its run
-// ends K - 1 tokens past its last.
+// takes 62 (4.3 TB/s; the exponentials and reciprocals are next, at about half their rate).
+//
+// The backward recomputes pre from x and carries the K unfinished sums of dx in registers the same way; its run ends
+// K - 1 tokens past its last.  x and dy come through a ring each, 24 tokens ahead, and tokens that lie in the middle of a
+// run are worked on eight at a time without questions about lengths and windows.  Ragged 6 x 2049 x 1536 bfloat16, forward
+// and backward: 61 us (71 with loads into registers), of which the backward is 36 and the sums of the CTAs' parts 5; no unit is
+// above half its rate there, the dependent instructions of few warps (128 registers each) are what is left.
 #pragma once
 
 #include "common.cuh"
@@ -26,8 +31,8 @@ constexpr int kVec = 2;        // channels of a thread
 constexpr int kRow = 32 * kVec;
 constexpr int kStages = 4, kStageTokens = 16;  // of a warp's ring
 constexpr int kUnroll = 8;     // without it: tokens whose loads are in flight together
-constexpr int kBwdThreads = 256;
-constexpr int kBwdUnroll = 8;
+constexpr int kBwdThreads = 128;
+constexpr int kBwdUnroll = 8;  // tokens of a stage, and of a group that is worked on without questions
 
 struct Params {
     int64_t batch, seq, channels;
@@ -77,12 +82,12 @@ __device__ __forceinline__ float2 sigmoid2(float2 x) {
 // silu(x) or x, of a pair
 __device__ __forceinline__ float2 activate(float2 a, bool silu) { return silu ? vec::mul2(a, sigmoid2(a)) : a; }
 
-// A warp's ring: `count` tokens of 64 channels (nch of them real) from src on.
-template <typename T>
+// A warp's ring: `count` tokens of 64 channels (nch of them real) from `from` on, TOKENS of them a stage.
+template <typename T, int TOKENS>
 struct Ring {
     static constexpr int kPer = kRow * sizeof(T) / 16, kEl = 16 / sizeof(T);       // copies per row
-    static constexpr int kRows = 32 / kPer, kEach = kStageTokens / kRows;          // rows of a warp's pass, passes of a stage
-    using Buffer = T[kStages][kStageTokens][kRow];
+    static constexpr int kRows = 32 / kPer, kEach = TOKENS / kRows;                // rows of a warp's pass, passes of a stage
+    using Buffer = T[kStages][TOKENS][kRow];
     const T *src;  // this lane's first copy of the next stage
     int64_t stride;
     uint32_t dst;
@@ -95,20 +100,26 @@ struct Ring {
         src = from + row * stride + (on ? q * kEl : 0);
         dst = ptx::smem_u32(&buf[0][row][q * kEl]);
     }
-    __device__ __forceinline__ void load() {  // the next stage (one commit whatever there is)
+    __device__ __forceinline__ void load() {  // the next stage, if there is one; the caller commits
         if (left > 0) {
-            const uint32_t to = dst + s * (int)sizeof(T) * kStageTokens * kRow;
+            const uint32_t to = dst + s * (int)sizeof(T) * TOKENS * kRow;
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
                 const bool in = on && row + i * kRows < left;
                 ptx::cp_async16(to + i * (int)sizeof(T) * kRows * kRow, in ? src + i * kRows * stride : src - row * stride, in ? 16u : 0u);
             }
-            src += kStageTokens * stride;
-            left -= kStageTokens;
+            src += TOKENS * stride;
+            left -= TOKENS;
             s = s + 1 < kStages ? s + 1 : 0;
         }
-        ptx::cp_async_commit();
     }
+};
+template <typename T>
+using FwdRing = Ring<T, kStageTokens>;
+template <typename TI, typename TO>
+struct BwdRings {
+    typename Ring<TI, kBwdUnroll>::Buffer x;
+    typename Ring<TO, kBwdUnroll>::Buffer dy;
 };
 
 // STAGED: rows start on 16-byte boundaries.  KT: taps compiled in (the call's own, or kMaxTaps with the first KT - K of
@@ -134,11 +145,14 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const Params p) {
     if (t0 < live) {
         const int count = (int)(live - t0);
         const int64_t row0 = (int64_t)blockIdx.y * kRow;
-        auto &buf = reinterpret_cast<typename Ring<TI>::Buffer *>(smem_bytes)[warp];
-        Ring<TI> ring(buf, x + t0 * p.x_t + row0, p.x_t, STAGED ? count : 0, (int)(p.channels - row0 < kRow ? p.channels - row0 : kRow), lane);
+        auto &buf = reinterpret_cast<typename FwdRing<TI>::Buffer *>(smem_bytes)[warp];
+        FwdRing<TI> ring(buf, x + t0 * p.x_t + row0, p.x_t, STAGED ? count : 0, (int)(p.channels - row0 < kRow ? p.channels - row0 : kRow), lane);
         if (STAGED)
 #pragma unroll
-            for (int s = 0; s < kStages - 1; ++s) ring.load();
+            for (int s = 0; s < kStages - 1; ++s) {
+                ring.load();
+                ptx::cp_async_commit();
+            }
         // w[j] belongs to token t - (KT - 1) + j
         float2 w[KT], hist[KT - 1], bias = vec::both(0.f);
         const int64_t ca = n > 0 ? c0 : 0, cb = n > 1 ? c0 + 1 : ca;
@@ -175,6 +189,7 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const Params p) {
                 ptx::cp_async_wait<kStages - 2>();
                 __syncwarp();  // every lane's copies of this stage have landed, and the last stage has been read
                 ring.load();
+                ptx::cp_async_commit();
                 if (left >= kStageTokens) {
 #pragma unroll
                     for (int i = 0; i < kStageTokens; ++i) next(at(i), to + i * p.y_t);
@@ -259,6 +274,7 @@ struct BwdParams {
     int64_t batch, seq, channels;
     int64_t x_b, x_t, dy_b, dy_t, dx_b, dx_t;
     int32_t K, silu, run, runs, y_dt;
+    int32_t dx_pair;  // pairs of dx's channels are aligned
     const void *dy, *x;
     const float *dwin_out, *weight, *bias, *window_in;
     const int32_t *lengths;
@@ -267,11 +283,12 @@ struct BwdParams {
     float *part;  // [gridDim.x][K + 1][channels]: each CTA's sums of d_weight (K lines) and d_bias
 };
 
-// A pair of channels per thread (with ALIGNED as one access), 64 of a warp.  The CTA's warps take consecutive runs of the
-// same channels and add their sums in order in shared memory.
-template <typename TI, typename TO, bool ALIGNED, int KT>
+// A pair of channels per thread, 64 of a warp; STAGED as in the forward, with a ring each for x and dy.  The CTA's warps take
+// consecutive runs of the same channels and add their sums in order in shared memory.
+template <typename TI, typename TO, bool STAGED, int KT>
 __global__ void __launch_bounds__(kBwdThreads) conv_bwd_kernel(const BwdParams p) {
     constexpr int kWarps = kBwdThreads / 32, VEC = kVec;
+    extern __shared__ __align__(16) unsigned char smem_bytes[];
     __shared__ float2 sums[kWarps][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t item = (int64_t)blockIdx.x * kWarps + warp;
@@ -281,7 +298,7 @@ __global__ void __launch_bounds__(kBwdThreads) conv_bwd_kernel(const BwdParams p
     float2 dw[KT], db = vec::both(0.f);
 #pragma unroll
     for (int j = 0; j < KT; ++j) dw[j] = vec::both(0.f);
-    if (item < p.batch * p.runs && n > 0) {
+    if (item < p.batch * p.runs) {
         const int64_t b = item / p.runs, t0 = (item - b * p.runs) * (int64_t)p.run;
         const int64_t len = length_of(p.lengths, b, p.seq);
         const int64_t t1 = t0 + p.run < p.seq ? t0 + p.run : p.seq;
@@ -290,28 +307,62 @@ __global__ void __launch_bounds__(kBwdThreads) conv_bwd_kernel(const BwdParams p
         const float *win = p.window_in ? p.window_in + b * p.channels * K : nullptr;
         const float *dnext = p.dwin_out ? p.dwin_out + b * p.channels * K : nullptr;
         float *dwin = p.dwin_in ? p.dwin_in + b * p.channels * K : nullptr;
-        const int64_t c1 = n > 1 ? c0 + 1 : c0;
+        const int64_t ca = n > 0 ? c0 : 0, c1 = n > 1 ? c0 + 1 : ca;  // a lane without channels reads channel 0's, writes none
+        const bool pair = n == VEC && p.dx_pair;
+        auto put = [&](TI *o, float2 v) {
+            const float out[VEC] = {v.x, v.y};
+            if (pair) vec::store<true>(o, out);
+            else vec::store<false>(o, out, n);
+        };
+        const int count = (int)(t1 - t0), end = count + KT - 1;               // tokens past t1 only finish the run's last sums
+        const int live = len - t0 < 0 ? 0 : len - t0 < end ? (int)(len - t0) : end;  // tokens that are read
+        const int64_t row0 = (int64_t)blockIdx.y * kRow;
+        const int nch = (int)(p.channels - row0 < kRow ? p.channels - row0 : kRow);
+        auto &rings = reinterpret_cast<BwdRings<TI, TO> *>(smem_bytes)[warp];
+        Ring<TI, kBwdUnroll> rx(rings.x, x + t0 * p.x_t + row0, p.x_t, STAGED ? live : 0, nch, lane);
+        Ring<TO, kBwdUnroll> rg(rings.dy, static_cast<const TO *>(p.dy) + b * p.dy_b + t0 * p.dy_t + row0, p.dy_t, STAGED ? live : 0, nch, lane);
+        auto load = [&] {
+            rx.load();
+            rg.load();
+            ptx::cp_async_commit();
+        };
+        if (STAGED)
+#pragma unroll
+            for (int s = 0; s < kStages - 1; ++s) load();
         float2 w[KT], hist[KT - 1], d[KT];
-        const float2 bias = p.bias ? make_float2(p.bias[c0], p.bias[c1]) : vec::both(0.f);
+        const float2 bias = p.bias ? make_float2(p.bias[ca], p.bias[c1]) : vec::both(0.f);
 #pragma unroll
         for (int j = 0; j < KT; ++j) {
-            w[j] = j >= KT - K ? make_float2(p.weight[c0 * K + j - (KT - K)], p.weight[c1 * K + j - (KT - K)]) : vec::both(0.f);
+            w[j] = j >= KT - K ? make_float2(p.weight[ca * K + j - (KT - K)], p.weight[c1 * K + j - (KT - K)]) : vec::both(0.f);
             d[j] = vec::both(0.f);
         }
 #pragma unroll
         for (int j = 0; j < KT - 1; ++j) {
             const int64_t t = t0 - (KT - 1) + j;
             hist[j] = vec::both(0.f);
-            if (j >= KT - K && t < len) {
-                hist[j].x = token(x, p.x_t, win, K, t, c0);
-                if (n > 1) hist[j].y = token(x, p.x_t, win, K, t, c1);
-            }
+            if (j >= KT - K && t < len) hist[j] = make_float2(token(x, p.x_t, win, K, t, ca), token(x, p.x_t, win, K, t, c1));
         }
+        const TI *from = x + t0 * p.x_t + ca;
+        const TO *gfrom = static_cast<const TO *>(p.dy) + b * p.dy_b + t0 * p.dy_t + ca;
+        int stage = -1;  // of the rings
+        auto advance = [&] {  // the next stage is there
+            ptx::cp_async_wait<kStages - 2>();
+            __syncwarp();
+            load();
+            stage = stage + 1 < kStages ? stage + 1 : 0;
+        };
+        auto fetch = [&](int t, float2 &v, float2 &g) {  // token t < live
+            float a[VEC], c[VEC];
+            if (STAGED) {
+                vec::load<true>(&rings.x[stage][t % kBwdUnroll][lane * VEC], a);
+                vec::load<true>(&rings.dy[stage][t % kBwdUnroll][lane * VEC], c);
+            } else {
+                vec::load<false>(from + t * p.x_t, a, n);
+                vec::load<false>(gfrom + t * p.dy_t, c, n);
+            }
+            v = make_float2(a[0], a[1]), g = make_float2(c[0], c[1]);
+        };
         // d[j] gathers dx of token t - (KT - 1) + j while the gradient of pre_t passes by; after token t, d[0] is complete
-        const int count = (int)(t1 - t0), end = count + KT - 1;               // tokens past t1 only finish the run's last sums
-        const int live = len - t0 < 0 ? 0 : len - t0 < end ? (int)(len - t0) : end;  // tokens that are read
-        const TI *from = x + t0 * p.x_t + c0;
-        const TO *gfrom = static_cast<const TO *>(p.dy) + b * p.dy_b + t0 * p.dy_t + c0;
         auto pass = [&](float2 v, float2 g, bool read, bool own) {  // token t: its gradients into d, and into dw and db if its own
             float2 pre = bias;
 #pragma unroll
@@ -339,64 +390,62 @@ __global__ void __launch_bounds__(kBwdThreads) conv_bwd_kernel(const BwdParams p
             for (int j = 0; j < KT - 2; ++j) hist[j] = j >= KT - K ? hist[j + 1] : vec::both(0.f);
             if (KT - 2 >= KT - K) hist[KT - 2] = v;
         };
+        auto window = [&](int64_t tau, float2 v) {  // the gradient of a token of the window (t0 is 0)
+            if (!dwin || tau < -(K - 1)) return;
+            const int m = K + (int)tau;
+            const bool more = dnext && m >= len;
+            if (n > 0) dwin[c0 * K + m] = v.x + (more ? dnext[c0 * K + m - (int)len] : 0.f);
+            if (n > 1) dwin[c1 * K + m] = v.y + (more ? dnext[c1 * K + m - (int)len] : 0.f);
+        };
         auto any = [&](int t) {  // a token of whatever place
             const bool read = t < live;
             float2 v = vec::both(0.f), g = vec::both(0.f);
-            if (read) {
-                vec::Raw<TI, VEC> in;
-                vec::Raw<TO, VEC> gin;
-                vec::load_raw<ALIGNED>(from + t * p.x_t, in, n);
-                vec::load_raw<ALIGNED>(gfrom + t * p.dy_t, gin, n);
-                v = vec::pair_of(in, 0), g = vec::pair_of(gin, 0);
-            }
+            if (STAGED && t % kBwdUnroll == 0) advance();
+            if (read) fetch(t, v, g);
             pass(v, g, read, t < count);
             const int64_t tau = t0 + t - (KT - 1);  // d[0]'s token
             if (tau >= t0) {
                 if (dnext && tau < len && tau >= len - K) {
-                    d[0].x += dnext[c0 * K + (int)(tau - len + K)];
+                    if (n > 0) d[0].x += dnext[c0 * K + (int)(tau - len + K)];
                     if (n > 1) d[0].y += dnext[c1 * K + (int)(tau - len + K)];
                 }
-                const float out[VEC] = {d[0].x, d[0].y};
-                vec::store<ALIGNED>(dx + tau * p.dx_t, out, n);
-            } else if (dwin && tau < 0 && tau >= -(K - 1)) {  // t0 is 0: a token of the window
-                const int m = K + (int)tau;
-                const bool more = dnext && m >= len;
-                dwin[c0 * K + m] = d[0].x + (more ? dnext[c0 * K + m - (int)len] : 0.f);
-                if (n > 1) dwin[c1 * K + m] = d[0].y + (more ? dnext[c1 * K + m - (int)len] : 0.f);
+                put(dx + tau * p.dx_t, d[0]);
+            } else if (tau < 0) {
+                window(tau, d[0]);
             }
             shift(v);
         };
+        // eight tokens that are read and the run's own, and finish tokens that the window's gradient does not reach
+        auto group = [&](int t, bool opens) {
+            if (STAGED) advance();
+            TI *o = dx + (t0 + t - (KT - 1)) * p.dx_t;
+            float2 v[kBwdUnroll], g[kBwdUnroll];
+#pragma unroll
+            for (int i = 0; i < kBwdUnroll; ++i) fetch(t + i, v[i], g[i]);
+#pragma unroll
+            for (int i = 0; i < kBwdUnroll; ++i) {
+                pass(v[i], g[i], true, true);
+                if (i < KT - 1 && opens) {
+                    if (t0 == 0) window(i - (KT - 1), d[0]);
+                } else {
+                    put(o + i * p.dx_t, d[0]);
+                }
+                shift(v[i]);
+            }
+        };
         // from `stop` on every sum is zero; a run that lies behind the sequence's end has none at all
         const int stop = live == 0 && t0 > 0 ? 0 : live + KT - 1 < end ? live + KT - 1 : end;
-        int t = 0;
-        for (; t < KT - 1 && t < stop; ++t) any(t);
-        // whole groups of tokens that are read, the run's own, and finish tokens before the window's gradient reaches
         const int plain_end = (int)min((int64_t)min(count, live), dnext ? len - K + (KT - 1) - t0 : (int64_t)count);
-        const TI *f = from + t * p.x_t;
-        const TO *gf = gfrom + t * p.dy_t;
-        TI *o = dx + t0 * p.dx_t;
-        for (; t + kBwdUnroll <= plain_end; t += kBwdUnroll, f += kBwdUnroll * p.x_t, gf += kBwdUnroll * p.dy_t, o += kBwdUnroll * p.dx_t) {
-            vec::Raw<TI, VEC> in[kBwdUnroll];
-            vec::Raw<TO, VEC> gin[kBwdUnroll];
-#pragma unroll
-            for (int i = 0; i < kBwdUnroll; ++i) {
-                vec::load_raw<ALIGNED>(f + i * p.x_t, in[i], n);
-                vec::load_raw<ALIGNED>(gf + i * p.dy_t, gin[i], n);
-            }
-#pragma unroll
-            for (int i = 0; i < kBwdUnroll; ++i) {
-                const float2 v = vec::pair_of(in[i], 0);
-                pass(v, vec::pair_of(gin[i], 0), true, true);
-                const float out[VEC] = {d[0].x, d[0].y};
-                vec::store<ALIGNED>(o + i * p.dx_t, out, n);
-                shift(v);
-            }
+        int t = 0;
+        if (KT - 1 <= kBwdUnroll && kBwdUnroll <= plain_end) {
+            group(0, true);
+            for (t = kBwdUnroll; t + kBwdUnroll <= plain_end; t += kBwdUnroll) group(t, false);
         }
         for (; t < stop; ++t) any(t);
-        const float none[VEC] = {0.f, 0.f};
-        for (int64_t tau = t0 + (stop > KT - 1 ? stop - (KT - 1) : 0); tau < t1; ++tau) vec::store<ALIGNED>(dx + tau * p.dx_t, none, n);
+        if (STAGED) ptx::cp_async_wait<0>();
+        for (int64_t tau = t0 + (stop > KT - 1 ? stop - (KT - 1) : 0); tau < t1; ++tau) put(dx + tau * p.dx_t, vec::both(0.f));
         if (dwin && t0 == 0) {  // column 0 reaches the output only as an unshifted window
-            dwin[c0 * K] = dnext && len == 0 ? dnext[c0 * K] : 0.f;
+            if (n > 0) dwin[c0 * K] = dnext && len == 0 ? dnext[c0 * K] : 0.f;
             if (n > 1) dwin[c1 * K] = dnext && len == 0 ? dnext[c1 * K] : 0.f;
         }
     }
