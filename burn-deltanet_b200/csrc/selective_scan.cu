@@ -27,17 +27,17 @@ struct Cut {
 };
 
 // By the CTAs that the walk would give and those that the card holds (`room`).  Measured, state 16, bfloat16, microseconds:
-//   8 x 4096 x 2048 (1024 CTAs): walk 467, segments 1067      4 x 2048 x 2048 (512): walk 153, segments 311
-//   2 x 4096 x 2048 (256): walk 254, segments 310, 4 pieces 217
-//   1 x 4096 x 2048 (128): walk 223, segments 159, 8 pieces 119
-//   1 x 16384 x 1024 (64): walk 872, segments 478, 16 pieces 226
+//   8 x 4096 x 2048 (1024 CTAs): walk 463, segments 1067      4 x 2048 x 2048 (512): walk 151, segments 311
+//   2 x 4096 x 2048 (256): walk 254, segments 310, 4 pieces 213
+//   1 x 4096 x 2048 (128): walk 223, segments 159, 8 pieces 116
+//   1 x 16384 x 1024 (64): walk 872, segments 478, 16 pieces 220
 // So: the walk from a third of the room on; below that as many pieces as fill the room, each 128 tokens at least, if
 // that makes three or more of them; else segments.
 Cut cut_of(const dc_selective_scan_args *a, bool workspace) {
     constexpr int64_t kLeast = 128;  // a multiple of every checkpoint's distance
     const int lanes = sc::lanes_of(a->state);
     const int64_t ctas = a->batch * a->groups * ceil_div(a->channels / a->groups, sc::walk_channels(lanes));
-    const int64_t room = (int64_t)sm_count() * sc::walk_ctas(lanes);
+    const int64_t room = (int64_t)sm_count() * sc::walk_ctas(lanes, dtype_size(a->in_dtype));
     Cut c{false, 1, a->seq};
     if (3 * ctas > room) return c;
     const int64_t want = room / ctas, most = a->seq / kLeast, pieces = want < most ? want : most;

@@ -102,6 +102,14 @@ __device__ __forceinline__ float dot(F4 a, F4 b) {
 __device__ __forceinline__ F4 zero4() { return {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}; }
 __device__ __forceinline__ F4 one4() { return {make_float2(1.f, 1.f), make_float2(1.f, 1.f)}; }
 
+// four values in shared memory
+template <typename T>
+__device__ __forceinline__ F4 four(const T *p) {
+    float v[kS];
+    vec::load<true>(p, v);
+    return {make_float2(v[0], v[1]), make_float2(v[2], v[3])};
+}
+
 // four states n .. n + 3 of a row of N (states past N are 0)
 __device__ __forceinline__ F4 load4(const float *row, int n, int N) {
     if ((N & 3) == 0 && aligned16(row)) return n < N ? f4(*reinterpret_cast<const float4 *>(row + n)) : zero4();
@@ -256,44 +264,52 @@ struct Quads {
         if (yquad) vec::store_as<true>(p.y_dt, p.y, y0 + t * p.y_t, v);
         else vec::store_as<false>(p.y_dt, p.y, y0 + t * p.y_t, v, ny);
     }
-    // raw dt and u of `live` tokens to (step, step * u)
+    // raw dt and u of a token to (step, step * u)
+    __device__ __forceinline__ void step_of(float2 *step, float (&v)[4], const float (&x)[4], bool live) const {
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+            float2 f = make_float2(v[j] + bias[j], v[j + 1] + bias[j + 1]);
+            if (p.softplus) f = softplus2(f);
+            v[j] = live ? f.x : 0.f, v[j + 1] = live ? f.y : 0.f;  // past the end: decay 1, nothing added
+        }
+        float4 *o = reinterpret_cast<float4 *>(step);
+        o[0] = make_float4(v[0], v[0] * x[0], v[1], v[1] * x[1]);
+        o[1] = make_float4(v[2], v[2] * x[2], v[3], v[3] * x[3]);
+    }
+    // a token's y, from the P shares of it: y[token][state group][channel]
+    __device__ __forceinline__ void sum_of(const float *y, int t, float (&v)[4]) const {
+        // from another share on in each token, so that a warp's reads meet in no bank
+        const float *row = y + t * CH * P + oc;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const float4 f = *reinterpret_cast<const float4 *>(row + ((i + t) & (P - 1)) * CH);
+            v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
+        }
+    }
+    __device__ __forceinline__ void finish(float (&v)[4], const float (&x)[4], const float (&z)[4], bool gated) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] = fmaf(skip[j], x[j], v[j]);
+            if (gated) v[j] *= z[j] * sigmoid(z[j]);
+        }
+    }
     __device__ __forceinline__ void steps(float2 *step, const TI *dt, const TI *u, int live) const {
 #pragma unroll 2
         for (int t = orow; t < TOK; t += kRows) {
             float v[4], x[4];
             vec::load<true>(dt + t * CH + oc, v);
             vec::load<true>(u + t * CH + oc, x);
-#pragma unroll
-            for (int j = 0; j < 4; j += 2) {
-                float2 f = make_float2(v[j] + bias[j], v[j + 1] + bias[j + 1]);
-                if (p.softplus) f = softplus2(f);
-                v[j] = t < live ? f.x : 0.f, v[j + 1] = t < live ? f.y : 0.f;  // past the end: decay 1, nothing added
-            }
-            float4 *o = reinterpret_cast<float4 *>(step + t * CH + oc);
-            o[0] = make_float4(v[0], v[0] * x[0], v[1], v[1] * x[1]);
-            o[1] = make_float4(v[2], v[2] * x[2], v[3], v[3] * x[3]);
+            step_of(step + t * CH + oc, v, x, t < live);
         }
     }
-    // y of `live` tokens from t0 on, from the P shares of each: y[token][state group][channel]
     __device__ __forceinline__ void outputs(const float *y, const TI *u, const TI *z, int64_t t0, int live) const {
 #pragma unroll 2
         for (int t = orow; t < live; t += kRows) {
-            float v[4] = {0.f, 0.f, 0.f, 0.f}, x[4];
-            // from another share on in each token, so that a warp's reads meet in no bank
-            const float *row = y + t * CH * P + oc;
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-                const float4 f = *reinterpret_cast<const float4 *>(row + ((i + t) & (P - 1)) * CH);
-                v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
-            }
+            float v[4] = {0.f, 0.f, 0.f, 0.f}, x[4], g[4];
+            sum_of(y, t, v);
             vec::load<true>(u + t * CH + oc, x);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = fmaf(skip[j], x[j], v[j]);
-            if (z) {
-                vec::load<true>(z + t * CH + oc, x);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] *= x[j] * sigmoid(x[j]);
-            }
+            if (z) vec::load<true>(z + t * CH + oc, g);
+            finish(v, x, g, z != nullptr);
             put(t0 + t, v);
         }
     }
@@ -321,14 +337,18 @@ struct Stager {
     static constexpr int kX = TOK * kXRow, kB = TOK * kBRow;                                                    // and per tensor
     static constexpr int kAll = FULL ? 3 * kX + 2 * kB : 2 * kX + kB, kEach = (kAll + NT - 1) / NT;
     const char *src[kEach];
-    int64_t step[kEach];  // bytes a tile
-    int dst[kEach], row[kEach], bytes[kEach];
+    int32_t step[kEach];    // bytes a tile
+    uint32_t where[kEach];  // the copy's place in the tile | its row << 16 (TOK: none) | its bytes << 24, to save registers
     bool on;
+    static_assert(kAll <= 65536 && TOK < 256, "they fit");
 
     __device__ __forceinline__ Stager(const Work<TI, CH, N4> &wk, int tid) {
         const Params &p = wk.p;
         on = p.vec_x == kVectors && p.vec_bc == kVectors && N4 % kEl == 0 && (!FULL || wk.Z) && aligned16(wk.U) && aligned16(wk.D) && aligned16(wk.B) &&
              (!FULL || (aligned16(wk.Z) && aligned16(wk.C)));
+        const int64_t strides[] = {p.u_t, p.dt_t, p.b_t, FULL ? p.c_t : 0, FULL ? p.z_t : 0};
+#pragma unroll
+        for (int k = 0; k < 5; ++k) on = on && strides[k] >= 0 && strides[k] <= INT32_MAX / (TOK * kEs);
         if (!on) return;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
@@ -350,11 +370,10 @@ struct Stager {
                 }
             }
             const int r = used ? c / per : 0, q = used ? c % per : 0, left = (width - q * kEl) * kEs;
-            row[j] = used ? r : TOK;  // a row that no tile has
-            bytes[j] = left < 0 ? 0 : left > 16 ? 16 : left;
-            dst[j] = (base + (used ? c : 0)) * 16;
-            src[j] = reinterpret_cast<const char *>(t + (wk.first + r) * st + (bytes[j] ? q * kEl : 0));
-            step[j] = st * (int64_t)(TOK * kEs);
+            const int bytes = left < 0 ? 0 : left > 16 ? 16 : left;
+            where[j] = (uint32_t)(base + (used ? c : 0)) | (uint32_t)(used ? r : TOK) << 16 | (uint32_t)bytes << 24;
+            src[j] = reinterpret_cast<const char *>(t + (wk.first + r) * st + (bytes ? q * kEl : 0));
+            step[j] = (int32_t)(st * (TOK * kEs));
         }
     }
     template <typename Raw>
@@ -363,41 +382,53 @@ struct Stager {
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
             // past the end: no bytes, from the tile's first row, which is always inside the sequence
-            if (row[j] < TOK)
-                ptx::cp_async16(to + dst[j], row[j] < live ? src[j] : src[j] - step[j] / TOK * row[j], row[j] < live ? bytes[j] : 0);
+            const int row = (int)(where[j] >> 16 & 255);
+            const bool real = row < live;
+            if (row < TOK) ptx::cp_async16(to + (where[j] & 65535) * 16, real ? src[j] : src[j] - step[j] / TOK * row, real ? where[j] >> 24 : 0);
             src[j] += step[j];
         }
     }
 };
 
-// ---- token by token.  A thread of the recurrence has four states of two neighbouring channels: b and c come from shared
-// memory once for both, and shared memory's bandwidth would be the bound otherwise (at one channel a thread, 80 % of it
-// was in use and the largest case took 568 us).  kHelp further threads stage the tiles, take the steps of the next tile
-// and write y of the last one, so that the two kinds of work, each a chain of dependent instructions, fill each other's
-// gaps.  One barrier per tile of 16 tokens.
+// ---- token by token.  A thread of the recurrence has four states of one channel (of two where a warp would not be full, or
+// where the threads would be too many for their registers).  kHelp further threads stage the tiles, take the steps of the
+// next tile and write y of the last one, so that the two kinds of work, each a chain of dependent instructions, fill each
+// other's gaps; one barrier per tile of 16 tokens.  8 x 4096 x 2048 x 16 bfloat16 takes 463 us: the special-function unit,
+// the issue slots and the shared memory's data path are each at 0.63 of their rate there (294 us for the first alone), and
+// what shortens one lengthens another: exponentials taken ahead of their use 495 us, b and c read as bfloat16 and widened by
+// the reader 498, steps stored twice to spare the moves of two-wide arithmetic 596.  5 x 777 x 1000 x 24 float32 in 2 groups:
+// 69 us, the longest sequence's chain of dependent instructions, 0.09 us a token.
 // FULL: the whole scan; else only the piece's end state from zero and its sum of steps.
 constexpr int walk_channels(int lanes) { return lanes >= 4 ? 16 : 64 / lanes; }       // of a CTA: a warp's at least
-constexpr int walk_ctas(int lanes) { return lanes == 4 ? 7 : lanes == 2 || lanes == 8 ? 4 : lanes == 16 ? 3 : 2; }  // of an SM, by their registers and shared memory
+constexpr int walk_each(int lanes) { return lanes == 1 || lanes == 16 ? 2 : 1; }     // channels of a thread of the recurrence
+// CTAs of an SM, by their registers and shared memory (float32 inputs take twice the staging space and more addresses).
+constexpr int walk_ctas(int lanes, int64_t bytes) {
+    return lanes == 4 ? (bytes == 2 ? 7 : 6) : lanes == 8 ? (bytes == 2 ? 4 : 3) : lanes == 16 ? (bytes == 2 ? 3 : 2) : lanes == 2 ? 4 : 2;
+}
 template <int P>
 struct WalkShape {
-    static constexpr int kCh = walk_channels(P), kMain = kCh * P / 2, kHelp = 4 * kCh, kNT = kMain + kHelp;
+    static constexpr int kCh = walk_channels(P), kV = walk_each(P), kMain = kCh * P / kV, kHelp = 4 * kCh, kNT = kMain + kHelp;
     static constexpr int kTok = kTile, kStages = 4, kN = kS * P;
 };
 template <typename TI, int P>
 struct WalkSmem {
     using S = WalkShape<P>;
+    // b and c of 16 bits once more in float32: the recurrence reads them for every channel (read as they are, and widened
+    // there: slower, as above)
+    static constexpr bool kWiden = sizeof(TI) < 4;
     RawTile<TI, S::kCh, S::kTok, S::kN> raw[S::kStages];
-    float2 step[2][S::kTok * S::kCh];
-    float4 b[2][S::kTok * P], c[2][S::kTok * P];
+    float2 step[2][S::kTok * S::kCh];  // (step, step * u)
+    float4 b[kWiden ? 2 : 1][kWiden ? S::kTok * P : 1], c[kWiden ? 2 : 1][kWiden ? S::kTok * P : 1];
     float y[2][S::kTok * S::kCh * P];
 };
 
 template <typename TI, int P, bool FULL>
-__global__ void __launch_bounds__(WalkShape<P>::kNT, walk_ctas(P)) scan_walk_kernel(const Params p) {
+__global__ void __launch_bounds__(WalkShape<P>::kNT, walk_ctas(P, sizeof(TI))) scan_walk_kernel(const Params p) {
     using S = WalkShape<P>;
-    constexpr int kTok = S::kTok, CH = S::kCh, kBatch = 4;
+    constexpr int V = S::kV, kTok = S::kTok, CH = S::kCh, kBatch = 4;
     extern __shared__ __align__(16) unsigned char smem_bytes[];
     WalkSmem<TI, P> &sm = *reinterpret_cast<WalkSmem<TI, P> *>(smem_bytes);
+    constexpr bool kWiden = WalkSmem<TI, P>::kWiden;
     const int64_t pieces = FULL ? p.pieces : p.pieces - 1;  // nothing follows the last piece's end
     const Work<TI, CH, S::kN> wk(p, blockIdx.x, pieces);
     const Place &at = wk.at;
@@ -408,50 +439,79 @@ __global__ void __launch_bounds__(WalkShape<P>::kNT, walk_ctas(P)) scan_walk_ker
         const int tid = threadIdx.x - S::kMain;
         const Quads<TI, P, CH, kTok, S::kHelp> quads(p, at, tid);
         Stager<TI, CH, S::kN, kTok, S::kHelp, FULL> stager(wk, tid);
-        auto live = [&](int i) { return len - first - (int64_t)i * kTok < kTok ? (int)(len - first - (int64_t)i * kTok) : kTok; };
-        auto prepare = [&](int i) {  // tile i's steps, b and c, once every helper's copies of it have landed
-            const auto &w = sm.raw[i % S::kStages];
-            ptx::named_sync(1, S::kHelp);
-            quads.steps(sm.step[i & 1], w.dt, w.u, live(i));
-            widen<S::kHelp>(sm.b[i & 1], w.b, kTok * S::kN, tid);
-            if (FULL) widen<S::kHelp>(sm.c[i & 1], w.c, kTok * S::kN, tid);
-        };
+        static_assert(kTok == decltype(quads)::kRows, "a helper has one token of a tile");
+        constexpr int kQuad = kTok * S::kN / 4, kBc = kWiden ? (kQuad + S::kHelp - 1) / S::kHelp : 0;  // quads of b in a tile, a helper's
+        const int end = n > 0 ? (int)(len - first - (int64_t)(n - 1) * kTok) : 0, row = quads.orow * CH + quads.oc;
+        auto live = [&](int i) { return i + 1 < n ? kTok : end; };
         auto load = [&](int i) {
             if (i < n) {
-                if (stager.on) stager.copy(sm.raw[i % S::kStages], live(i));
-                else wk.template load<S::kHelp, kTok, FULL>(sm.raw[i % S::kStages], first + (int64_t)i * kTok, tid);
+                if (stager.on) stager.copy(sm.raw[i & (S::kStages - 1)], live(i));
+                else wk.template load<S::kHelp, kTok, FULL>(sm.raw[i & (S::kStages - 1)], first + (int64_t)i * kTok, tid);
             }
             ptx::cp_async_commit();
         };
+        // One token and four channels of tile i - 1's outputs and of tile i + 1's steps: two chains of dependent
+        // instructions in one stretch of code, the loads of both in front.
+        auto turn = [&](int i, bool before, bool after) {
+            const auto &w = sm.raw[(i + 1) & (S::kStages - 1)], &o = sm.raw[(i - 1) & (S::kStages - 1)];
+            float v[4] = {0.f, 0.f, 0.f, 0.f}, x[4], z[4], f[4], g[4], bv[kBc + 1][4], cv[kBc + 1][4];
+            if (FULL && before) {
+                quads.sum_of(sm.y[(i - 1) & 1], quads.orow, v);
+                vec::load<true>(o.u + row, x);
+                vec::load<true>(o.z + row, z);  // (nothing of use without a gate)
+            }
+            if (after) {
+                vec::load<true>(w.dt + row, f);
+                vec::load<true>(w.u + row, g);
+#pragma unroll
+                for (int j = 0; j < kBc; ++j)
+                    if (kQuad % S::kHelp == 0 || tid + j * S::kHelp < kQuad) {
+                        vec::load<true>(w.b + 4 * (tid + j * S::kHelp), bv[j]);
+                        if (FULL) vec::load<true>(w.c + 4 * (tid + j * S::kHelp), cv[j]);
+                    }
+                quads.step_of(sm.step[(i + 1) & 1] + row, f, g, quads.orow < live(i + 1));
+            }
+            if (FULL && before) {
+                quads.finish(v, x, z, wk.Z != nullptr);
+                quads.put(first + (int64_t)(i - 1) * kTok + quads.orow, v);
+            }
+            if (after) {
+#pragma unroll
+                for (int j = 0; j < kBc; ++j)
+                    if (kQuad % S::kHelp == 0 || tid + j * S::kHelp < kQuad) {
+                        sm.b[(i + 1) & 1][tid + j * S::kHelp] = make_float4(bv[j][0], bv[j][1], bv[j][2], bv[j][3]);
+                        if (FULL) sm.c[(i + 1) & 1][tid + j * S::kHelp] = make_float4(cv[j][0], cv[j][1], cv[j][2], cv[j][3]);
+                    }
+            }
+        };
         load(0);
         load(1);
-        ptx::cp_async_wait<1>();
-        if (n > 0) prepare(0);
+        ptx::cp_async_wait<0>();
+        ptx::named_sync(1, S::kHelp);  // every helper's copies
+        if (n > 0) turn(-1, false, true);
         __syncthreads();
         for (int i = 0; i < n; ++i) {
             load(i + 2);
-            if (FULL && i > 0) {
-                const auto &w = sm.raw[(i - 1) % S::kStages];
-                quads.outputs(sm.y[(i - 1) & 1], w.u, wk.Z ? w.z : nullptr, first + (int64_t)(i - 1) * kTok, kTok);
-            }
-            ptx::cp_async_wait<1>();
-            if (i + 1 < n) prepare(i + 1);
+            if (FULL && i > 0 && i + 1 < n) turn(i, true, true);
+            else if (i + 1 < n) turn(i, false, true);
+            else if (FULL && i > 0) turn(i, true, false);
+            ptx::cp_async_wait<0>();
             __syncthreads();
         }
         if (FULL && n > 0) {
-            const auto &w = sm.raw[(n - 1) % S::kStages];
-            quads.outputs(sm.y[(n - 1) & 1], w.u, wk.Z ? w.z : nullptr, first + (int64_t)(n - 1) * kTok, live(n - 1));
+            const auto &w = sm.raw[(n - 1) & (S::kStages - 1)];
+            quads.outputs(sm.y[(n - 1) & 1], w.u, wk.Z ? w.z : nullptr, first + (int64_t)(n - 1) * kTok, end);
         }
         if (FULL) quads.zeros(len > first ? len : first, wk.last);
         return;
     }
 
-    const int ch = 2 * (threadIdx.x % (CH / 2)), q = threadIdx.x / (CH / 2), N = p.N;
+    const int ch = V * (threadIdx.x % (CH / V)), q = threadIdx.x / (CH / V), N = p.N;
     const int64_t d = at.d0 + ch, piece = pieces > 1 ? blockIdx.x % pieces : 0;
-    bool real[2];
-    F4 a2[2], h[2];
+    bool real[V];
+    F4 a2[V], h[V];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < V; ++j) {
         real[j] = ch + j < at.nch;
         a2[j] = real[j] ? mul(kLog2e, load4(p.a + (d + j) * N, kS * q, N)) : zero4();
         h[j] = zero4();
@@ -466,37 +526,47 @@ __global__ void __launch_bounds__(WalkShape<P>::kNT, walk_ctas(P)) scan_walk_ker
             h[j] = load4(p.state_in + (at.b * p.channels + d + j) * N, kS * q, N);
         }
     }
-    float2 steps = make_float2(0.f, 0.f);
+    float steps[V] = {};
     __syncthreads();
     for (int i = 0; i < n; ++i) {
         const float2 *step = sm.step[i & 1] + ch;
-        const float4 *b = sm.b[i & 1] + q, *c = sm.c[i & 1] + q;
+        const auto &raw = sm.raw[i & (S::kStages - 1)];
+        const float *b = reinterpret_cast<const float *>(kWiden ? (const void *)sm.b[i & 1] : (const void *)raw.b) + kS * q;
+        const float *c = reinterpret_cast<const float *>(kWiden ? (const void *)sm.c[i & 1] : (const void *)raw.c) + kS * q;
         float *y = sm.y[i & 1] + q * CH + ch;
         if (FULL && p.ckpt)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < V; ++j)
                 if (real[j]) checkpoint(p, at, first + (int64_t)i * kTok, d + j, q, h[j]);
 #pragma unroll 1
         for (int k0 = 0; k0 < kTok; k0 += kK) {
 #pragma unroll
             for (int k1 = 0; k1 < kK; k1 += kBatch) {
-                F4 av[kBatch][2], bv[kBatch][2];
+                F4 av[kBatch][V], bv[kBatch][V];
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) {
                     const int t = k0 + k1 + k;
-                    const float4 sd = *reinterpret_cast<const float4 *>(step + t * CH);  // both channels' (step, step * u)
-                    const F4 bt = f4(b[t * P]);
-                    av[k][0] = ex2(mul(sd.x, a2[0])), av[k][1] = ex2(mul(sd.z, a2[1]));
-                    bv[k][0] = mul(sd.y, bt), bv[k][1] = mul(sd.w, bt);
-                    if (!FULL) steps.x += sd.x, steps.y += sd.z;
+                    float sd[2 * V];  // each channel's (step, step * u)
+                    vec::load<true>(&step[t * CH].x, sd);
+                    const F4 bt = four(b + t * S::kN);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        av[k][j] = ex2(mul(sd[2 * j], a2[j])), bv[k][j] = mul(sd[2 * j + 1], bt);
+                        if (!FULL) steps[j] += sd[2 * j];
+                    }
                 }
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) {
                     const int t = k0 + k1 + k;
-                    h[0] = fma(av[k][0], h[0], bv[k][0]), h[1] = fma(av[k][1], h[1], bv[k][1]);
+                    float sum[V];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) h[j] = fma(av[k][j], h[j], bv[k][j]);
                     if (FULL) {
-                        const F4 ct = f4(c[t * P]);
-                        *reinterpret_cast<float2 *>(y + t * CH * P) = make_float2(dot(h[0], ct), dot(h[1], ct));
+                        const F4 ct = four(c + t * S::kN);
+#pragma unroll
+                        for (int j = 0; j < V; ++j) sum[j] = dot(h[j], ct);
+                        if constexpr (V == 2) *reinterpret_cast<float2 *>(y + t * CH * P) = make_float2(sum[0], sum[1]);
+                        else y[t * CH * P] = sum[0];
                     }
                 }
             }
@@ -504,7 +574,7 @@ __global__ void __launch_bounds__(WalkShape<P>::kNT, walk_ctas(P)) scan_walk_ker
         __syncthreads();
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < V; ++j) {
         if (!real[j]) continue;
         const int64_t own = (at.b * p.channels + d + j) * N;
         if (FULL) {
@@ -513,7 +583,7 @@ __global__ void __launch_bounds__(WalkShape<P>::kNT, walk_ctas(P)) scan_walk_ker
         }
         const int64_t row = at.b * p.pieces * p.channels + d + j;
         store4(p.piece_end + (row + (piece + 1) * p.channels) * N, kS * q, N, h[j]);
-        if (q == 0) p.piece_step[(at.b * (p.pieces - 1) + piece) * p.channels + d + j] = j ? steps.y : steps.x;
+        if (q == 0) p.piece_step[(at.b * (p.pieces - 1) + piece) * p.channels + d + j] = steps[j];
         // the first state is kept with them: the second launch may overwrite state_in (state_out == state_in)
         if (piece == 0) store4(p.piece_end + row * N, kS * q, N, p.state_in ? load4(p.state_in + own, kS * q, N) : zero4());
     }
