@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, bwd_ctas(P)) scan_bwd_kernel
 #pragma unroll
                     for (int k = 0; k < kT; ++k, step += CH, bs += P) {
                         const float2 s = *step;
-                        av[k] = ex2(mul(s.x, wa[x]));
+                        av[k] = decays(s.x, wa[x]);
                         bv[k] = mul(s.y, f4(*bs));
                     }
 #pragma unroll
@@ -392,8 +392,8 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, bwd_ctas(P)) scan_bwd_kernel
                 const float4 sd = *reinterpret_cast<const float4 *>(step + t * CH);
                 const float2 rv = *reinterpret_cast<const float2 *>(rr + t * CH);
                 const F4 c = f4(cs[t * P]);
-                g[0] = mul(ex2(mul(sd.x, a2[0])), fma(rv.x, c, g[0]));
-                g[1] = mul(ex2(mul(sd.z, a2[1])), fma(rv.y, c, g[1]));
+                g[0] = mul(decays(sd.x, a2[0]), fma(rv.x, c, g[0]));
+                g[1] = mul(decays(sd.z, a2[1]), fma(rv.y, c, g[1]));
                 steps[0] += sd.x, steps[1] += sd.z;
             }
             __syncthreads();  // tile i is done, i + 1 is ready
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, bwd_ctas(P)) scan_bwd_kernel
                 const int t = m * kT + k;
                 const float4 sd = *reinterpret_cast<const float4 *>(step + t * CH);
                 const F4 b = f4(bs[t * P]);
-                av[k][0] = ex2(mul(sd.x, a2[0])), av[k][1] = ex2(mul(sd.z, a2[1]));
+                av[k][0] = decays(sd.x, a2[0]), av[k][1] = decays(sd.z, a2[1]);
                 hv[k][0] = fma(av[k][0], k ? hv[k ? k - 1 : 0][0] : h_in[0], mul(sd.y, b));
                 hv[k][1] = fma(av[k][1], k ? hv[k ? k - 1 : 0][1] : h_in[1], mul(sd.w, b));
             }
