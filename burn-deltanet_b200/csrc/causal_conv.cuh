@@ -14,7 +14,7 @@
 // The backward recomputes pre from x and carries the K unfinished sums of dx in registers the same way; its run ends
 // K - 1 tokens past its last.  x and dy come through a ring each, 24 tokens ahead, and tokens that lie in the middle of a
 // run are worked on eight at a time without questions about lengths and windows.  Ragged 6 x 2049 x 1536 bfloat16, forward
-// and backward: 61 us (71 with loads into registers), of which the backward is 36 and the sums of the CTAs' parts 5; no unit is
+// and backward: 59 us (71 with loads into registers), of which the backward is 36 and the sums of the CTAs' parts 3; no unit is
 // above half its rate there, the dependent instructions of few warps (128 registers each) are what is left.
 #pragma once
 
@@ -475,9 +475,7 @@ __global__ void __launch_bounds__(256) conv_bwd_sum_kernel(const float *part, in
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     const int j = blockIdx.y;
     float v = 0.f;
-    if (c < channels)
-#pragma unroll 8
-        for (int64_t i = down; i < ctas; i += 8) v += part[(i * (K + 1) + j) * channels + c];
+    if (c < channels) v = vec::sum_lines(part + j * channels + c, down, ctas, 8, (K + 1) * channels);
     sum[down][lane] = v;
     __syncthreads();
     if (down == 0 && c < channels) {

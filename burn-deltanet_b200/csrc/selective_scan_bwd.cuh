@@ -492,9 +492,7 @@ __global__ void __launch_bounds__(256) scan_bwd_bc_kernel(const float *part, int
     const int64_t in_row = i % row, t = i / row % seq, be = i / (row * seq), b = be / groups, e = be - b * groups;
     float v = 0.f;
     if (t < length_of(lengths, b, seq)) {
-        const float *src = part + (be * blocks * seq + t) * row + in_row;
-#pragma unroll 8
-        for (int64_t k = 0; k < blocks; ++k) v += src[k * seq * row];
+        v = vec::sum_lines(part + (be * blocks * seq + t) * row + in_row, 0, blocks, 1, seq * row);
     }
     const int64_t n = in_row % N;
     TI *o = (in_row >= N ? dc : db) + ((b * seq + t) * groups + e) * N + n;
@@ -506,13 +504,10 @@ __global__ void __launch_bounds__(256) scan_bwd_batch_kernel(const float *a_part
                                                              float *da, float *dd, float *dbias) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, na = channels * N;
     if (i < na) {
-        float v = 0.f;
-        for (int64_t b = 0; b < batch; ++b) v += a_part[b * na + i];
-        da[i] = v;
+        da[i] = vec::sum_lines(a_part + i, 0, batch, 1, na);
     } else if (i < na + 2 * channels) {
         const int64_t j = i - na;
-        float v = 0.f;
-        for (int64_t b = 0; b < batch; ++b) v += d_part[b * 2 * channels + j];
+        const float v = vec::sum_lines(d_part + j, 0, batch, 1, 2 * channels);
         if (j < channels) {
             if (dd) dd[j] = v;
         } else if (dbias) {

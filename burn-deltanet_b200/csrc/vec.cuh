@@ -33,6 +33,21 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
+// p[first * stride] + p[(first + step) * stride] + .. below `lines`, in order, eight loads under way together whatever their
+// number (an unrolled loop does its last few one by one: 2 us for the 50 lines of 6 x 2049 x 1536 in the convolution).
+__device__ __forceinline__ float sum_lines(const float *p, int64_t first, int64_t lines, int64_t step, int64_t stride) {
+    constexpr int kBatch = 8;
+    float v = 0.f;
+    for (int64_t i = first; i < lines; i += kBatch * step) {
+        float x[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) x[k] = i + k * step < lines ? p[(i + k * step) * stride] : 0.f;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) v += x[k];
+    }
+    return v;
+}
+
 
 // `n` of N elements from p (the others 0).  ALIGNED: p is aligned to the run's size (16 bytes at most) and n == N.
 template <bool ALIGNED, int N>
