@@ -12,7 +12,7 @@
 // row it reads anyway, so the forward saves nothing beside r.
 //
 // Measured: 32768 x 2048 bfloat16 88 us (6.1 TB/s), 16384 x 4096 with a float32 residual into e4m3 125 us (6.0 TB/s),
-// 16381 x 1560 with a float32 residual, forward and backward, 131 us (5.5 TB/s): 0.83 to 0.93 of a plain copy.
+// 16381 x 1560 with a float32 residual, forward and backward, 127 us (5.6 TB/s): 0.86 to 0.93 of a plain copy.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -470,9 +470,10 @@ __global__ void __launch_bounds__(512) rms_norm_bwd_kernel(const BwdParams p, in
 
 }  // namespace rms
 
-// out[c] = sum over i < lines of in[i * stride + c], c < cols, in a fixed order: 32 columns per CTA, eight threads
-// down each, then the eight sums in order.
-constexpr int kColThreads = 256, kColDown = kColThreads / 32;
+// out[c] = sum over i < lines of in[i * stride + c], c < cols, in a fixed order: 32 columns per CTA, 32 threads down each,
+// then their sums in order.  Narrow rows give few CTAs, so loads under way are what counts: 4 us less than with eight threads
+// down, at 296 lines of 1560 columns.
+constexpr int kColThreads = 1024, kColDown = kColThreads / 32;
 __global__ void __launch_bounds__(kColThreads) column_sum_kernel(const float *in, int64_t lines, int64_t stride, int64_t cols,
                                                                  float *out) {
     __shared__ float sum[kColDown][33];
