@@ -14,7 +14,7 @@ struct Layout {
 };
 
 // Pieces of the time axis: as many as the card has room for, 256 tokens each at least (1 x 4096 x 1024 x 16, forward and
-// backward: 233 us with nine of them, 773 us in one).
+// backward: 225 us with nine of them, 773 us in one).
 Layout layout_of(const dc_selective_scan_args *f) {
     constexpr int64_t kLeast = 256;
     const int lanes = sc::lanes_of(f->state);
