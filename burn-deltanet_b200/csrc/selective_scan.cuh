@@ -638,6 +638,8 @@ __global__ void __launch_bounds__(SegShape<P>::kNT, 512 / SegShape<P>::kNT) scan
         ptx::cp_async_wait<0>();
         __syncthreads();
         prepare(0, 0);
+    } else {
+        __syncthreads();  // every segment has read the state, which may be written below
     }
     int s = 0;
     for (int64_t t0 = 0; t0 < len; t0 += kTok, s ^= 1) {
@@ -715,7 +717,8 @@ __global__ void __launch_bounds__(kThreads) scan_step_kernel(const Params p) {
 #pragma unroll
     for (int k = 0; k < SEQS; ++k) {
         const int b = k < left ? k : left - 1;
-        h[k] = p.state_in ? load4_as<WHOLE>(p.state_in + row0 + b * row, kS * q, N) : zero4();
+        // (a thread behind the last channel leaves its states alone: their owner may be writing them)
+        h[k] = p.state_in && at < channels ? load4_as<WHOLE>(p.state_in + row0 + b * row, kS * q, N) : zero4();
         bv[k] = load4_as<WHOLE>(B + b * p.b_b, kS * q, N);
         cv[k] = load4_as<WHOLE>(C + b * p.c_b, kS * q, N);
     }
