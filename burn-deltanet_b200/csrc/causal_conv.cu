@@ -3,6 +3,7 @@
 #include "../../include/deltacore_layers.h"
 #include "causal_conv.cuh"
 #include "host.hpp"
+#include "rows.hpp"
 
 namespace {
 
@@ -10,11 +11,6 @@ using namespace dc::host;
 namespace cv = dc::conv;
 
 static_assert(DC_CONV_MAX_TAPS == cv::kMaxTaps, "the header's limit is the kernels'");
-
-// Elements from a tensor's first to its last, for the overlap checks.
-int64_t extent(int64_t batch, int64_t seq, int64_t channels, int64_t bs, int64_t ts) {
-    return (batch - 1) * bs + (seq - 1) * ts + channels;
-}
 
 bool valid_strides(int64_t batch, int64_t seq, int64_t channels, int64_t bs, int64_t ts) {
     return (seq <= 1 || ts >= channels) && (batch <= 1 || bs >= 0);
@@ -58,17 +54,10 @@ int validate_conv(const dc_causal_conv_args *a) {
         return DC_EINVAL_SHAPE;
     const int64_t wb = a->batch * a->channels * a->taps * 4;
     if (overlap(a->window_in, wb, a->window_out, wb) && !(a->seq == 1 && a->window_in == a->window_out)) return DC_EINVAL_ARG;
-    if (a->seq > 0 && overlap(a->x, extent(a->batch, a->seq, a->channels, a->x_batch_stride, a->x_token_stride) * is, a->y,
-                              extent(a->batch, a->seq, a->channels, a->y_batch_stride, a->y_token_stride) * os)) {
-        // slices of one buffer (the halves of a projection) interleave without touching: allowed when the token and
-        // batch strides are the same bytes and the rows stay apart
-        const int64_t xt = a->x_token_stride * is, yt = a->y_token_stride * os;
-        const int64_t off = static_cast<const char *>(a->y) - static_cast<const char *>(a->x);
-        const int64_t at = xt > 0 ? ((off % xt) + xt) % xt : 0;
-        const bool apart = a->seq > 1 && xt == yt && a->x_batch_stride * is == a->y_batch_stride * os &&
-                           (a->batch == 1 || (a->x_batch_stride * is) % xt == 0) && at >= a->channels * is && at + a->channels * os <= xt;
-        if (!apart) return DC_EINVAL_ARG;
-    }
+    const Rows x{a->x, a->batch, a->seq, a->x_batch_stride * is, a->x_token_stride * is, a->channels * is};
+    const Rows y{a->y, a->batch, a->seq, a->y_batch_stride * os, a->y_token_stride * os, a->channels * os};
+    if (rows_fold(y)) return DC_EINVAL_SHAPE;
+    if (rows_meet(x, y)) return DC_EINVAL_ARG;
     return DC_OK;
 }
 
@@ -131,9 +120,14 @@ int validate_bwd(const dc_causal_conv_bwd_args *a) {
         !valid_strides(a->batch, a->seq, a->channels, a->d_y_batch_stride, a->d_y_token_stride) ||
         !valid_strides(a->batch, a->seq, a->channels, a->d_x_batch_stride, a->d_x_token_stride))
         return DC_EINVAL_SHAPE;
+    const Rows x{a->x, a->batch, a->seq, a->x_batch_stride * is, a->x_token_stride * is, a->channels * is};
+    const Rows dy{a->d_y, a->batch, a->seq, a->d_y_batch_stride * os, a->d_y_token_stride * os, a->channels * os};
+    const Rows dx{a->d_x, a->batch, a->seq, a->d_x_batch_stride * is, a->d_x_token_stride * is, a->channels * is};
+    if (rows_fold(dx)) return DC_EINVAL_SHAPE;
     // a run's neighbour still reads what the run would overwrite
-    if (a->d_x && (a->d_x == a->x || a->d_x == a->d_y)) return DC_EINVAL_ARG;
-    if (a->d_window_in && a->d_window_in == a->d_window_out) return DC_EINVAL_ARG;
+    if (rows_meet(x, dx) || rows_meet(dy, dx)) return DC_EINVAL_ARG;
+    const int64_t wb = a->batch * a->channels * a->taps * 4;
+    if (overlap(a->d_window_in, wb, a->d_window_out, wb) || overlap(a->d_window_in, wb, a->window_in, wb)) return DC_EINVAL_ARG;
     return DC_OK;
 }
 

@@ -100,7 +100,8 @@ DC_API int dc_rms_norm_bwd(const dc_rms_norm_bwd_args *args, dc_stream_t stream)
  * b short, clamped to [0, seq]: x is not read past it and y is zero there.  window_out (or NULL) receives the
  * last `taps` columns of [window_in | x up to the length].  window_out may be window_in when seq == 1; they
  * must not overlap otherwise.  A decode step is seq = 1.  Token t of sequence b starts at b * batch_stride +
- * t * token_stride of its tensor; channels are contiguous.  y must not overlap x.  1 <= taps <=
+ * t * token_stride of its tensor; channels are contiguous.  y's rows must overlap neither x's nor one another
+ * (slices of one buffer that lie beside each other do not).  x may have a batch stride of 0.  1 <= taps <=
  * DC_CONV_MAX_TAPS; batch, seq and channels may be 0 (seq = 0 copies the window).
  */
 #define DC_CONV_SILU 0x1u
@@ -125,8 +126,9 @@ DC_API int dc_causal_conv(const dc_causal_conv_args *args, dc_stream_t stream);
 /*
  * The backward of dc_causal_conv, given d_y (out_dtype) and the gradient d_window_out of window_out (NULL:
  * zero): d_x in in_dtype (zero past a sequence's length), d_weight [channels, taps], d_bias [channels] (or NULL)
- * and d_window_in [batch, channels, taps] (or NULL) in float32.  Workspace: dc_causal_conv_bwd_workspace_size
- * bytes, 16-byte aligned.
+ * and d_window_in [batch, channels, taps] (or NULL) in float32.  d_x's rows must overlap neither x's nor d_y's nor one
+ * another, d_window_in neither d_window_out nor window_in.  Workspace: dc_causal_conv_bwd_workspace_size bytes, 16-byte
+ * aligned.
  */
 typedef struct dc_causal_conv_bwd_args {
     int64_t batch, seq, channels;
