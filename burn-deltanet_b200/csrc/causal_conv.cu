@@ -154,7 +154,7 @@ template <typename TI, typename TO, bool STAGED>
 int launch_bwd(const cv::BwdParams &p, dim3 grid, cudaStream_t s) {
     const size_t smem = STAGED ? sizeof(cv::BwdRings<TI, TO>) * (cv::kBwdThreads / 32) : 0;
     auto go = [&](auto *kernel) {
-        if (smem > 48 * 1024) {
+        if (smem + sizeof(float2) * cv::kBwdThreads > 48 * 1024) {  // with the kernel's sums, which lie beside the rings
             const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
             if (e != cudaSuccess) return cuda_fail(e);
         }
