@@ -22,6 +22,8 @@
 //     the work: nearly twice the exponentials, for sequences long enough and channels few enough.
 #pragma once
 
+#include <float.h>
+
 #include "common.cuh"
 #include "ptx.cuh"
 #include "vec.cuh"
@@ -99,6 +101,16 @@ __device__ __forceinline__ F4 ex2(F4 v) { return {make_float2(ex2(v.lo.x), ex2(v
 // that remembers many tokens multiplies that up: 2^-25 in the exponent takes it off, where the argument is small enough to
 // hold it.  (8 x 98 x 219 x 16 in float32, final state against 64 bits: 1.4e-6 without it, 5.6e-7 with.)  At step 0 it leaves 1.
 constexpr float kTilt = 1.f / (1 << 25);
+// a log2(e), held inside float32's range: a rate of -inf or near the lowest value, which switches a state off, would give -inf,
+// and a step of 0 (a token behind the end, or one whose softplus vanishes) times that NaN.  So the decay is 0 for every other
+// step and 1 for those.  NaN stays NaN.
+__device__ __forceinline__ float rate(float a) {
+    const float r = kLog2e * a;
+    return r < -FLT_MAX ? -FLT_MAX : r > FLT_MAX ? FLT_MAX : r;
+}
+__device__ __forceinline__ F4 rates(F4 a) {
+    return {make_float2(rate(a.lo.x), rate(a.lo.y)), make_float2(rate(a.hi.x), rate(a.hi.y))};
+}
 __device__ __forceinline__ F4 decays(float step, F4 a2) { return ex2(fma(step, a2, F4{both(kTilt), both(kTilt)})); }
 __device__ __forceinline__ float dot(F4 a, F4 b) {
     const float2 s = fma2(a.lo, b.lo, mul2(a.hi, b.hi));
@@ -518,7 +530,7 @@ __global__ void __launch_bounds__(WalkShape<P>::kNT, walk_ctas(P, sizeof(TI))) s
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         real[j] = ch + j < at.nch;
-        a2[j] = real[j] ? mul(kLog2e, load4(p.a + (d + j) * N, kS * q, N)) : zero4();
+        a2[j] = real[j] ? rates(load4(p.a + (d + j) * N, kS * q, N)) : zero4();
         h[j] = zero4();
         if (FULL && p.pieces > 1 && real[j]) {  // what the pieces before this one make of the first state
             const int64_t at_end = at.b * p.pieces * p.channels + d + j, at_step = at.b * (p.pieces - 1) * p.channels + d + j;
@@ -630,7 +642,7 @@ __global__ void __launch_bounds__(SegShape<P>::kNT, 512 / SegShape<P>::kNT) scan
     };
     const bool real = ch < at.nch;
     const int64_t d = at.d0 + (real ? ch : 0);
-    const F4 a2 = real ? mul(kLog2e, load4(p.a + d * N, kS * q, N)) : zero4();
+    const F4 a2 = real ? rates(load4(p.a + d * N, kS * q, N)) : zero4();
     F4 carry = p.state_in && real ? load4(p.state_in + (at.b * p.channels + d) * N, kS * q, N) : zero4();
     if (len > 0) {
         wk.template load<kNT, kTok, true>(sm.raw[0], 0, tid);
@@ -731,7 +743,7 @@ __global__ void __launch_bounds__(kThreads) scan_step_kernel(const Params p) {
         step[j] = ld(static_cast<const TI *>(p.dt) + b * p.dt_b + d);
         z[j] = p.z ? ld(static_cast<const TI *>(p.z) + b * p.z_b + d) : 0.f;
     }
-    const F4 a2 = mul(kLog2e, load4_as<WHOLE>(p.a + (int64_t)d * N, kS * q, N));
+    const F4 a2 = rates(load4_as<WHOLE>(p.a + (int64_t)d * N, kS * q, N));
     const float bias = p.dt_bias ? p.dt_bias[d] : 0.f, skip = p.d ? p.d[d] : 0.f;
 #pragma unroll
     for (int j = 0; j < kOwn; ++j) {

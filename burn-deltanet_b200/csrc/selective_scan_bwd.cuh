@@ -253,6 +253,8 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, bwd_ctas(P)) scan_bwd_kernel
                 vec::load<true>(sm.skip + oc, skip);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
+                    // where softplus has no slope left, rates at the end of the range may have taken their terms past it
+                    if (k.slope[j] == 0.f && !(fabsf(aw[j]) <= FLT_MAX)) aw[j] = 0.f;
                     du[j] = fmaf(gb[j], k.step[j], k.r[j] * skip[j]);
                     ds[j] = fmaf(gb[j], k.u[j], kLn2 * aw[j]) * k.slope[j];
                     dz[j] = fmaf(skip[j], k.u[j], y[j]) * k.dz[j];
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, bwd_ctas(P)) scan_bwd_kernel
         for (int x = 0; x < kWalks; ++x) {
             const int v = tid + x * S::kHelp, of = v % S::kMain, r = of % S::kSegT;
             wch[x] = v < 2 * S::kMain ? of / S::kSegT * S::kBlk + 2 * (r % S::kPairs) + v / S::kMain : CH, wq[x] = r / S::kPairs;
-            wa[x] = wch[x] < at.nch ? mul(kLog2e, load4(p.a + (at.d0 + wch[x]) * N, kS * wq[x], N)) : zero4();
+            wa[x] = wch[x] < at.nch ? rates(load4(p.a + (at.d0 + wch[x]) * N, kS * wq[x], N)) : zero4();
         }
         auto fetch = [&](int i) {  // the checkpoints of tile i
 #pragma unroll
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__(BwdShape<P>::kNT, bwd_ctas(P)) scan_bwd_kernel
     for (int j = 0; j < 2; ++j) {
         real[j] = ch + j < at.nch;
         const int64_t d = at.d0 + ch + j;
-        a2[j] = real[j] ? mul(kLog2e, load4(p.a + d * N, kS * q, N)) : zero4();
+        a2[j] = real[j] ? rates(load4(p.a + d * N, kS * q, N)) : zero4();
         g[j] = FULL && real[j] && bp.dstate_out ? load4(bp.dstate_out + (at.b * p.channels + d) * N, kS * q, N) : zero4();
         da[j] = zero4();
         if (FULL && real[j])

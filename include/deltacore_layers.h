@@ -160,6 +160,7 @@ DC_API int dc_causal_conv_bwd(const dc_causal_conv_bwd_args *args, dc_stream_t s
  *   step_t = softplus(dt[t, d] + dt_bias[d])                 (without DC_SCAN_SOFTPLUS: dt + dt_bias)
  *   h_n    = exp(step_t * a[d, n]) * h_n + step_t * u[t, d] * b[t, e, n]
  *   y[t,d] = (sum_n c[t, e, n] * h_n + d[d] * u[t, d]) * z[t, d] * sigma(z[t, d])
+ * exp(step_t * a) is 1 for a step of 0 whatever a is, -inf included (a state switched off: 0 for every other step).
  * dt_bias, d, z and state_in may be NULL (0, 0, no gate, 0).  u, dt, z, b and c share in_dtype; token t of
  * sequence s starts at s * batch_stride + t * token_stride of each tensor, with contiguous channels (u, dt, z,
  * y) or contiguous [groups, state] (b, c), so all of them may be column slices of projections.  lengths as in
