@@ -9,14 +9,17 @@ namespace sc = dc::scan;
 static_assert(DC_SCAN_MAX_STATE == 16 * sc::kS, "the header's limit is the kernels'");
 
 int validate_output(const dc_selective_scan_args *a, int64_t seq) {
-    const int64_t os = dtype_size(a->out_dtype), c = a->channels;
+    const int64_t os = dtype_size(a->out_dtype), c = a->channels, states = a->batch * c * a->state * 4;
+    // in place, or apart: a CTA that runs later would read what another one wrote
+    if (a->state_out != a->state_in && overlap(a->state_out, states, a->state_in, states)) return DC_EINVAL_ARG;
     if (seq == 0) return DC_OK;
     if (!a->y || !aligned(a->y, os)) return DC_EINVAL_ARG;
     if ((seq > 1 && a->y_token_stride < c) || (a->batch > 1 && a->y_batch_stride < c)) return DC_EINVAL_SHAPE;
-    // y over an input would be read by a CTA that runs later; interleaved slices of one buffer start elsewhere
-    const void *ins[] = {a->u, a->dt, a->z, a->b, a->c};
-    for (const void *q : ins)
-        if (q && q == a->y) return DC_EINVAL_ARG;
+    const Rows y{a->y, a->batch, seq, a->y_batch_stride * os, a->y_token_stride * os, c * os};
+    if (rows_fold(y)) return DC_EINVAL_SHAPE;
+    if (sc::meets_inputs(a, seq, y) || rows_meet(a->a, c * a->state * 4, y) || rows_meet(a->d, c * 4, y) || rows_meet(a->dt_bias, c * 4, y) ||
+        rows_meet(a->state_in, states, y) || rows_meet(a->state_out, states, y))
+        return DC_EINVAL_ARG;
     return DC_OK;
 }
 

@@ -60,10 +60,18 @@ int validate(const dc_selective_scan_bwd_args *a) {
         for (const void *i : ins)
             if (o && o == i) return DC_EINVAL_ARG;
     }
+    // of these, a CTA that runs later would read what another one wrote
+    const int64_t row = f->channels * is, states = f->batch * f->channels * f->state * 4, os = dtype_size(f->out_dtype);
+    const Rows dy{a->d_y, f->batch, f->seq, a->d_y_batch_stride * os, a->d_y_token_stride * os, f->channels * os};
+    for (const void *o : {a->d_u, a->d_dt, a->d_z}) {
+        const Rows out{o, f->batch, f->seq, f->seq * row, row, row};
+        if (sc::meets_inputs(f, f->seq, out) || rows_meet(dy, out)) return DC_EINVAL_ARG;
+    }
+    if (overlap(a->d_state_in, states, a->d_state_out, states)) return DC_EINVAL_ARG;
     const void *f32s[] = {a->d_a, a->d_d, a->d_dt_bias, a->d_state_in, a->d_state_out};
     for (const void *o : f32s)
         if (!aligned(o, 4)) return DC_EINVAL_ARG;
-    if (!aligned(a->d_y, dtype_size(f->out_dtype)) || (a->d_state_in && a->d_state_in == a->d_state_out)) return DC_EINVAL_ARG;
+    if (!aligned(a->d_y, os)) return DC_EINVAL_ARG;
     return DC_OK;
 }
 

@@ -4,6 +4,7 @@
 
 #include "../../include/deltacore_layers.h"
 #include "host.hpp"
+#include "rows.hpp"
 #include "selective_scan.cuh"
 
 namespace dc {
@@ -43,6 +44,19 @@ inline int validate_inputs(const dc_selective_scan_args *a, int64_t seq) {
     for (const auto &s : strides)
         if (s[2] && ((seq > 1 && s[1] < s[2]) || (seq > 0 && a->batch > 1 && s[0] < s[2]))) return DC_EINVAL_SHAPE;
     return DC_OK;
+}
+
+// Whether rows that a call writes meet what it reads token by token (with `seq` tokens).
+inline bool meets_inputs(const dc_selective_scan_args *a, int64_t seq, const host::Rows &out) {
+    const int64_t is = host::dtype_size(a->in_dtype), c = a->channels * is, n = a->groups * a->state * is;
+    const host::Rows ins[] = {{a->u, a->batch, seq, a->u_batch_stride * is, a->u_token_stride * is, c},
+                              {a->dt, a->batch, seq, a->dt_batch_stride * is, a->dt_token_stride * is, c},
+                              {a->z, a->batch, seq, a->z_batch_stride * is, a->z_token_stride * is, c},
+                              {a->b, a->batch, seq, a->b_batch_stride * is, a->b_token_stride * is, n},
+                              {a->c, a->batch, seq, a->c_batch_stride * is, a->c_token_stride * is, n}};
+    for (const host::Rows &in : ins)
+        if (host::rows_meet(in, out)) return true;
+    return false;
 }
 
 inline Params params_of(const dc_selective_scan_args *a) {

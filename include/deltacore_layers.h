@@ -165,7 +165,8 @@ DC_API int dc_causal_conv_bwd(const dc_causal_conv_bwd_args *args, dc_stream_t s
  * sequence s starts at s * batch_stride + t * token_stride of each tensor, with contiguous channels (u, dt, z,
  * y) or contiguous [groups, state] (b, c), so all of them may be column slices of projections.  lengths as in
  * dc_causal_conv: nothing is read past a sequence's length, y is zero there, and state_out [batch, channels,
- * state] is the state after its last token.  state_out may be state_in or NULL.  y must not overlap an input.
+ * state] is the state after its last token.  state_out may be state_in or NULL, and must not overlap it otherwise.
+ * y's rows must overlap neither an input's nor one another nor state_out (slices of one buffer beside each other do not).
  * checkpoints (or NULL) receives the states that dc_selective_scan_bwd starts from:
  * dc_selective_scan_checkpoint_size bytes.  1 <= state <= DC_SCAN_MAX_STATE; batch, seq and channels may be 0.
  *
@@ -212,7 +213,8 @@ DC_API int dc_selective_scan_step(const dc_selective_scan_args *args, dc_stream_
  * (fwd.out_dtype) and the gradient d_state_out of state_out (NULL: zero), writes every gradient that is not NULL:
  * d_u, d_dt, d_z [batch, seq, channels] and d_b, d_c [batch, seq, groups, state], contiguous, in fwd.in_dtype
  * (zero past a sequence's length); d_a [channels, state], d_d, d_dt_bias [channels] and d_state_in [batch,
- * channels, state] in float32.  d_u, d_dt, d_b, d_c and d_a are required, d_z when z is given.  Workspace:
+ * channels, state] in float32.  d_u, d_dt, d_b, d_c and d_a are required, d_z when z is given.  No gradient may overlap
+ * an input, nor d_state_in d_state_out.  Workspace:
  * dc_selective_scan_bwd_workspace_size bytes, 16-byte aligned.
  */
 typedef struct dc_selective_scan_bwd_args {

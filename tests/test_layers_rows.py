@@ -128,3 +128,73 @@ def test_conv_bwd_refuses_windows_over_windows():
     for buffer in (a.d_window_out, a.window_in):
         for at in (0, 16, -16, 2 * 32 * 4 * 4 - 4):
             assert abi.lib().dc_causal_conv_bwd(conv(True, d_window_in=buffer + at), None) == abi.DC_EINVAL_ARG
+
+
+def scan(**over):
+    """Inputs 1 MB apart; y, state_out and checkpoints behind them."""
+    a = abi.SelectiveScanArgs()
+    a.batch, a.seq, a.channels, a.state, a.groups = 2, 6, 32, 16, 2
+    for f, _ in a._fields_:
+        if f.endswith("_batch_stride"):
+            setattr(a, f, 192)
+        elif f.endswith("_token_stride"):
+            setattr(a, f, 32)
+    for i, f in enumerate(f for f, t in a._fields_ if t is ctypes.c_void_p and f not in ("lengths", "workspace")):
+        setattr(a, f, P + i * 0x100000)
+    for k, v in over.items():
+        setattr(a, k, v)
+    return a
+
+
+LAST = (192 + 5 * 32) * 4  # of a tensor's rows
+
+
+@pytest.mark.parametrize("name", ["u", "dt", "z", "b", "c"])
+def test_scan_refuses_outputs_over_inputs(name):
+    at = getattr(scan(), name)
+    for off in (0, 4, 124, -4, -124, LAST, LAST + 124):
+        assert abi.lib().dc_selective_scan(scan(y=at + off), None) == abi.DC_EINVAL_ARG
+    for off in (0, 4, 124, -124, 192 * 4 + 4):
+        assert abi.lib().dc_selective_scan_step(scan(seq=1, y=at + off), None) == abi.DC_EINVAL_ARG
+
+
+@pytest.mark.parametrize("name,size", [("a", 32 * 16 * 4), ("d", 128), ("dt_bias", 128), ("state_in", 2 * 32 * 16 * 4)])
+def test_scan_refuses_outputs_over_parameters_and_state(name, size):
+    at = getattr(scan(), name)
+    for off in (0, size - 4, -LAST - 124):
+        assert abi.lib().dc_selective_scan(scan(y=at + off), None) == abi.DC_EINVAL_ARG
+
+
+def test_scan_refuses_outputs_that_fold():
+    for over in (dict(y_batch_stride=160), dict(y_batch_stride=32), dict(y_batch_stride=191)):
+        assert abi.lib().dc_selective_scan(scan(**over), None) == abi.DC_EINVAL_SHAPE
+
+
+def test_scan_refuses_states_that_meet():
+    size = 2 * 32 * 16 * 4
+    for off in (4, -4, size - 4, 4 - size):  # (the very same buffer is in place)
+        for call, seq in ((abi.lib().dc_selective_scan, 6), (abi.lib().dc_selective_scan_step, 1)):
+            assert call(scan(seq=seq, state_out=scan().state_in + off), None) == abi.DC_EINVAL_ARG
+    assert abi.lib().dc_selective_scan(scan(state_out=scan().y + 64), None) == abi.DC_EINVAL_ARG
+
+
+def test_scan_bwd_refuses_outputs_over_inputs():
+    def call(**over):
+        w = abi.SelectiveScanBwdArgs()
+        w.fwd = scan()
+        w.d_y_batch_stride, w.d_y_token_stride = 192, 32
+        for i, f in enumerate(f for f, t in w._fields_ if t is ctypes.c_void_p):
+            setattr(w, f, P + 0x2000000 + i * 0x100000)
+        w.workspace_bytes = 1 << 24
+        d_y, d_state = w.d_y, w.d_state_out
+        for k, v in over.items():
+            setattr(w, k, v(w))
+        return abi.lib().dc_selective_scan_bwd(w, None)
+
+    for out in ("d_u", "d_dt", "d_z"):
+        for name in ("u", "dt", "z", "b", "c"):
+            for off in (0, 4, -4, LAST + 124):
+                assert call(**{out: lambda w: getattr(w.fwd, name) + off}) == abi.DC_EINVAL_ARG
+        assert call(**{out: lambda w: w.d_y + 64}) == abi.DC_EINVAL_ARG
+    for off in (0, 4, -4):
+        assert call(d_state_in=lambda w: w.d_state_out + off) == abi.DC_EINVAL_ARG
