@@ -4,6 +4,7 @@
 #include "../../include/deltacore_layers.h"
 #include "host.hpp"
 #include "rms_norm.cuh"
+#include "rows.hpp"
 
 namespace {
 
@@ -12,6 +13,8 @@ using namespace dc::host;
 constexpr int kThreads = 256, kMaxThreads = 512;
 
 bool valid_stride(int64_t stride, int64_t width, int64_t rows) { return rows <= 1 || stride >= width; }
+
+Rows rows_of(const void *p, int64_t rows, int64_t stride, int64_t width, int64_t elem) { return {p, 1, rows, 0, stride * elem, width * elem}; }
 
 // Whether every row of a tensor starts on a 16-byte boundary (8 for one-byte elements).
 bool rows_aligned(const void *p, int64_t stride, int64_t elem, int64_t rows) {
@@ -78,6 +81,20 @@ int validate_norm(const dc_rms_norm_args *a) {
         return DC_EINVAL_ARG;
     if (a->residual_out && a->residual_out == a->x && (a->residual_dtype != a->x_dtype || a->residual_out_stride != a->x_stride))
         return DC_EINVAL_ARG;
+    const int64_t xs = dtype_size(a->x_dtype), rs = res ? dtype_size(a->residual_dtype) : 0, ys = f8 ? 1 : dtype_size(a->out_dtype);
+    const Rows x = rows_of(a->x, a->rows, a->x_stride, a->width, xs), rin = rows_of(a->residual_in, a->rows, a->residual_in_stride, a->width, rs);
+    const Rows y = rows_of(a->y, a->rows, a->y_stride, a->width, ys), rout = rows_of(a->residual_out, a->rows, a->residual_out_stride, a->width, rs);
+    for (const Rows *out : {&y, &rout}) {
+        if (rows_meet(a->weight, a->width * 4, *out)) return DC_EINVAL_ARG;
+        for (const Rows *in : {&x, &rin})
+            if (out->p != in->p && rows_meet(*in, *out)) return DC_EINVAL_ARG;
+    }
+    if (rows_meet(y, rout)) return DC_EINVAL_ARG;
+    if (f8) {
+        const int64_t scales = a->rows * (a->group ? a->width / a->group : 1) * 4;
+        if (rows_meet(a->scale, scales, x) || rows_meet(a->scale, scales, rin) || rows_meet(a->scale, scales, y) || rows_meet(a->scale, scales, rout))
+            return DC_EINVAL_ARG;
+    }
     return DC_OK;
 }
 
@@ -125,6 +142,16 @@ int validate_norm_bwd_buffers(const dc_rms_norm_bwd_args *a) {
     if (a->d_residual && ((a->d_residual == a->d_r && a->d_residual_stride != a->d_r_stride) || a->d_residual == a->r ||
                           a->d_residual == a->d_y))
         return DC_EINVAL_ARG;
+    const int64_t w = a->width, xs = a->d_x ? dtype_size(a->x_dtype) : 0;
+    const Rows dy = rows_of(a->d_y, a->rows, a->d_y_stride, w, ys), dr = rows_of(a->d_r, a->rows, a->d_r_stride, w, rs);
+    const Rows r = rows_of(a->r, a->rows, a->r_stride, w, rs), dx = rows_of(a->d_x, a->rows, a->d_x_stride, w, xs);
+    const Rows dres = rows_of(a->d_residual, a->rows, a->d_residual_stride, w, rs);
+    for (const Rows *out : {&dx, &dres}) {
+        if (rows_meet(a->weight, w * 4, *out)) return DC_EINVAL_ARG;
+        for (const Rows *in : {&dy, &dr, &r})
+            if (out->p != in->p && rows_meet(*in, *out)) return DC_EINVAL_ARG;
+    }
+    if (rows_meet(dx, dres)) return DC_EINVAL_ARG;
     return DC_OK;
 }
 

@@ -45,7 +45,8 @@ extern "C" {
  *   scale = max|y| / 448 over the group (at least 2^-126; 1 where every y is 0 or NaN), float32,
  *   [rows, width / group] (or [rows, 1]).
  * A row that holds a NaN is NaN throughout.  Row i of a tensor starts at i * its stride, columns are
- * contiguous.  residual_out may be residual_in, and y may be x (same dtype and stride): in place.
+ * contiguous.  residual_out may be residual_in or x, and y may be x or residual_in (same dtype and stride): in place.
+ * Otherwise no output's rows may overlap another buffer's (columns or rows of one buffer beside each other do not).
  * rows may be 0.  1 <= width <= DC_RMS_MAX_WIDTH.
  */
 typedef struct dc_rms_norm_args {
@@ -70,7 +71,8 @@ DC_API int dc_rms_norm(const dc_rms_norm_args *args, dc_stream_t stream);
  *   d = inv * weight * d_y - r * inv^3 * mean(weight * d_y * r) + d_r
  *   d_x = d in x_dtype, d_residual = d in r_dtype (either may be NULL)
  *   d_weight = sum over rows of d_y * r * inv, float32 [width] (may be NULL)
- * d_residual may be d_r.  d_weight needs a workspace of dc_rms_norm_bwd_workspace_size bytes (16-byte aligned).
+ * d_residual may be d_r, and d_x may be d_y or d_r (same dtype and stride); otherwise neither may overlap another buffer.
+ * d_weight needs a workspace of dc_rms_norm_bwd_workspace_size bytes (16-byte aligned).
  */
 typedef struct dc_rms_norm_bwd_args {
     int64_t rows, width;

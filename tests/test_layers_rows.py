@@ -198,3 +198,52 @@ def test_scan_bwd_refuses_outputs_over_inputs():
         assert call(**{out: lambda w: w.d_y + 64}) == abi.DC_EINVAL_ARG
     for off in (0, 4, -4):
         assert call(d_state_in=lambda w: w.d_state_out + off) == abi.DC_EINVAL_ARG
+
+
+def norm(bwd=False, **over):
+    a = abi.RmsNormBwdArgs() if bwd else abi.RmsNormArgs()
+    a.rows, a.width, a.eps = 4, 128, 1e-5
+    for f, _ in a._fields_:
+        if f.endswith("_stride"):
+            setattr(a, f, 200)
+    for i, f in enumerate(f for f, t in a._fields_ if t is ctypes.c_void_p):
+        setattr(a, f, P + i * 0x100000)
+    if bwd:
+        a.workspace_bytes = 1 << 24
+    for k, v in over.items():
+        setattr(a, k, v)
+    return a
+
+
+END = (3 * 200 + 127) * 4  # a row buffer's last element
+
+
+@pytest.mark.parametrize("out", ["y", "residual_out"])
+def test_norm_refuses_outputs_that_meet_others(out):
+    others = ["x", "residual_in", "y" if out == "residual_out" else "residual_out"]
+    for other in others:
+        at = getattr(norm(), other)
+        for off in (4, -4, 127 * 4, -127 * 4, END, 200 * 4 + 4):
+            assert abi.lib().dc_rms_norm(norm(**{out: at + off}), None) == abi.DC_EINVAL_ARG
+        # a whole row further is no in-place call either
+        assert abi.lib().dc_rms_norm(norm(**{out: at + 800}), None) == abi.DC_EINVAL_ARG
+    at = norm().weight
+    for off in (0, 127 * 4, -END):
+        assert abi.lib().dc_rms_norm(norm(**{out: at + off}), None) == abi.DC_EINVAL_ARG
+
+
+def test_norm_refuses_scales_that_meet_others():
+    for other in ("x", "residual_in", "residual_out", "y"):
+        for off in (0, 4, 127 * 4 if other != "y" else 124):
+            a = norm(out_dtype=abi.DC_E4M3, group=32, scale=getattr(norm(), other) + off)
+            assert abi.lib().dc_rms_norm(a, None) == abi.DC_EINVAL_ARG
+
+
+@pytest.mark.parametrize("out", ["d_x", "d_residual"])
+def test_norm_bwd_refuses_outputs_that_meet_others(out):
+    for other in ("d_y", "d_r", "r", "d_residual" if out == "d_x" else "d_x"):
+        at = getattr(norm(True), other)
+        for off in (4, -4, 127 * 4, END, 800):
+            assert abi.lib().dc_rms_norm_bwd(norm(True, **{out: at + off}), None) == abi.DC_EINVAL_ARG
+    at = norm(True).weight
+    assert abi.lib().dc_rms_norm_bwd(norm(True, **{out: at + 4}), None) == abi.DC_EINVAL_ARG
