@@ -1,8 +1,8 @@
 // rms_norm.cuh — the residual stream's addition with the RMS norm of the sum, and its backward.
 //
 //   forward   s = x + residual;  y = s w / sqrt(mean(s^2) + eps);  optionally y as e4m3 with scales
-//   backward  with inv = 1 / sqrt(mean(r^2) + eps) of the stored sum r, and m = mean(w dy r):
-//             d = inv w dy - r inv^3 m + d_r,  d_w = sum over rows of dy r inv
+//   backward  with inv = 1 / sqrt(mean(r^2) + eps) of the stored sum r, and m = mean(w dy r inv):
+//             d = inv (w dy - r inv m) + d_r,  d_w = sum over rows of dy r inv
 //
 // HBM-bound: the forward reads x and the residual and writes the sum and y once, the backward reads dy, d_r and r
 // and writes d once; the row stays in registers between the reduction and its use.  A row is spread over TPR
@@ -314,7 +314,7 @@ __device__ __forceinline__ void bwd_row(const BwdParams &p, const float (&r)[VPT
     both = row_reduce<false>(both, tpr, red);
     const float inv_width = 1.f / (float)p.width;
     const float inv = 1.f / sqrtf(fmaf(both.x, inv_width, p.eps));
-    const float back = inv * inv * inv * (both.y * inv_width);
+    const float mean = both.y * inv_width * inv;  // of w dy r inv.  (Powers of inv would leave float32's range before inv does.)
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
         if (!on || n[i] <= 0) continue;
@@ -323,8 +323,9 @@ __device__ __forceinline__ void bwd_row(const BwdParams &p, const float (&r)[VPT
         weight(i, w);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-            dw[i][e] = fmaf(g[i][e], r[i][e] * inv, dw[i][e]);
-            d[e] += fmaf(inv * w[e], g[i][e], -r[i][e] * back);
+            const float unit = r[i][e] * inv;
+            dw[i][e] = fmaf(g[i][e], unit, dw[i][e]);
+            d[e] = fmaf(inv, fmaf(w[e], g[i][e], -unit * mean), d[e]);
         }
         if (p.dx) store_cols<LAY>(p.x_dt, p.dx, row * p.dx_stride, i, tx, tpr, d, n[i]);
         if (p.dres) store_cols<LAY>(p.r_dt, p.dres, row * p.dres_stride, i, tx, tpr, d, n[i]);
