@@ -100,8 +100,9 @@ struct LaunchStep {
         const int64_t blocks = ceil_div(p.channels, sc::kThreads / P), seqs = ceil_div(p.batch, sc::kStepSeqs);
         const bool many = blocks * seqs >= 2 * (int64_t)sm_count();
         const int64_t rows = many ? seqs : p.batch;
-        if (blocks > 0x7fffffff || rows > 65535) return DC_EUNSUPPORTED;
-        const dim3 grid((unsigned)blocks, (unsigned)rows);
+        if (blocks > 0x7fffffff) return DC_EUNSUPPORTED;
+        constexpr int64_t kRows = 65535;  // of a grid's second axis
+        const dim3 grid((unsigned)blocks, (unsigned)(rows < kRows ? rows : kRows), (unsigned)ceil_div(rows, kRows));
         // every group of four states whole and aligned
         const int64_t four = 4 * (int64_t)sizeof(TI);
         const bool whole = p.N == 4 * P && aligned(p.a, 16) && aligned(p.state_in, 16) && aligned(p.state_out, 16) && aligned(p.b, four) &&

@@ -721,7 +721,8 @@ __global__ void __launch_bounds__(kThreads) scan_step_kernel(const Params p) {
     const uint32_t at = blockIdx.x * (kThreads / P) + threadIdx.x / P, channels = (uint32_t)p.channels, d = at < channels ? at : channels - 1;
     const uint32_t e = p.groups == 1 ? 0 : d / (uint32_t)p.per;
     const int q = threadIdx.x % P, N = p.N;
-    const int64_t b0 = (int64_t)blockIdx.y * SEQS;
+    const int64_t b0 = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * SEQS;
+    if (b0 >= p.batch) return;  // the last layer of a grid of more rows than its second axis holds
     const int left = p.batch - b0 < SEQS ? (int)(p.batch - b0) : SEQS;  // sequences that exist; the last one stands in for the others
     const int64_t row0 = (b0 * channels + d) * N, row = (int64_t)channels * N;
     const TI *B = static_cast<const TI *>(p.b) + b0 * p.b_b + e * (uint32_t)N, *C = static_cast<const TI *>(p.c) + b0 * p.c_b + e * (uint32_t)N;

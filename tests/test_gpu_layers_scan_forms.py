@@ -123,3 +123,15 @@ def test_step_on_column_slices(batch, c, off, dtype):
     assert torch.equal(y, want[0]) and torch.equal(h, want[1])
     assert (out[:, :off] == 0).all() and (out[:, off + c:] == 0).all()
     check_step(t, (y, h), [0, 1, c // groups - 1], groups)
+
+
+@pytest.mark.parametrize("n,dtype", [(4, BF), (16, F32)])
+def test_step_of_very_many_sequences(n, dtype):
+    """More pairs of sequences than one axis of a grid holds."""
+    b, c = 140001, 12
+    t = inputs(b, 1, c, n, dtype=dtype, seed=n)
+    t = {k: v[:, 0] if k in ("u", "dt", "b", "c", "z") else v for k, v in t.items()}
+    y, h = dn.selective_scan_step(*(t[k] for k in NAMES))
+    for part in (slice(0, 300), slice(130900, 131300), slice(139800, None)):
+        cut = {k: v if k in ("a", "d", "dt_bias") else v[part] for k, v in t.items()}
+        check_step(cut, (y[part], h[part]), range(c), 1)
