@@ -21,6 +21,9 @@ import torch
 from . import _abi
 from .core import DeltaCoreError, DeltaShapeError, _raise
 
+# Counts a buffer of the caller's that a call wrote as changed, so that autograd refuses a backward which saved its old values.
+_wrote = torch.autograd.graph.increment_version
+
 _CODES = {torch.float32: _abi.DC_F32, torch.bfloat16: _abi.DC_BF16}
 
 
@@ -221,6 +224,10 @@ def _norm(x, weight, residual, eps, out_dtype, residual_dtype, y_out, residual_o
     if residual is not None:
         a.residual_in = residual.data_ptr()
     _call(_abi.lib().dc_rms_norm, a, dev, "dc_rms_norm")
+    if y_out is not None:
+        _wrote(y_out)
+    if residual_out is not None:
+        _wrote(residual_out)
     return y, scale, r
 
 
@@ -367,9 +374,18 @@ def _conv(x, weight, bias, window, silu, lengths, out_dtype, y_out, window_out, 
     nxt = window_out
     if nxt is None:
         nxt = torch.empty((a.batch, a.channels, a.taps), device=dev, dtype=torch.float32) if window is None else _new(window, torch.float32)
-    a.x, a.weight, a.bias, a.window_in, a.lengths = x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(window), _ptr(lengths)
-    a.y, a.window_out = y.data_ptr(), nxt.data_ptr()
+    a.x, a.weight, a.y, a.window_out = x.data_ptr(), weight.data_ptr(), y.data_ptr(), nxt.data_ptr()
+    if bias is not None:
+        a.bias = bias.data_ptr()
+    if window is not None:
+        a.window_in = window.data_ptr()
+    if lengths is not None:
+        a.lengths = lengths.data_ptr()
     _call(_abi.lib().dc_causal_conv, a, dev, "dc_causal_conv")
+    if y_out is not None:
+        _wrote(y_out)
+    if window_out is not None:
+        _wrote(window_out)
     return y, nxt
 
 
@@ -534,13 +550,26 @@ def _scan(u, dt, a, b, c, d, z, dt_bias, state, softplus, lengths, out_dtype, y_
     else:
         keep = _workspace(need, g, workspace, dev)
         _call(_abi.lib().dc_selective_scan, g, dev, "dc_selective_scan")
+    if y_out is not None:
+        _wrote(y_out)
+    if state_out is not None:
+        _wrote(state_out)
     del keep
     return y, h, saved
 
 
 def _scan_inputs(g, u, dt, a, b, c, d, z, dt_bias, state, lengths):
     g.u, g.dt, g.a, g.b, g.c = u.data_ptr(), dt.data_ptr(), a.data_ptr(), b.data_ptr(), c.data_ptr()
-    g.d, g.z, g.dt_bias, g.state_in, g.lengths = _ptr(d), _ptr(z), _ptr(dt_bias), _ptr(state), _ptr(lengths)
+    if d is not None:
+        g.d = d.data_ptr()
+    if z is not None:
+        g.z = z.data_ptr()
+    if dt_bias is not None:
+        g.dt_bias = dt_bias.data_ptr()
+    if state is not None:
+        g.state_in = state.data_ptr()
+    if lengths is not None:
+        g.lengths = lengths.data_ptr()
 
 
 def selective_scan(u: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, d: Optional[torch.Tensor] = None,
