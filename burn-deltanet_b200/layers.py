@@ -4,7 +4,8 @@
   norm of the sum, in float32 / bfloat16 or in 8 bits (e4m3) with scales;
 * :func:`causal_conv`, :func:`causal_conv_step`, :func:`causal_conv_backward` — the short causal depthwise convolution;
 * :func:`selective_scan`, :func:`selective_scan_step`, :func:`selective_scan_backward` — the selective state space scan;
-* :class:`AddRmsNormFunction`, :class:`CausalConvFunction`, :class:`SelectiveScanFunction` — their autograd nodes.
+* :class:`AddRmsNormFunction`, :class:`CausalConvFunction`, :class:`SelectiveScanFunction` — their autograd nodes, once
+  differentiable (a second derivative is an error).  The functions above are no nodes: their outputs carry no gradient.
 
 They have no counterpart in burn-deltanet (the norm in front of a block is a Burn module there, and the selective scan is the
 diagonal relative of the delta rule that hybrid stacks interleave with it).  The manner is :mod:`.core`'s: CUDA tensors only,
@@ -14,6 +15,7 @@ axis contiguous, one stride per token.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -156,6 +158,40 @@ def _new(like: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     if like.dtype == dtype and like.is_contiguous():
         return torch.empty_like(like)
     return torch.empty(like.shape, device=like.device, dtype=dtype)
+
+
+class _Gradients(torch.autograd.Function):
+    """`count` gradients as they are, depending on the tensors behind them; to differentiate them is an error."""
+
+    @staticmethod
+    def forward(ctx, count, *tensors):
+        return tuple(t.detach() for t in tensors[:count])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("this operator can be differentiated once: its backward has no derivative")
+
+
+def _once(backward):
+    """A node's backward whose gradients refuse a second derivative, also where only a part of it would pass through them (torch's
+    own once_differentiable leaves that part out where the derivative is asked for by torch.autograd.grad)."""
+
+    @functools.wraps(backward)
+    def once(ctx, *d_outputs):
+        with torch.no_grad():
+            grads = backward(ctx, *d_outputs)
+        if not torch.is_grad_enabled():
+            return grads
+        behind = [t for t in (*d_outputs, *ctx.saved_tensors) if t is not None and t.requires_grad]
+        given = [i for i, g in enumerate(grads) if g is not None]
+        if not behind:
+            return grads
+        grads = list(grads)
+        for i, g in zip(given, _Gradients.apply(len(given), *(grads[i] for i in given), *behind)):
+            grads[i] = g
+        return tuple(grads)
+
+    return once
 
 
 # ------------------------------------------------------------------------------------------------ residual add + norm
@@ -316,6 +352,7 @@ class AddRmsNormFunction(torch.autograd.Function):
         return y if residual is None else (y, r)
 
     @staticmethod
+    @_once
     def backward(ctx, d_y, d_r=None):
         r, weight = ctx.saved_tensors
         eps, x_dtype, has_residual = ctx.cfg
@@ -458,6 +495,7 @@ class CausalConvFunction(torch.autograd.Function):
         return y, nxt
 
     @staticmethod
+    @_once
     def backward(ctx, d_y, d_next):
         x, weight, bias, window, lengths = ctx.saved_tensors
         d_x, d_weight, d_bias, d_window = causal_conv_backward(d_y.contiguous(), d_next.contiguous(), x, weight, bias, window,
@@ -665,6 +703,7 @@ class SelectiveScanFunction(torch.autograd.Function):
         return y, h
 
     @staticmethod
+    @_once
     def backward(ctx, d_y, d_h):
         *args, lengths, saved = ctx.saved_tensors
         grads = selective_scan_backward(d_y.contiguous(), d_h.contiguous(), *args, softplus=ctx.softplus, lengths=lengths, checkpoints=saved)

@@ -1,5 +1,5 @@
 """What autograd knows of the block-level operators on the GPU: buffers that a call writes count as changed, so that a backward
-which still needs their old values is refused."""
+which still needs their old values is refused, and a second derivative is refused, not left out."""
 import importlib
 
 import pytest
@@ -77,3 +77,23 @@ def test_in_inference_mode():
         got = dn.selective_scan_step(*one(args), state_out=args[-1])
         assert torch.equal(got[0], want[0]) and torch.equal(args[-1], want[1])
     dn.selective_scan_step(*one([t.clone() for t in args[:-1]]), args[-1], state_out=args[-1])
+
+
+def test_a_second_derivative_is_refused():
+    """By backward and by torch.autograd.grad, also where another part of it exists; the first derivative is there."""
+    x, w, res = rand(4, 64, grad=True), rand(64, seed=1, grad=True), rand(4, 64, seed=2, grad=True)
+    cx, cw = rand(2, 6, 8, grad=True), rand(8, 4, seed=1, grad=True)
+    for apply, arg in ((lambda: dn.AddRmsNormFunction.apply(x, w, res)[0], x), (lambda: dn.AddRmsNormFunction.apply(x, w), x),
+                       (lambda: dn.AddRmsNormFunction.apply(x, w, res)[1] + dn.AddRmsNormFunction.apply(x, w), w),
+                       (lambda: dn.CausalConvFunction.apply(cx, cw)[0], cx), (lambda: dn.CausalConvFunction.apply(cx, cw)[1], cw),
+                       (lambda: dn.SelectiveScanFunction.apply(*([cx] + [t.detach() for t in scan_args()[1:]]))[0], cx)):
+        for head in (lambda y: y.square().sum(), lambda y: y.sum()):
+            plain, = torch.autograd.grad(head(apply()), arg)
+            grad, = torch.autograd.grad(head(apply()), arg, create_graph=True)
+            assert torch.equal(grad.detach(), plain)
+            with pytest.raises(RuntimeError, match="differentiated once"):
+                torch.autograd.grad((grad * arg).sum(), arg)
+            grad, = torch.autograd.grad(head(apply()), arg, create_graph=True)
+            with pytest.raises(RuntimeError, match="differentiated once"):
+                (grad.square().sum() + arg.sum()).backward()
+        x.grad = w.grad = res.grad = cx.grad = cw.grad = None
