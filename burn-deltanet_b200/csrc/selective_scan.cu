@@ -37,7 +37,7 @@ struct Cut {
 // So: the walk from a third of the room on; below that as many pieces as fill the room, each 128 tokens at least, if
 // that makes three or more of them; else segments.
 Cut cut_of(const dc_selective_scan_args *a, bool workspace) {
-    constexpr int64_t kLeast = 128;  // a multiple of every checkpoint's distance
+    constexpr int64_t kLeast = 128;
     const int lanes = sc::lanes_of(a->state);
     const int64_t ctas = a->batch * a->groups * ceil_div(a->channels / a->groups, sc::walk_channels(lanes));
     const int64_t room = (int64_t)sm_count() * sc::walk_ctas(lanes, dtype_size(a->in_dtype));
@@ -45,7 +45,7 @@ Cut cut_of(const dc_selective_scan_args *a, bool workspace) {
     if (3 * ctas > room) return c;
     const int64_t want = room / ctas, most = a->seq / kLeast, pieces = want < most ? want : most;
     if (workspace && pieces >= 3) {
-        c.piece = ceil_div(ceil_div(a->seq, pieces), kLeast) * kLeast;
+        c.piece = ceil_div(ceil_div(a->seq, pieces), sc::kTile) * sc::kTile;  // (still three or more: seq >= 3 kLeast)
         c.pieces = ceil_div(a->seq, c.piece);
     } else {
         c.segments = true;

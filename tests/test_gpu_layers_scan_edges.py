@@ -89,3 +89,21 @@ def test_a_nan_rate_is_not_hidden():
     t["a"][3, 2] = float("nan")
     y, h = dn.selective_scan(*(t[k] for k in NAMES))
     assert torch.isnan(y[:, :, 3]).all() and torch.isnan(h[:, 3, 2]).all() and torch.isfinite(y[:, :, :3]).all()
+
+
+@pytest.mark.parametrize("s", [384, 385, 400, 511, 513, 1023, 1025])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_lengths_around_the_pieces(s, dtype):
+    """Pieces of 128 to 192 tokens, the last one short; checkpoints in each of them."""
+    t = inputs(2, s, 24, 16, dtype=dtype, seed=s)
+    lens = [s, s // 3 + 1]
+    y, h, saved = dn.selective_scan(*(t[k] for k in NAMES), lengths=int32(lens), checkpoints=True)
+    x = clean(t, lens)
+    ry, rh, before, _ = ol.selective_scan(**x, lengths=lens, keep=True)
+    sy, sh, size, _ = ol.selective_scan(**magnitudes(x), lengths=lens, keep=True)
+    close("y", y, ry, np.abs(sy), 3e-7 * s + 4e-6)
+    close("state", h, rh, np.abs(sh), 3e-7 * s + 4e-6)
+    saved = saved.view(2, -(-s // 16), 24, 16)
+    for b, n in enumerate(lens):
+        for i in range(-(-n // 16)):
+            close("checkpoint", saved[b, i], before[16 * i][b], np.abs(size[16 * i][b]), 3e-7 * s + 4e-6)
