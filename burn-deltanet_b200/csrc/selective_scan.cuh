@@ -117,7 +117,6 @@ __device__ __forceinline__ float dot(F4 a, F4 b) {
     return s.x + s.y;
 }
 __device__ __forceinline__ F4 zero4() { return {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}; }
-__device__ __forceinline__ F4 one4() { return {make_float2(1.f, 1.f), make_float2(1.f, 1.f)}; }
 
 // four values in shared memory
 template <typename T>

@@ -149,12 +149,8 @@ __device__ __forceinline__ void load_raw(const T *p, Raw<T, N> &r, int n) {
             const uint4 v = reinterpret_cast<const uint4 *>(p)[i / 4];
             r.w[i] = v.x, r.w[i + 1] = v.y, r.w[i + 2] = v.z, r.w[i + 3] = v.w;
         }
-    } else if constexpr (ALIGNED && kWords == 2) {
-        const uint2 v = *reinterpret_cast<const uint2 *>(p);
-        r.w[0] = v.x, r.w[1] = v.y;
-    } else if constexpr (ALIGNED && kWords == 1) {
-        r.w[0] = *reinterpret_cast<const uint32_t *>(p);
     } else {
+        static_assert(!ALIGNED, "aligned runs are whole 16-byte accesses");
         T v[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
