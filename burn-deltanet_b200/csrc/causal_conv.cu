@@ -30,9 +30,10 @@ bool vectors(const void *p, int64_t bs, int64_t ts, int64_t elem, int64_t n) {
     return aligned(p, (size_t)(elem * n)) && bs % n == 0 && ts % n == 0;
 }
 
-// Tokens per thread: as many as leave 24 warps for every SM, between `least` and `most`.  Each run reads K - 1 tokens of
-// its neighbour again (5 % at 64 tokens and 4 taps); ragged 6 x 2049 x 1536 takes 19 us at 24 warps and 23 at
-// 16; at 48 the runs of the backward get too short.
+// Tokens per thread: halved from `most` until there are 24 warps for every SM, or `least` is reached.  Each run reads K - 1
+// tokens of its neighbour again (5 % at 64 tokens and 4 taps).  24 is what the forward holds on an SM (the backward holds 16);
+// halving may give up to twice that.  Chosen at one shape: ragged 6 x 2049 x 1536 forward takes 19 us at 24 warps, 23 at 16; with
+// 48 the runs of its backward get too short.
 int run_length(int64_t batch, int64_t seq, int64_t groups, int least, int most) {
     int run = most;
     while (run > least && batch * ceil_div(seq, run) * groups < (int64_t)sm_count() * 24) run /= 2;

@@ -9,13 +9,15 @@
 // tokens before its run.  Where rows start on 16-byte boundaries each warp stages its 64 channels' tokens through a ring of
 // its own in shared memory (asynchronous copies, 48 tokens ahead, no barrier beyond the warp), so that the bytes in flight
 // do not depend on registers; loads into registers, eight tokens at a time, took 69 us at 8 x 4096 x 2048 bfloat16 where this
-// takes 62 (4.3 TB/s; the exponentials and reciprocals are next, at about half their rate).
+// takes 62 (4.3 TB/s).  No unit is full there (HBM 0.66, the special-function unit and the issue slots about half): 2048 CTAs
+// make 2.3 waves of the 888 that the card holds, and each warp fills its ring anew for its run.
 //
 // The backward recomputes pre from x and carries the K unfinished sums of dx in registers the same way; its run ends
 // K - 1 tokens past its last.  x and dy come through a ring each, 24 tokens ahead, and tokens that lie in the middle of a
 // run are worked on eight at a time without questions about lengths and windows.  Ragged 6 x 2049 x 1536 bfloat16, forward
 // and backward: 59 us (71 with loads into registers), of which the backward is 36 and the sums of the CTAs' parts 3; no unit is
-// above half its rate there, the dependent instructions of few warps (128 registers each) are what is left.
+// above half its rate there: 128 registers allow 16 warps an SM, whose dependent instructions show, and 1200 CTAs are two
+// waves of 592 and a remnant.
 #pragma once
 
 #include "common.cuh"
@@ -48,7 +50,8 @@ struct Params {
     float *window_out;
 };
 
-// sigma(x) from the fast exponential and reciprocal (x -> -inf gives 0): a few ulp
+// sigma(x) from the fast exponential and reciprocal (x -> -inf gives 0): 3 ulp and, from the rounding of the exponential's
+// argument, about 1.2 more per unit of |x|
 __device__ __forceinline__ float sigmoid(float x) {
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * x));

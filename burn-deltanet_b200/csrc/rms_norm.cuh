@@ -110,7 +110,8 @@ __device__ __forceinline__ float row_reduce(float v, int tpr, float2 *red) {
     return v;
 }
 
-// e4m3 values of v[i] * inv in one 8-byte word
+// e4m3 values of v[i] * inv in one 8-byte word.  With inv = 1 / scale this is the quotient to about 2^-22 before its rounding to
+// e4m3: next to a tie the other neighbour may come out.
 __device__ __forceinline__ uint2 to_e4m3(const float (&v)[kVec], float inv) {
     uint32_t w[2];
 #pragma unroll

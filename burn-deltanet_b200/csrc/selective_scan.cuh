@@ -410,8 +410,8 @@ struct Stager {
 // where the threads would be too many for their registers).  kHelp further threads stage the tiles, take the steps of the
 // next tile and write y of the last one, so that the two kinds of work, each a chain of dependent instructions, fill each
 // other's gaps; one barrier per tile of 16 tokens.  8 x 4096 x 2048 x 16 bfloat16 takes 463 us: the special-function unit,
-// the issue slots and the shared memory's data path are each at 0.63 of their rate there (294 us for the first alone), and
-// what shortens one lengthens another: exponentials taken ahead of their use 495 us, b and c read as bfloat16 and widened by
+// the issue slots and the shared memory's data path are at 0.64, 0.65 and 0.72 of their rates there (294 us for the first
+// alone), and what shortens one lengthens another: exponentials taken ahead of their use 495 us, b and c read as bfloat16 and widened by
 // the reader 498, steps stored twice to spare the moves of two-wide arithmetic 596.  5 x 777 x 1000 x 24 float32 in 2 groups:
 // 69 us, the longest sequence's chain of dependent instructions, 0.09 us a token.
 // FULL: the whole scan; else only the piece's end state from zero and its sum of steps.
@@ -710,8 +710,11 @@ __device__ __forceinline__ F4 load4_as(const T *row, int n, int N) {
 
 // Four states of one channel per thread, for SEQS sequences, whose states are all under way together; HBM-bound (the state
 // read and written once, 8 bytes per state, against 4 elements per channel).  A channel's P threads share out what is per
-// sequence: the step, the gate and the output.  256 x 2048 x 16 in place: 15 us (4.8 TB/s), 19 with four sequences, whose
-// registers halve the threads on an SM, and 26 with one and nothing shared.
+// sequence: the step, the gate and the output.  256 x 2048 x 16 in place takes 17.7 us with states that come from memory, as a
+// model's layers find them (4.0 TB/s), and 13.6 with the same states again and again, which stay in L2.  Short CTAs that load,
+// wait and compute hold it below the memory's rate.  One, two and four sequences per thread, from memory, bfloat16:
+//   256 x 2048 x 16: 18.8, 17.7, 15.0 us      256 x 2048 x 8: 11.7, 11.2, 11.7      128 x 2048 x 64: 34.5, 28.1, 29.7
+// Two is the fastest at 8 and at 64 states, four at 16.
 constexpr int kStepSeqs = 2;
 template <typename TI, int P, int SEQS, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) scan_step_kernel(const Params p) {

@@ -13,7 +13,7 @@
 // tile, so that the walk back, the longest chain, waits for nothing: one barrier per tile.  This takes 1.75 exponentials
 // per token and state; the other way, segments of threads that run their tokens from zero and exchange, takes one but twice
 // the shared memory traffic.  4 x 2048 x 2048 x 16 bfloat16 with the forward: 620 us, of which this kernel is about 440, with
-// the shared memory at 67 % of its peak and the issue slots at 47 %; 690 us the other way.
+// the shared memory at 62 % of its peak and the issue slots at 47 %; 690 us the other way.
 //
 // With few channels the time axis is cut into pieces, as in the forward: a first launch walks back through each piece but
 // the first from zero, for the gradient that leaves it and its sum of steps, and the second starts each piece from what the

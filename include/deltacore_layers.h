@@ -41,7 +41,8 @@ extern "C" {
  *   residual_out = s rounded to residual_dtype (not written when NULL);
  *   y = s / sqrt(mean(s^2) + eps) * weight (of the unrounded s), in out_dtype.
  * With out_dtype DC_E4M3, y is divided by a scale per `group` consecutive columns (group 32, 64, 128 or 256
- * dividing width; 0: one scale per row) and rounded to the nearest e4m3 value:
+ * dividing width; 0: one scale per row) and rounded to the nearest e4m3 value (the quotient is taken in float32 to about
+ * 2^-22, so that a value within that of a tie may go either way):
  *   scale = max|y| / 448 over the group (at least 2^-126; 1 where every y is 0 or NaN), float32,
  *   [rows, width / group] (or [rows, 1]).
  * A row that holds a NaN is NaN throughout.  Row i of a tensor starts at i * its stride, columns are
@@ -104,7 +105,7 @@ DC_API int dc_rms_norm_bwd(const dc_rms_norm_bwd_args *args, dc_stream_t stream)
  * must not overlap otherwise.  A decode step is seq = 1.  Token t of sequence b starts at b * batch_stride +
  * t * token_stride of its tensor; channels are contiguous.  y's rows must overlap neither x's nor one another
  * (slices of one buffer that lie beside each other do not).  x may have a batch stride of 0.  1 <= taps <=
- * DC_CONV_MAX_TAPS; batch, seq and channels may be 0 (seq = 0 copies the window).
+ * DC_CONV_MAX_TAPS; up to 65535 * 32 channels; batch, seq and channels may be 0 (seq = 0 copies the window).
  */
 #define DC_CONV_SILU 0x1u
 
