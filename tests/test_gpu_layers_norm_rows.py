@@ -1,5 +1,5 @@
 """The residual add + RMS norm on the GPU with more rows than the card holds at once, so that CTAs go on to further rows with the
-next row's loads under way and the last round is partly empty; and rows far from 1 in size.
+next row's loads under way and the last pass is partly empty; and rows far from 1 in size.
 
 Tolerances are test_gpu_layers_norm's.  The longest chain of additions behind a row's mean is 32 values of a thread, 5 shuffles
 and the 15 other warps of the widest rows: 52 roundings of 2^-24, halved by the root, and four more make 1.8e-6 of REL's 4e-6."""
